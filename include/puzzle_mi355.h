@@ -541,6 +541,60 @@ int pz_embed_fwd(const int32_t *words, const float *vocab, float *out, size_t to
 int pz_embed_bwd_params(const int32_t *words, const float *grad, float *vocab, float scale, size_t tokens, int embsize,
                         pz_stream_t stream);
 
+/* ---- operators over rows of channels (tokens, or the pixels of a channels-last map): the feed-forward block
+ *      x + dropout(act2(W2 act1(W1 norm(x) + b1) + b2)) in three operators. Tensors are float32 or float16 (`dtype`); sums, statistics,
+ *      bias, scale and their gradients are float32. Row pitches are in elements.                                                       */
+enum { PZ_F32 = 0, PZ_F16 = 1 };
+enum { PZ_ACT_NONE = 0, PZ_ACT_RELU = 1, PZ_ACT_GELU = 2, PZ_ACT_SILU = 3 };
+
+/* A dropout mask by its key: element i (in row-major order of the tensor) is kept where word i of call `call` of the generator `seed`
+ * — exactly the word pz_rng_fill_u32 would have written — is below `threshold`; kept elements are divided by `keep`, dropped ones are
+ * zero whatever they hold. The same key gives the same mask forward and backward; nothing is stored.                                  */
+typedef struct pz_dropout_mask {
+	uint64_t seed, call;
+	uint32_t threshold;
+	float keep;
+} pz_dropout_mask;
+/* takes the next call number of the generator, as one fill would: *seed, *call name a mask nobody else gets */
+int pz_rng_reserve(pz_rng_t rng, uint64_t *seed, uint64_t *call);
+/* y = residual + dropout(x) over `count` elements (residual may be NULL; y may be x or residual); its own backward pass with dy for x.
+ * Beside PZ_OP_DROPOUT (Cuda/Kernels/ElementWise.py:495-536), whose words come from memory. */
+int pz_dropout(int dtype, const void *x, const void *residual, void *y, size_t count, const pz_dropout_mask *mask, pz_stream_t stream);
+
+/* y[m][n] = residual + dropout(act(x[m][k] W + b)); W is [k][n], or [n][k] with trans_w. mask, bias, residual, preact may be NULL;
+ * preact receives x W + b, which the backward pass of an activation needs. y may be residual, nothing else may overlap.
+ * The backward pass: dz = act'(preact) * dropout(dy); dx = dz W^T; dW <- beta dW + alpha x^T dz (Modules/Linear.py:44-54's contract,
+ * float32 or the operands' type); db <- beta db + alpha * column sums of dz. NULL outputs are not computed; the residual's gradient is
+ * dy itself. In float16 dz is rounded to float16 in front of the two products (the matrix pipe's operand type).                       */
+typedef struct pz_linear_desc {
+	int dtype, act, trans_w;
+	int m, n, k;
+	int64_t ldx, ldw, ldy;          /* x, W, y (backward: x, W, dy) */
+	int64_t ldr, ldp;               /* residual (backward: dx), preact */
+} pz_linear_desc;
+int pz_linear_fwd_workspace_bytes(const pz_linear_desc *d, const void *x, const void *w, size_t *nbytes);
+int pz_linear_fwd(const pz_linear_desc *d, const void *x, const void *w, const float *bias, const void *residual, const pz_dropout_mask *mask,
+                  void *y, void *preact, void *workspace, size_t ws_bytes, pz_stream_t stream);
+int pz_linear_bwd_workspace_bytes(const pz_linear_desc *d, const void *dy, const void *x, const void *w, int dropping, int want_dx, int want_dw,
+                                  int want_db, size_t *nbytes);
+int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const void *w, const void *preact, const pz_dropout_mask *mask,
+                  void *dx, void *dw, int dw_dtype, float *db, float alpha, float beta, void *workspace, size_t ws_bytes, pz_stream_t stream);
+
+/* Group normalisation with an activation, channels last: x is (n, pixels, c), the c channels form `groups` groups of c / groups, and
+ * y = act(scale[c] * (x - mean) * invvar + bias[c]) with mean and invvar = 1 / sqrt(var + epsilon) over the pixels and channels of a
+ * group of a sample (biased variance). scale / bias may be NULL (1 / 0). savemean, saveinvvar: (n, groups), may be NULL in the forward
+ * pass. The backward pass recomputes the normalised value from x and the saved pair; dscale, dbias may be NULL.                       */
+typedef struct pz_groupnorm_desc {
+	int dtype, act;
+	int n, pixels, c, groups;
+	float epsilon;
+} pz_groupnorm_desc;
+int pz_groupnorm_workspace_bytes(const pz_groupnorm_desc *d, int backward, size_t *nbytes);
+int pz_groupnorm_fwd(const pz_groupnorm_desc *d, const void *x, const float *scale, const float *bias, void *y, float *savemean, float *saveinvvar,
+                     void *workspace, size_t ws_bytes, pz_stream_t stream);
+int pz_groupnorm_bwd(const pz_groupnorm_desc *d, const void *dy, const void *x, const float *scale, const float *bias, const float *savemean,
+                     const float *saveinvvar, void *dx, float *dscale, float *dbias, void *workspace, size_t ws_bytes, pz_stream_t stream);
+
 /* ---- run-time compiled kernels: replaces Driver.compile (Cuda/Source/Core/Driver.c:501-515; NVRTC there, `hipcc --genco` on the
  *      reference's HIP backend, Hip/SourceModule.py:61-99) and Driver.Module / Function (Cuda/Source/Core/Module.c:258-290). For
  *      USER kernels — backend.SourceModule / ElementwiseKernel / ReductionKernel (Cuda/SourceModule.py:31-393) — every operator

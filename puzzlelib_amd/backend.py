@@ -8,7 +8,7 @@ Hip/Backend.py:19-71 on top of Cuda/GPUBackend.py:17-433): GPUArray, memoryPool,
 Underneath every entry is one or two calls into libpuzzle_mi355.so — no MIOpen, no rocBLAS, no JIT.
 """
 import os, weakref, sys, time, ctypes
-from ctypes import byref, c_int, c_size_t, c_void_p
+from ctypes import byref, c_int, c_size_t, c_uint64, c_void_p
 from collections import OrderedDict, deque
 from types import SimpleNamespace
 
@@ -20,7 +20,7 @@ from puzzlelib_amd.driver import streamHandle
 from puzzlelib_amd.gpuarray import GPUArray, prod, eltwise, contiguousStrides
 from puzzlelib_amd.common import (
 	ConvFwdAlgo, ConvBwdFilterAlgo, ConvBwdDataAlgo, PoolMode, SoftMaxMode, BatchNormMode, LRNMode, RNNMode, DirectionMode, RNNAlgo,
-	GroupFormat, ConvPerf, toAlgoId, pair, requireF32, rptrOf
+	GroupFormat, ConvPerf, FusedAct, DropoutMask, toAlgoId, pair, requireF32, rptrOf
 )
 from puzzlelib_amd.blas import BlasContext
 from puzzlelib_amd.dnn import DnnContext, conv3d
@@ -28,7 +28,7 @@ from puzzlelib_amd.modules import (
 	MatModule, ReductionCallable, CostModule, MemModule, PoolModule, StubModule, PointwiseCost, PReluModule, PadModule,
 	UpsampleModule, CTCModule, EmbedModule
 )
-from puzzlelib_amd.kernels import EltwiseKernel, memoizedKernel, AddKernelFactory, absorbRelu, absorbReluDer, absorbAxpy
+from puzzlelib_amd.kernels import EltwiseKernel, memoizedKernel, AddKernelFactory, CounterDropoutFactory, absorbRelu, absorbReluDer, absorbAxpy
 
 
 # ---------------------------------------------------------------------------------------------- helpers
@@ -121,6 +121,13 @@ class RandomNumberGenerator:
 		lib.pz_rng_fill_normal(self.handle, data.optr, data.size, mean, stddev, None)
 
 
+	def dropoutMask(self, p):
+		"""The key of a dropout mask of this generator's next call (common.DropoutMask): what fillInteger would write, unwritten."""
+		seed, call = c_uint64(0), c_uint64(0)
+		lib.pz_rng_reserve(self.handle, byref(seed), byref(call))
+		return DropoutMask(seed.value, call.value, p)
+
+
 	def __del__(self):
 		handle, self.handle = getattr(self, "handle", None), None
 		if handle is not None:
@@ -154,6 +161,7 @@ class Mi355Backend:
 	ConvFwdAlgo, ConvBwdDataAlgo, ConvBwdFilterAlgo = ConvFwdAlgo, ConvBwdDataAlgo, ConvBwdFilterAlgo
 	PoolMode, SoftMaxMode, BatchNormMode, LRNMode = PoolMode, SoftMaxMode, BatchNormMode, LRNMode
 	RNNAlgo, RNNMode, DirectionMode = RNNAlgo, RNNMode, DirectionMode
+	FusedAct, DropoutMask = FusedAct, DropoutMask
 
 
 	def __init__(self, deviceIdx, initmode=0, logger=None):
@@ -238,6 +246,7 @@ class Mi355Backend:
 
 		self.dropoutKer = K(lib.OP_DROPOUT, 3, 2, "dropoutKer", rawScalar=(0, ))
 		self.dropout2dKer = K(lib.OP_DROPOUT2D, 3, 3, "dropout2dKer", rawScalar=(0, 2))
+		self.counterDropoutKer = CounterDropoutFactory()
 		self.toVectorAddVectorKer = K(lib.OP_AXPY, 2, 1, "toVectorAddVectorKer")
 
 		self.classicMomSGDKer = K(lib.OP_CLASSIC_MOM_SGD, 3, 2, "classicMomSGDKer")

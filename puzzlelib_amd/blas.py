@@ -14,7 +14,7 @@ from puzzlelib_amd.driver import streamHandle
 from puzzlelib_amd.gpuarray import GPUArray, prod, eltwise, contiguousStrides
 from puzzlelib_amd.common import (
 	ConvFwdAlgo, ConvBwdFilterAlgo, ConvBwdDataAlgo, PoolMode, SoftMaxMode, BatchNormMode, LRNMode, RNNMode, DirectionMode, RNNAlgo,
-	GroupFormat, ConvPerf, toAlgoId, pair, requireF32, rptrOf
+	GroupFormat, ConvPerf, FusedAct, DropoutMask, toAlgoId, pair, requireF32, rptrOf, rowDtype, rowPitch, requireVector, requireDisjoint
 )
 
 
@@ -108,6 +108,142 @@ class BlasContext:
 			lib.pz_gemm(int(transpA), int(transpB), m, n, k, alpha, pa + 4 * offA(i), lda, pb + 4 * offB(i), ldb, beta,
 						pc + 4 * offC(i), ldc, None)
 		return out
+
+
+	@staticmethod
+	def linearDesc(what, data, W, transpW, act, dropout):
+		"""descriptor of data (..., k) times W (k, n), or (n, k) with transpW; (desc, rows' shape, dropout key or None)"""
+		dtype = rowDtype(data, what)
+		if data.ndim < 2 or W.ndim != 2:
+			raise ValueError("%s: data of two axes or more and a matrix W expected, got %s and %s" % (what, data.shape, W.shape))
+		if W.dtype != data.dtype:
+			raise ValueError("%s: W is %s, data is %s" % (what, W.dtype, data.dtype))
+		k, n = (W.shape[1], W.shape[0]) if transpW else W.shape
+		if data.shape[-1] != k or k == 0 or n == 0:
+			raise ValueError("%s: data %s does not fit W %s%s" % (what, data.shape, W.shape, " (transposed)" if transpW else ""))
+		if dropout is not None and not isinstance(dropout, DropoutMask):
+			raise ValueError("%s: dropout is a DropoutMask, got %r" % (what, dropout))
+		m = prod(data.shape[:-1])
+		if max(m, n, k) > 0x7fffffff:
+			raise ValueError("%s: %d rows are too many" % (what, m))
+		desc = lib.LinearDesc(dtype, FusedAct(act).value, int(transpW), m, n, k, rowPitch(data, what + ": data"), rowPitch(W, what + ": W"), n, n, n)
+		return desc, data.shape[:-1], None if dropout is None or dropout.p == 0.0 else byref(dropout.key)
+
+
+	@staticmethod
+	def linearOperand(what, ary, shape, dtype):
+		if tuple(ary.shape) != tuple(shape) or ary.dtype != dtype:
+			raise ValueError("%s is %s %s, expected %s %s" % (what, ary.shape, ary.dtype, tuple(shape), dtype))
+		return rowPitch(ary, what)
+
+
+	def linear(self, data, W, bias=None, act=FusedAct.none, residual=None, dropout=None, preact=None, transpW=False, out=None,
+			   allocator=None):
+		"""out = residual + dropout(act(data W + bias)) in one product (float32 or float16 tensors, float32 sums and bias): what
+		Linear, Activation, Dropout and Add do one after the other (Modules/Linear.py:36-41, Activation.py:52-55, Dropout.py:33-58,
+		Add.py:15-22). data is (..., k) in rows of one pitch, W (k, n), or (n, k) with transpW. `preact`: an array for
+		data W + bias (linearBackward needs it behind an activation), or True to have one made; the call then returns (out, preact).
+		`out` may be `residual` (in place)."""
+		what = "linear"
+		desc, rows, key = self.linearDesc(what, data, W, transpW, act, dropout)
+		shape = rows + (desc.n, )
+		requireVector(bias, desc.n, "linear: bias")
+		if residual is not None:
+			desc.ldr = self.linearOperand("linear: residual", residual, shape, data.dtype)
+		if out is None:
+			out = GPUArray.empty(shape, dtype=data.dtype, allocator=allocator)
+		else:
+			desc.ldy = self.linearOperand("linear: out", out, shape, data.dtype)
+			inplace = residual is not None and lazy.sameBuffer(out, residual) and out.strides == residual.strides
+			requireDisjoint("linear: out", out, data, W, bias, None if inplace else residual)
+		if preact is True:
+			preact = GPUArray.empty(shape, dtype=data.dtype, allocator=allocator)
+		elif preact is not None:
+			desc.ldp = self.linearOperand("linear: preact", preact, shape, data.dtype)
+			requireDisjoint("linear: preact", preact, data, W, bias, residual, out)
+
+		if desc.m > 0:
+			xptr, wptr, bptr, rptr = data.rptr, W.rptr, rptrOf(bias), rptrOf(residual)
+			size = c_size_t(0)
+			lib.pz_linear_fwd_workspace_bytes(byref(desc), xptr, wptr, byref(size))
+			ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+			if desc.dtype == lib.F16:
+				lazy.matrixBegin()
+			lib.pz_linear_fwd(
+				byref(desc), xptr, wptr, bptr, rptr, key, out.optr, None if preact is None else preact.optr,
+				None if ws is None else ws.optr, size.value, None
+			)
+		return out if preact is None else (out, preact)
+
+
+	def linearBackward(self, grad, data, W, act=FusedAct.none, preact=None, dropout=None, transpW=False, wgrad=None, bgrad=None,
+					   scale=1.0, momentum=0.0, wantInput=True, wantParams=True, withbias=True, out=None, allocator=None):
+		"""The gradients of `linear`: (ingrad, wgrad, bgrad), None for what is not wanted. grad has the output's shape; the
+		residual's gradient is grad itself. Passed-in wgrad (float32, or the operands' type) and bgrad (float32) follow
+		Modules/Linear.py:44-54: dst = momentum * dst + scale * d; momentum 0 overwrites. Behind an activation `preact` is what the
+		forward pass left, with dropout the same mask is passed again."""
+		what = "linearBackward"
+		desc, rows, key = self.linearDesc(what, data, W, transpW, act, dropout)
+		shape = rows + (desc.n, )
+		desc.ldy = self.linearOperand("linearBackward: grad", grad, shape, data.dtype)
+		if desc.act != lib.ACT_NONE:
+			if preact is None:
+				raise ValueError("linearBackward: the gradient of %s needs the pre-activation" % FusedAct(act).name)
+			desc.ldp = self.linearOperand("linearBackward: preact", preact, shape, data.dtype)
+		else:
+			preact = None
+		withbias = wantParams and withbias
+		if wantInput:
+			desc.ldr = desc.k
+			if out is None:
+				out = GPUArray.empty(rows + (desc.k, ), dtype=data.dtype, allocator=allocator)
+			else:
+				desc.ldr = self.linearOperand("linearBackward: out", out, rows + (desc.k, ), data.dtype)
+		else:
+			out = None
+		if not wantParams:
+			wgrad = bgrad = None
+		else:
+			if wgrad is None and bgrad is None:
+				momentum = 0.0                                  # fresh arrays hold nothing to add to
+			elif momentum != 0.0 and (wgrad is None or (withbias and bgrad is None)):
+				raise ValueError("linearBackward: momentum needs both gradients passed in")
+			if wgrad is None:
+				wgrad = GPUArray.empty(W.shape, dtype=W.dtype, allocator=allocator)
+			elif wgrad.shape != W.shape or wgrad.dtype not in (np.float32, W.dtype) or not wgrad.contiguous:
+				raise ValueError("linearBackward: wgrad is %s %s, expected contiguous %s float32 or %s" % (wgrad.shape, wgrad.dtype, W.shape, W.dtype))
+			if not withbias:
+				bgrad = None
+			elif bgrad is None:
+				bgrad = GPUArray.empty((desc.n, ), dtype=np.float32, allocator=allocator)
+			else:
+				requireVector(bgrad, desc.n, "linearBackward: bgrad")
+		operands = (grad, data, W, preact)
+		requireDisjoint("linearBackward: out", out, *operands)
+		requireDisjoint("linearBackward: wgrad", wgrad, out, *operands)
+		requireDisjoint("linearBackward: bgrad", bgrad, wgrad, out, *operands)
+		if out is None and wgrad is None:
+			return None, None, None
+
+		gptr, xptr, wptr, pptr = grad.rptr, data.rptr, W.rptr, rptrOf(preact)
+		size = c_size_t(0)
+		lib.pz_linear_bwd_workspace_bytes(
+			byref(desc), gptr, xptr, wptr, int(key is not None), int(out is not None), int(wgrad is not None), int(bgrad is not None),
+			byref(size)
+		)
+		ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+
+		def target(ary):
+			return None if ary is None else ary.wptr if momentum != 0.0 else ary.optr
+
+		if desc.dtype == lib.F16:
+			lazy.matrixBegin()
+		lib.pz_linear_bwd(
+			byref(desc), gptr, xptr, wptr, pptr, key, None if out is None else out.optr, target(wgrad),
+			lib.F32 if wgrad is None or wgrad.dtype == np.float32 else lib.F16, target(bgrad), scale, momentum,
+			None if ws is None else ws.optr, size.value, None
+		)
+		return out, wgrad, bgrad
 
 
 	def scalarOut(self):

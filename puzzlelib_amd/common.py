@@ -80,6 +80,30 @@ class GroupFormat(Enum):              # Hip/Backend.py:39-41
 	bgp = 1
 
 
+class FusedAct(Enum):                  # the activation inside blas.linear / dnn.groupNormNd (enum PZ_ACT_*)
+	none = 0
+	relu = 1
+	gelu = 2
+	silu = 3
+
+
+class DropoutMask:
+	"""A dropout mask by its key. Element i of a tensor (row-major) is kept where word i of call `call` of the generator `seed` is
+	below (1 - p) * (2^32 - 1), and kept elements are divided by 1 - p: the mask fillInteger + dropoutKer
+	(Modules/Dropout.py:33-72) would apply, computed where it is needed instead of stored. The same object gives the same mask
+	forward and backward. RandomNumberGenerator.dropoutMask(p) hands out a mask nobody else gets."""
+	__slots__ = ("seed", "call", "p", "key")
+
+	def __init__(self, seed, call, p):
+		if not 0.0 <= p < 1.0:
+			raise ValueError("dropout probability %r is outside [0, 1)" % (p, ))
+		self.seed, self.call, self.p = int(seed), int(call), float(p)
+		if not (0 <= self.seed < 1 << 64 and 0 <= self.call < 1 << 64):
+			raise ValueError("a dropout mask's seed and call are unsigned 64-bit numbers")
+		keep = 1.0 - self.p
+		self.key = lib.DropoutKey(self.seed, self.call, int(keep * np.iinfo(np.uint32).max), keep)
+
+
 class ConvPerf:                        # Hip/Wrappers/MIOpen.py:82-100
 	def __init__(self, algo, time, memory):
 		self.algo, self.time, self.memory = algo, time, memory
@@ -116,3 +140,62 @@ def requireF32(*arrays):
 
 def rptrOf(ary):
 	return None if ary is None else ary.rptr
+
+
+# ---- operators over rows of channels (blas.linear, dnn.groupNormNd, counterDropoutKer): float32 and float16 tensors
+ROW_DTYPES = {np.dtype(np.float32): lib.F32, np.dtype(np.float16): lib.F16}
+
+
+def rowDtype(ary, what):
+	dtype = ROW_DTYPES.get(ary.dtype, None)
+	if dtype is None:
+		raise ValueError("%s: float32 or float16 gpuarray expected, got %s" % (what, ary.dtype))
+	return dtype
+
+
+def rowPitch(ary, what):
+	"""Elements from one row (the last axis) to the next: rows are dense, and all leading axes step by one pitch"""
+	item = ary.dtype.itemsize
+	if ary.contiguous:
+		return ary.shape[-1]
+	strides, shape = ary.strides, ary.shape
+	pitch, expect = None, None
+	if shape[-1] > 1 and strides[-1] != item:
+		raise ValueError("%s: the last axis is not contiguous" % what)
+	for axis in range(ary.ndim - 2, -1, -1):
+		if shape[axis] == 1:
+			continue
+		if pitch is None:
+			pitch = strides[axis]
+		elif strides[axis] != expect:
+			raise ValueError("%s: rows of one pitch expected, got strides %s of shape %s" % (what, strides, shape))
+		expect = strides[axis] * shape[axis]
+	pitch = shape[-1] * item if pitch is None else pitch
+	if pitch % item or pitch < shape[-1] * item:
+		raise ValueError("%s: rows overlap or do not start on whole elements (strides %s)" % (what, strides))
+	return pitch // item
+
+
+def requireVector(ary, size, what):
+	if ary is not None and (ary.dtype != np.float32 or ary.size != size or not ary.contiguous):
+		raise ValueError("%s: contiguous float32 vector of %d expected, got %s %s" % (what, size, ary.dtype, ary.shape))
+
+
+def requireDisjoint(what, out, *others):
+	"""`out` shares no element with any of `others` (side by side columns of one buffer are fine)"""
+	if out is None:
+		return
+	a, asize = out.gpudata.ptr, out.gpudata.size
+	for other in others:
+		if other is None:
+			continue
+		b, bsize = other.gpudata.ptr, other.gpudata.size
+		if a + asize <= b or b + bsize <= a:
+			continue
+		if out.ndim >= 2 and other.ndim >= 2 and not (out.contiguous and other.contiguous):
+			pitch = rowPitch(out, what) * out.dtype.itemsize
+			if pitch == rowPitch(other, what) * other.dtype.itemsize:
+				off = (a - b) % pitch
+				if off >= other.shape[-1] * other.dtype.itemsize and off + out.shape[-1] * out.dtype.itemsize <= pitch:
+					continue
+		raise ValueError("%s overlaps one of the operands" % what)

@@ -1,0 +1,762 @@
+// Matrix product with its epilogue: y = residual + dropout(act(x W + b)), and the backward pass (dx, dW, db). float32 and float16
+// operands, float32 sums; bias and its gradient are float32. A layer of the package's Linear -> Activation -> Dropout -> Add chain
+// (Modules/Linear.py:36-54, Activation.py:52-60, Dropout.py:33-72, Add.py:15-26) in one launch instead of five passes.
+//
+// Every product is C[m][n] = sum_k A(m, k) B(k, n) with A stored [m][k] or [k][m] and B stored [k][n] or [n][k]; the forward pass is
+// x W, the backward pass dz W^T and x^T dz with dz = dy * keep / (1 - p) * act'(z) written once by linear_gate_kernel, which also
+// leaves the column sums that become db.
+#include "gemm_tile.h"
+#include "philox.h"
+#include "rows.h"
+
+#include <type_traits>
+
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __fp16 tr16x4 __attribute__((ext_vector_type(4)));
+
+namespace {
+
+// ---- what happens to a finished sum -------------------------------------------------------------------------------------------------
+enum { EPI_FORWARD = 0, EPI_ACCUMULATE = 1 };        // y = residual + dropout(act(s + b)) | c = beta * c + alpha * s
+
+struct Epilogue {
+	void *out;                       // T, or float32 when out_f32
+	void *preact;                    // T: s + b, optional
+	const void *residual;            // T, optional
+	const float *bias;               // optional
+	long ldo, ldp, ldr;              // row pitches in elements
+	int m, n;
+	int kind, act, dropping, out_f32;
+	float alpha, beta;
+	int vec;                         // every pitch and base of the tensors above takes runs of COUNT (16 bytes of T, 32 of float32)
+	DropKey drop;
+};
+
+// COUNT sums of row `row`, columns col ... (col + COUNT - 1 may lie beyond the matrix)
+template <typename T, int COUNT>
+__device__ __forceinline__ void finish_run(const Epilogue &e, int row, int col, float (&s)[COUNT]) {
+	const int left = e.n - col;
+	if (row >= e.m || left <= 0) return;
+	const bool whole = e.vec && left >= COUNT;
+
+	if (e.kind == EPI_ACCUMULATE) {
+#pragma unroll
+		for (int i = 0; i < COUNT; ++i) s[i] *= e.alpha;
+		auto add = [&](auto *c) {
+			if (e.beta != 0.f) {
+				float old[COUNT];
+				load_run(c, whole, left, old);
+#pragma unroll
+				for (int i = 0; i < COUNT; ++i) s[i] += e.beta * old[i];
+			}
+			store_run(c, whole, left, s);
+		};
+		const size_t at = (size_t)row * e.ldo + col;
+		if (e.out_f32) add((float *)e.out + at);
+		else add((T *)e.out + at);
+		return;
+	}
+
+	if (e.bias) {
+		float b[COUNT];
+		load_run(e.bias + col, whole, left, b);
+#pragma unroll
+		for (int i = 0; i < COUNT; ++i) s[i] += b[i];
+	}
+	if (e.preact) store_run((T *)e.preact + (size_t)row * e.ldp + col, whole, left, s);
+	if (e.act != PZ_ACT_NONE) {
+#pragma unroll
+		for (int i = 0; i < COUNT; ++i) s[i] = act_value(s[i], e.act);
+	}
+	if (e.dropping) {
+		const unsigned bits = drop_bits<COUNT>(e.drop, (uint64_t)row * e.n + col);
+#pragma unroll
+		for (int i = 0; i < COUNT; ++i) s[i] = bits >> i & 1u ? s[i] / e.drop.keep : 0.f;
+	}
+	if (e.residual) {
+		float r[COUNT];
+		load_run((const T *)e.residual + (size_t)row * e.ldr + col, whole, left, r);
+#pragma unroll
+		for (int i = 0; i < COUNT; ++i) s[i] += r[i];
+	}
+	store_run((T *)e.out + (size_t)row * e.ldo + col, whole, left, s);
+}
+
+struct Product {
+	const void *a, *b;
+	float *slabs;                    // partial sums [split][m][n] when splits > 1
+	long lda, ldb;
+	int m, n, k;
+	int tiles_m, tiles_n, splits, ksteps_per_split;
+	size_t a_bytes, b_bytes;         // extents of the operands
+	Epilogue epi;
+};
+
+// Tiles in groups of kGroup rows of tiles, groups dealt out so that the blocks of one XCD (block id mod 8) work on neighbouring tiles:
+// its L2 then holds the few operand strips they share
+constexpr int kGroup = 4;
+
+__device__ __forceinline__ void tile_of(const Product &g, int &tm, int &tn) {
+	const int tiles = g.tiles_m * g.tiles_n, xcd = blockIdx.x % pz::kNumXCD, at = blockIdx.x / pz::kNumXCD;
+	const int each = tiles / pz::kNumXCD, more = tiles % pz::kNumXCD;
+	const int id = xcd * each + min(xcd, more) + at;
+	const int group = id / (kGroup * g.tiles_n), rest = id % (kGroup * g.tiles_n);
+	const int rows = min(kGroup, g.tiles_m - group * kGroup);
+	tm = group * kGroup + rest % rows;
+	tn = rest / rows;
+}
+
+// A wave's accumulators -> rows. The matrix instruction took the operand of the n side first, so a lane holds, of row m = lane & 31,
+// the columns 8 q + 4 (lane >> 5) ... + 3 in registers 4 q ... 4 q + 3. They go through LDS in slabs of 32 rows x 32 TN columns (the wave's own,
+// no barrier), so that consecutive lanes store consecutive runs of a row: whole 128-byte lines instead of 32 pieces of 16 bytes.
+template <typename T, int TM, int TN>
+struct Drain {
+	static constexpr int COUNT = 16 / sizeof(T);                 // values a lane stores at once
+	static constexpr int COLS = 32 * TN, PITCH = COLS + 4;       // (+4: the rows of a store start 4 banks apart)
+	static constexpr int FLOATS = 32 * PITCH;
+
+	static __device__ __forceinline__ void run(const Product &g, const f32x16 (&acc)[TM][TN], float *lds, int row0, int col0, int split, int lane) {
+		const int l31 = lane & 31, lhi = lane >> 5;
+#pragma unroll
+		for (int i = 0; i < TM; ++i) {
+#pragma unroll
+			for (int j = 0; j < TN; ++j)
+#pragma unroll
+				for (int q = 0; q < 4; ++q)
+					*reinterpret_cast<f32x4 *>(lds + l31 * PITCH + j * 32 + q * 8 + lhi * 4) =
+					    (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+			__builtin_amdgcn_wave_barrier();
+			constexpr int RUNS = COLS / COUNT, STEP = 64 / RUNS;         // runs in a row, rows a wave handles at once
+			static_assert(64 % RUNS == 0, "runs of a row over lanes");
+			const int run = lane % RUNS;
+#pragma unroll 2
+			for (int r = lane / RUNS; r < 32; r += STEP) {
+				float s[COUNT];
+#pragma unroll
+				for (int v = 0; v < COUNT; v += 4) {
+					const f32x4 x = *reinterpret_cast<const f32x4 *>(lds + r * PITCH + run * COUNT + v);
+#pragma unroll
+					for (int e = 0; e < 4; ++e) s[v + e] = x[e];
+				}
+				const int row = row0 + i * 32 + r, col = col0 + run * COUNT;
+				if (g.splits == 1) {
+					finish_run<T>(g.epi, row, col, s);
+				} else if (row < g.m && col < g.n) {
+					float *o = g.slabs + ((size_t)split * g.m + row) * g.n + col;
+					store_run(o, g.n % 4 == 0 && col + COUNT <= g.n, g.n - col, s);
+				}
+			}
+			__builtin_amdgcn_wave_barrier();
+		}
+	}
+};
+
+// ---- float32: v_mfma_f32_32x32x2_f32, operands through registers (gemm_tile.h) -----------------------------------------------------
+template <int BM, int BN, int WM, int WN, bool TA, bool TB, bool VEC>
+__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(4, 8))) linear_f32_kernel(Product g) {
+	constexpr int NT = 64 * WM * WN, TM = BM / (32 * WM), TN = BN / (32 * WN);
+	using LA = Loader<NT, BM, TA, VEC>;
+	using LB = Loader<NT, BN, !TB, VEC>;
+	using Out = Drain<float, TM, TN>;
+	constexpr int TILES = 2 * BK * (LA::LD + LB::LD), SLABS = WM * WN * Out::FLOATS;
+	__shared__ __attribute__((aligned(16))) float lds[TILES > SLABS ? TILES : SLABS];
+	float *const As = lds, *const Bs = lds + 2 * BK * LA::LD;
+	constexpr int A = BK * LA::LD, B = BK * LB::LD;
+
+	const int tid = threadIdx.x, lane = tid & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+	const int wm = wave / WN, wn = wave % WN;
+	int tm, tn;
+	tile_of(g, tm, tn);
+	const int m0 = tm * BM, n0 = tn * BN;
+	const int split = blockIdx.z;
+	const int kbeg = split * g.ksteps_per_split * BK;
+	const int kend = min(g.k, kbeg + g.ksteps_per_split * BK);
+	const int l31 = lane & 31, lhi = lane >> 5;
+
+	const float *a = (const float *)g.a, *b = (const float *)g.b;
+	const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc((void *)a, 0, VEC ? (unsigned)g.a_bytes : 0u, 0x00020000);
+	const __amdgpu_buffer_rsrc_t br = __builtin_amdgcn_make_buffer_rsrc((void *)b, 0, VEC ? (unsigned)g.b_bytes : 0u, 0x00020000);
+
+	f32x16 acc[TM][TN];
+#pragma unroll
+	for (int i = 0; i < TM; ++i)
+#pragma unroll
+		for (int j = 0; j < TN; ++j)
+#pragma unroll
+			for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+	LA la;
+	LB lb;
+	la.init((int)g.lda, m0, g.m, kbeg, tid);
+	lb.init((int)g.ldb, n0, g.n, kbeg, tid);
+	la.load(a, ar, (int)g.lda, m0, g.m, kbeg, kend, tid);
+	lb.load(b, br, (int)g.ldb, n0, g.n, kbeg, kend, tid);
+	la.park(As, tid);
+	lb.park(Bs, tid);
+	__syncthreads();
+
+	int buf = 0;
+	for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
+		const bool more = k0 + BK < kend;
+		if (more) {
+			la.load(a, ar, (int)g.lda, m0, g.m, k0 + BK, kend, tid);
+			lb.load(b, br, (int)g.ldb, n0, g.n, k0 + BK, kend, tid);
+		}
+		const float *as = As + buf * A + wm * (BM / WM) + l31, *bs = Bs + buf * B + wn * (BN / WN) + l31;
+#pragma unroll
+		for (int ks = 0; ks < BK; ks += 2) {
+			float av[TM], bv[TN];
+#pragma unroll
+			for (int i = 0; i < TM; ++i) av[i] = as[(ks + lhi) * LA::LD + i * 32];
+#pragma unroll
+			for (int j = 0; j < TN; ++j) bv[j] = bs[(ks + lhi) * LB::LD + j * 32];
+#pragma unroll
+			for (int i = 0; i < TM; ++i)
+#pragma unroll
+				for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(bv[j], av[i], acc[i][j], 0, 0, 0);
+		}
+		if (more) {
+			la.park(As + (buf ^ 1) * A, tid);
+			lb.park(Bs + (buf ^ 1) * B, tid);
+		}
+		__syncthreads();
+	}
+	Out::run(g, acc, lds + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);
+}
+
+// ---- float16: v_mfma_f32_32x32x16_f16, operands straight into LDS --------------------------------------------------------------------
+constexpr int HK = 64;               // reduction steps per LDS tile
+
+__device__ __forceinline__ unsigned lds_address(const void *p) {
+	return (unsigned)(size_t)(__attribute__((address_space(3))) const void *)p;
+}
+
+// 16 bytes per lane from `voff` of the buffer to lds + 16 * lane, no register in between; outside the buffer: zeros. The caller waits
+// (vmcnt) before anyone reads them.
+__device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned lds, unsigned voff) {
+	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rs) : "memory");
+}
+
+__device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void meet() { asm volatile("s_barrier" ::: "memory"); }
+
+// One operand of the tile: ROWS x HK, staged by WAVES waves.
+// KMAJOR = false: [row][k] in memory, so 128 bytes of k per row in LDS; the 16-byte pieces of row r stand at piece ^ (r & 7) — a
+//   fragment read (32 rows, one piece each) then touches all 64 banks evenly.
+// KMAJOR = true: [k][row] in memory, so ROWS * 2 bytes per k in LDS; the 32-byte pieces of step k stand at piece ^ turn(k), and
+//   fragments are read with ds_read_b64_tr_b16, which hands 16 lanes the 4 x 16 block of 4 steps x 16 rows transposed; turn() puts
+//   the 16 steps that one such instruction reads onto 8 different piece positions (256 bytes: all banks).
+template <int ROWS, bool KMAJOR, int WAVES>
+struct Stage {
+	static constexpr int HALVES = ROWS * HK;
+	static constexpr int PIECES = ROWS / 8 / WAVES;            // dma16 per wave and tile
+	static_assert(PIECES >= 1 && PIECES * WAVES * 8 == ROWS, "tile / waves");
+	static constexpr int TURNS = ROWS / 16 < 8 ? ROWS / 16 : 8;
+
+	__device__ __forceinline__ static int turn(int k) { return ((k & 3) | (k >> 3 & 1) << 2) & (TURNS - 1); }
+
+	size_t base, bytes;              // start of the tile in the operand at the next k step, and what is left of the operand from there
+	size_t step;                     // advance per k step
+	const char *p;
+	unsigned off[PIECES];            // a lane's byte offsets from the start
+	int kpiece;                      // KMAJOR = false: first k of the lane's piece
+
+	__device__ __forceinline__ void init(const void *src, size_t extent, long ld, int row0, int kbeg, int wave, int lane) {
+		const size_t start = KMAJOR ? ((size_t)kbeg * ld + row0) * 2 : ((size_t)row0 * ld + kbeg) * 2;
+		p = (const char *)src + start;
+		bytes = extent > start ? extent - start : 0;
+		step = KMAJOR ? (size_t)HK * ld * 2 : (size_t)HK * 2;
+		kpiece = 0;
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) {
+			const int o = ((wave * PIECES + i) * 64 + lane) * 16;                // place in the LDS tile
+			if (KMAJOR) {
+				const int k = o / (ROWS * 2), at = o % (ROWS * 2) / 16;
+				off[i] = (unsigned)((size_t)k * ld * 2) + (((at >> 1) ^ turn(k)) * 2 + (at & 1)) * 16;
+			} else {
+				const int r = o / 128, piece = (o / 16 & 7) ^ (r & 7);
+				kpiece = piece * 8;                                               // (r & 7 is lane >> 3 for every i)
+				off[i] = (unsigned)((size_t)r * ld * 2) + piece * 16;
+			}
+		}
+	}
+
+	// k steps [k, k + HK) into the tile at LDS address `lds`; moves on
+	__device__ __forceinline__ void issue(unsigned lds, int k, int kend, int wave) {
+		const unsigned span = bytes > 0xfffff000ull ? 0xfffff000u : (unsigned)bytes;
+		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, __builtin_amdgcn_readfirstlane(span), 0x00020000);
+		const bool in = KMAJOR || k + kpiece < kend;
+#pragma unroll
+		for (int i = 0; i < PIECES; ++i) dma16(rs, lds + (wave * PIECES + i) * 1024, in ? off[i] : 0xfffffff0u);
+		p += step;
+		bytes = bytes > step ? bytes - step : 0;
+	}
+
+	// fragment of v_mfma_f32_32x32x16_f16: rows row0 + (lane & 31), steps 16 s + 8 (lane >> 5) ... + 7
+	__device__ __forceinline__ static f16x8 fragment(const f16 *tile, int row0, int s, int lane) {
+		if (!KMAJOR) {
+			const int r = row0 + (lane & 31), piece = s * 2 + (lane >> 5);
+			return *reinterpret_cast<const f16x8 *>(tile + r * HK + ((piece ^ (r & 7)) * 8));
+		}
+		// 16 lanes: rows base ... base + 15; lane j of them points at step (j >> 2), rows 4 (j & 3) ... + 3 of the block
+		const int j = lane & 15, base = row0 + (lane >> 4 & 1) * 16, k = s * 16 + (lane >> 5) * 8 + (j >> 2);
+		union { f16x8 v; tr16x4 h[2]; } f;
+#pragma unroll
+		for (int half = 0; half < 2; ++half) {
+			const int kk = k + half * 4;
+			const f16 *at = tile + kk * ROWS + ((base / 16) ^ turn(kk)) * 16 + (j & 3) * 4;
+			f.h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr16x4 *)at);
+		}
+		return f.v;
+	}
+};
+
+template <int BM, int BN, int WM, int WN, bool TA, bool TB>
+__global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
+	constexpr int WAVES = WM * WN, TM = BM / (32 * WM), TN = BN / (32 * WN);
+	using SA = Stage<BM, TA, WAVES>;
+	using SB = Stage<BN, !TB, WAVES>;
+	using Out = Drain<f16, TM, TN>;
+	constexpr int TILE = SA::HALVES + SB::HALVES, SLABS = 2 * WAVES * Out::FLOATS;
+	__shared__ __attribute__((aligned(1024))) f16 lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
+
+	const int lane = threadIdx.x & 63;
+	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+	const int wm = wave / WN, wn = wave % WN;
+	int tm, tn;
+	tile_of(g, tm, tn);
+	const int m0 = tm * BM, n0 = tn * BN;
+	const int split = blockIdx.z;
+	const int kbeg = split * g.ksteps_per_split * HK;
+	const int kend = min(g.k, kbeg + g.ksteps_per_split * HK);
+
+	f32x16 acc[TM][TN];
+#pragma unroll
+	for (int i = 0; i < TM; ++i)
+#pragma unroll
+		for (int j = 0; j < TN; ++j)
+#pragma unroll
+			for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+	SA sa;
+	SB sb;
+	sa.init(g.a, g.a_bytes, g.lda, m0, kbeg, wave, lane);
+	sb.init(g.b, g.b_bytes, g.ldb, n0, kbeg, wave, lane);
+	const unsigned at = lds_address(lds);
+	if (kbeg < kend) {
+		sa.issue(at, kbeg, kend, wave);
+		sb.issue(at + SA::HALVES * 2, kbeg, kend, wave);
+	}
+
+	int buf = 0;
+	for (int k0 = kbeg; k0 < kend; k0 += HK, buf ^= 1) {
+		dma_landed();                // this wave's share of tile k0 is in LDS; behind the barrier everybody's is,
+		meet();                      // and everybody is done reading the other half
+		if (k0 + HK < kend) {
+			const unsigned next = at + (buf ^ 1) * (TILE * 2);
+			sa.issue(next, k0 + HK, kend, wave);
+			sb.issue(next + SA::HALVES * 2, k0 + HK, kend, wave);
+		}
+		const f16 *as = lds + buf * TILE, *bs = as + SA::HALVES;
+#pragma unroll
+		for (int s = 0; s < HK / 16; ++s) {
+			f16x8 av[TM], bv[TN];
+#pragma unroll
+			for (int i = 0; i < TM; ++i) av[i] = SA::fragment(as, wm * (BM / WM) + i * 32, s, lane);
+#pragma unroll
+			for (int j = 0; j < TN; ++j) bv[j] = SB::fragment(bs, wn * (BN / WN) + j * 32, s, lane);
+#pragma unroll
+			for (int i = 0; i < TM; ++i)
+#pragma unroll
+				for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bv[j], av[i], acc[i][j], 0, 0, 0);
+		}
+	}
+	__syncthreads();                 // the slabs below lie over the tiles
+	Out::run(g, acc, reinterpret_cast<float *>(lds) + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);
+}
+
+// ---- partial sums of a product split along k, added in order, then the epilogue ------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(256) linear_join_kernel(Product g) {
+	constexpr int COUNT = 16 / sizeof(T);
+	const int runs = (g.n + COUNT - 1) / COUNT;
+	const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
+	if (idx >= (size_t)runs * g.m) return;
+	const int row = (int)(idx / runs), col = (int)(idx % runs) * COUNT, left = g.n - col;
+	const bool whole = g.n % 4 == 0 && left >= COUNT;
+	float s[COUNT];
+	const float *p = g.slabs + (size_t)row * g.n + col;
+	load_run(p, whole, left, s);
+	for (int i = 1; i < g.splits; ++i) {
+		float more[COUNT];
+		load_run(p + (size_t)i * g.m * g.n, whole, left, more);
+#pragma unroll
+		for (int e = 0; e < COUNT; ++e) s[e] += more[e];
+	}
+	finish_run<T>(g.epi, row, col, s);
+}
+
+// ---- operands whose rows do not start on 16 bytes: a copy whose pitch is a multiple of 8 elements, the rest of each row zero -----------
+template <typename T>
+__global__ void __launch_bounds__(256) linear_align_kernel(const T *__restrict__ src, T *__restrict__ dst, int rows, int cols, long ld, int pitch) {
+	constexpr int COUNT = 16 / sizeof(T);
+	const int runs = pitch / COUNT;
+	const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
+	if (idx >= (size_t)runs * rows) return;
+	const int row = (int)(idx / runs), col = (int)(idx % runs) * COUNT;
+	float v[COUNT];
+	load_run(src + (size_t)row * ld + col, false, cols - col, v);
+	store_run(dst + (size_t)row * pitch + col, true, COUNT, v);
+}
+
+// ---- dz = dy * keep / (1 - p) * act'(z), and partial column sums -----------------------------------------------------------------------
+struct Gate {
+	const void *dy, *preact;
+	void *dz;                        // optional: without it only the sums are made
+	float *sums;                     // [row blocks][n], optional
+	long lddy, ldp, lddz;
+	int m, n, act, dropping, vec, rows_per_block;
+	DropKey drop;
+};
+
+// block = 4 waves x (64 lanes x 8 columns), rows dealt out over the waves
+template <typename T>
+__global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
+	constexpr int COUNT = 8;
+	__shared__ float part[4][64][COUNT + 1];
+	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+	const int col = (blockIdx.x * 64 + lane) * COUNT, left = g.n - col;
+	const int row0 = blockIdx.y * g.rows_per_block, row1 = min(g.m, row0 + g.rows_per_block);
+	float sum[COUNT];
+#pragma unroll
+	for (int e = 0; e < COUNT; ++e) sum[e] = 0.f;
+
+	if (left > 0) {
+		const bool whole = g.vec && left >= COUNT;
+		for (int row = row0 + wave; row < row1; row += 4) {
+			float d[COUNT];
+			load_run((const T *)g.dy + (size_t)row * g.lddy + col, whole, left, d);
+			if (g.dropping) {
+				const unsigned bits = drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col);
+#pragma unroll
+				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] / g.drop.keep : 0.f;
+			}
+			if (g.act != PZ_ACT_NONE) {
+				float z[COUNT];
+				load_run((const T *)g.preact + (size_t)row * g.ldp + col, whole, left, z);
+#pragma unroll
+				for (int e = 0; e < COUNT; ++e) d[e] *= act_slope(z[e], g.act);
+			}
+			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)
+#pragma unroll
+			for (int e = 0; e < COUNT; ++e) sum[e] += d[e];
+		}
+	}
+	if (!g.sums) return;
+#pragma unroll
+	for (int e = 0; e < COUNT; ++e) part[wave][lane][e] = sum[e];
+	__syncthreads();
+	for (int i = threadIdx.x; i < 64 * COUNT; i += 256) {
+		const int l = i / COUNT, e = i % COUNT, c = (blockIdx.x * 64 + l) * COUNT + e;
+		if (c < g.n) g.sums[(size_t)blockIdx.y * g.n + c] = part[0][l][e] + part[1][l][e] + part[2][l][e] + part[3][l][e];
+	}
+}
+
+// db = beta * db + alpha * (sums of the row blocks, in order)
+__global__ void __launch_bounds__(256) linear_bias_grad_kernel(const float *__restrict__ sums, int blocks, int n, float *__restrict__ db,
+                                                                float alpha, float beta) {
+	const int c = blockIdx.x * 256 + threadIdx.x;
+	if (c >= n) return;
+	float s = 0.f;
+	for (int i = 0; i < blocks; ++i) s += sums[(size_t)i * n + c];
+	db[c] = (beta == 0.f ? 0.f : beta * db[c]) + alpha * s;
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------------------------------
+constexpr size_t kAlign = 256;
+size_t rounded(size_t nbytes) { return (nbytes + kAlign - 1) / kAlign * kAlign; }
+int padded(int n) { return (n + 7) / 8 * 8; }
+
+// what a product takes from the workspace: copies of operands that are not aligned, slabs of a split
+struct Plan {
+	int bm, bn, bk, splits, ksteps_per_split, tiles_m, tiles_n;
+	bool copy_a, copy_b;
+	size_t a_bytes, b_bytes, slab_bytes;
+	size_t bytes() const { return a_bytes + b_bytes + slab_bytes; }
+};
+
+struct Operands {
+	const void *a, *b;
+	long lda, ldb;
+	int m, n, k;
+	bool ta, tb;
+	int wide_a, wide_b;              // readable length of a stored row: its elements, and zeros behind them
+};
+
+// 16-byte loads: rows that start on 16 bytes and are whole pieces long
+bool aligned(const void *p, long ld, int wide, int size) {
+	const int piece = 16 / size;
+	return (uintptr_t)p % 16 == 0 && ld % piece == 0 && wide % piece == 0;
+}
+
+Plan plan_product(int dtype, const Operands &o) {
+	Plan p{};
+	if (o.m == 0 || o.n == 0) return p;                                 // (no output, nothing runs)
+	const int size = dtype == PZ_F16 ? 2 : 4;
+	p.bk = dtype == PZ_F16 ? HK : BK;
+	p.bm = o.m > 64 ? 128 : 64, p.bn = o.n > 64 ? 128 : 64;
+	const long tiles256 = (long)pz::ceil_div(o.m, 256) * pz::ceil_div(o.n, 256);
+	if (o.k >= (dtype == PZ_F16 ? 256 : 1024) && tiles256 >= pz::kNumCU) p.bm = p.bn = 256;
+	p.tiles_m = pz::ceil_div(o.m, p.bm), p.tiles_n = pz::ceil_div(o.n, p.bn);
+	const long tiles = (long)p.tiles_m * p.tiles_n;
+	const int ksteps = pz::ceil_div(o.k, p.bk), least = 128 / p.bk;      // a split keeps 128 steps at least
+	int splits = 1;
+	if (tiles < pz::kNumCU) {
+		splits = (int)(2 * pz::kNumCU / tiles);
+		splits = splits > ksteps / least ? ksteps / least : splits;
+		splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
+	}
+	p.ksteps_per_split = ksteps > 0 ? pz::ceil_div(ksteps, splits) : 1;
+	p.splits = ksteps > 0 ? pz::ceil_div(ksteps, p.ksteps_per_split) : 1;
+	p.copy_a = !aligned(o.a, o.lda, o.wide_a, size);
+	p.copy_b = !aligned(o.b, o.ldb, o.wide_b, size);
+	p.a_bytes = p.copy_a ? rounded((size_t)(o.ta ? o.k : o.m) * padded(o.ta ? o.m : o.k) * size) : 0;
+	p.b_bytes = p.copy_b ? rounded((size_t)(o.tb ? o.n : o.k) * padded(o.tb ? o.k : o.n) * size) : 0;
+	p.slab_bytes = p.splits > 1 ? rounded((size_t)p.splits * o.m * o.n * sizeof(float)) : 0;
+	return p;
+}
+
+template <typename T>
+int align_operand(const void *&src, long &ld, int rows, int cols, char *at, hipStream_t st) {
+	const int pitch = padded(cols), runs = pitch / (16 / (int)sizeof(T));
+	const size_t items = (size_t)rows * runs;
+	if (items > 0) {
+		linear_align_kernel<T><<<(unsigned)((items + 255) / 256), 256, 0, st>>>((const T *)src, (T *)at, rows, cols, ld, pitch);
+		PZ_LAUNCH_CHECK();
+	}
+	src = at, ld = pitch;
+	return PZ_OK;
+}
+
+template <bool TA, bool TB>
+void launch_f16(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
+	if (p.bm == 256) linear_f16_kernel<256, 256, 2, 4, TA, TB><<<grid, 512, 0, st>>>(g);
+	else if (p.bm == 128 && p.bn == 128) linear_f16_kernel<128, 128, 2, 2, TA, TB><<<grid, 256, 0, st>>>(g);
+	else if (p.bm == 128) linear_f16_kernel<128, 64, 2, 1, TA, TB><<<grid, 128, 0, st>>>(g);
+	else if (p.bn == 128) linear_f16_kernel<64, 128, 1, 2, TA, TB><<<grid, 128, 0, st>>>(g);
+	else linear_f16_kernel<64, 64, 1, 1, TA, TB><<<grid, 64, 0, st>>>(g);
+}
+
+template <bool TA, bool TB, bool VEC>
+void launch_f32(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
+	if (p.bm == 256) linear_f32_kernel<256, 256, 4, 4, TA, TB, VEC><<<grid, 1024, 0, st>>>(g);
+	else if (p.bm == 128 && p.bn == 128) linear_f32_kernel<128, 128, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	else if (p.bm == 128) linear_f32_kernel<128, 64, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	else if (p.bn == 128) linear_f32_kernel<64, 128, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	else linear_f32_kernel<64, 64, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+}
+
+size_t extent_of(int rows, int wide, long ld, int size) { return rows > 0 ? ((size_t)(rows - 1) * ld + wide) * size : 0; }
+
+// C = epilogue(A B); ws: plan_product(...).bytes()
+int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st) {
+	if (o.m == 0 || o.n == 0) return PZ_OK;
+	const Plan p = plan_product(dtype, o);
+	const int size = dtype == PZ_F16 ? 2 : 4;
+	if (p.copy_a) {
+		const int rows = o.ta ? o.k : o.m, cols = o.ta ? o.m : o.k;
+		if (int rc = dtype == PZ_F16 ? align_operand<f16>(o.a, o.lda, rows, cols, ws, st) : align_operand<float>(o.a, o.lda, rows, cols, ws, st)) return rc;
+	}
+	if (p.copy_b) {
+		const int rows = o.tb ? o.n : o.k, cols = o.tb ? o.k : o.n;
+		char *at = ws + p.a_bytes;
+		if (int rc = dtype == PZ_F16 ? align_operand<f16>(o.b, o.ldb, rows, cols, at, st) : align_operand<float>(o.b, o.ldb, rows, cols, at, st)) return rc;
+	}
+
+	Product g;
+	g.a = o.a, g.b = o.b, g.lda = o.lda, g.ldb = o.ldb;
+	g.slabs = (float *)(ws + p.a_bytes + p.b_bytes);
+	g.m = o.m, g.n = o.n, g.k = o.k;
+	g.tiles_m = p.tiles_m, g.tiles_n = p.tiles_n, g.splits = p.splits, g.ksteps_per_split = p.ksteps_per_split;
+	g.a_bytes = extent_of(o.ta ? o.k : o.m, p.copy_a ? (int)o.lda : o.wide_a, o.lda, size);
+	g.b_bytes = extent_of(o.tb ? o.n : o.k, p.copy_b ? (int)o.ldb : o.wide_b, o.ldb, size);
+	g.epi = epi;
+	g.epi.m = o.m, g.epi.n = o.n;
+
+	const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits);
+	if (dtype == PZ_F16) {
+		if (o.ta) launch_f16<true, false>(p, g, grid, st);
+		else if (o.tb) launch_f16<false, true>(p, g, grid, st);
+		else launch_f16<false, false>(p, g, grid, st);
+	} else {
+		const bool vec = g.a_bytes < 0xffff0000ull && g.b_bytes < 0xffff0000ull;       // 16-byte buffer loads reach 4 GiB
+		if (o.ta) vec ? launch_f32<true, false, true>(p, g, grid, st) : launch_f32<true, false, false>(p, g, grid, st);
+		else if (o.tb) vec ? launch_f32<false, true, true>(p, g, grid, st) : launch_f32<false, true, false>(p, g, grid, st);
+		else vec ? launch_f32<false, false, true>(p, g, grid, st) : launch_f32<false, false, false>(p, g, grid, st);
+	}
+	PZ_LAUNCH_CHECK();
+	if (p.splits > 1) {
+		const size_t items = (size_t)o.m * pz::ceil_div(o.n, 16 / size);
+		const unsigned blocks = (unsigned)((items + 255) / 256);
+		if (dtype == PZ_F16) linear_join_kernel<f16><<<blocks, 256, 0, st>>>(g);
+		else linear_join_kernel<float><<<blocks, 256, 0, st>>>(g);
+		PZ_LAUNCH_CHECK();
+	}
+	return PZ_OK;
+}
+
+int check_desc(const pz_linear_desc *d, const char *who) {
+	PZ_REQUIRE(d, "%s: null descriptor", who);
+	PZ_REQUIRE(d->dtype == PZ_F32 || d->dtype == PZ_F16, "%s: unknown dtype %d", who, d->dtype);
+	PZ_REQUIRE(d->act >= PZ_ACT_NONE && d->act <= PZ_ACT_SILU, "%s: unknown activation %d", who, d->act);
+	PZ_REQUIRE(d->m >= 0 && d->n > 0 && d->k > 0, "%s: bad dimensions (%d, %d, %d)", who, d->m, d->n, d->k);
+	PZ_REQUIRE(d->ldx >= d->k && d->ldw >= (d->trans_w ? d->k : d->n) && d->ldy >= d->n, "%s: row pitch too small", who);
+	return PZ_OK;
+}
+
+int check_mask(const pz_dropout_mask *mask, const char *who) {
+	PZ_REQUIRE(!mask || (mask->keep > 0.f && mask->keep <= 1.f), "%s: keep probability %g", who, mask ? mask->keep : 0.f);
+	return PZ_OK;
+}
+
+bool runs_ok(const void *p, long ld, int size) { return !p || ((uintptr_t)p % 16 == 0 && ld * size % 16 == 0); }
+
+Operands forward_operands(const pz_linear_desc *d, const void *x, const void *w) {
+	return Operands{x, w, d->ldx, d->ldw, d->m, d->n, d->k, false, d->trans_w != 0, d->k, d->trans_w ? d->k : d->n};
+}
+
+// the backward pass's workspace: dz (where dy cannot serve itself), row-block sums for db, then what the larger product takes
+struct BackPlan {
+	bool write_dz;
+	int row_blocks, rows_per_block;
+	size_t dz_bytes, sum_bytes, product_bytes;
+	size_t bytes() const { return dz_bytes + sum_bytes + product_bytes; }
+};
+
+Operands data_operands(const pz_linear_desc *d, const void *dz, long lddz, int wide, const void *w) {      // dx[m][k] = dz W^T
+	return Operands{dz, w, lddz, d->ldw, d->m, d->k, d->n, false, d->trans_w == 0, wide, d->trans_w ? d->k : d->n};
+}
+
+Operands weight_operands(const pz_linear_desc *d, const void *dz, long lddz, int wide, const void *x) {    // dW = x^T dz (or its transpose)
+	if (d->trans_w) return Operands{dz, x, lddz, d->ldx, d->n, d->k, d->m, true, false, wide, d->k};
+	return Operands{x, dz, d->ldx, lddz, d->k, d->n, d->m, true, false, d->k, wide};
+}
+
+BackPlan plan_backward(const pz_linear_desc *d, const void *dy, const void *x, const void *w, bool dropping, bool want_dx, bool want_dw, bool want_db) {
+	BackPlan p;
+	const int size = d->dtype == PZ_F16 ? 2 : 4;
+	p.write_dz = (want_dx || want_dw) && (d->act != PZ_ACT_NONE || dropping || !aligned(dy, d->ldy, d->n, size));
+	p.dz_bytes = p.write_dz ? rounded((size_t)d->m * padded(d->n) * size) : 0;
+	const int strips = pz::ceil_div(d->n, 512);
+	p.rows_per_block = 128;                                              // fewer rows a block where there are few blocks
+	while (p.rows_per_block > 8 && (long)strips * pz::ceil_div(d->m, p.rows_per_block) < 4 * pz::kNumCU) p.rows_per_block /= 2;
+	while (pz::ceil_div(d->m, p.rows_per_block) > 65535) p.rows_per_block *= 2;
+	p.row_blocks = pz::ceil_div(d->m, p.rows_per_block);
+	p.sum_bytes = want_db ? rounded((size_t)p.row_blocks * d->n * sizeof(float)) : 0;
+	// (dz in the workspace is aligned: any multiple of 256 stands for its address)
+	const void *dz = p.write_dz ? (const void *)kAlign : dy;
+	const long lddz = p.write_dz ? padded(d->n) : d->ldy;
+	const int wide = p.write_dz ? padded(d->n) : d->n;
+	const size_t dx_bytes = want_dx ? plan_product(d->dtype, data_operands(d, dz, lddz, wide, w)).bytes() : 0;
+	const size_t dw_bytes = want_dw ? plan_product(d->dtype, weight_operands(d, dz, lddz, wide, x)).bytes() : 0;
+	p.product_bytes = dx_bytes > dw_bytes ? dx_bytes : dw_bytes;
+	return p;
+}
+
+DropKey key_of(const pz_dropout_mask *mask) {
+	return mask ? DropKey{mask->seed, mask->call, mask->threshold, mask->keep} : DropKey{0, 0, 0, 1.f};
+}
+
+}  // namespace
+
+extern "C" {
+
+int pz_linear_fwd_workspace_bytes(const pz_linear_desc *d, const void *x, const void *w, size_t *nbytes) {
+	if (int rc = check_desc(d, "pz_linear_fwd_workspace_bytes")) return rc;
+	PZ_REQUIRE(nbytes, "pz_linear_fwd_workspace_bytes: null output");
+	*nbytes = d->m > 0 ? plan_product(d->dtype, forward_operands(d, x, w)).bytes() : 0;
+	return PZ_OK;
+}
+
+int pz_linear_fwd(const pz_linear_desc *d, const void *x, const void *w, const float *bias, const void *residual, const pz_dropout_mask *mask,
+                  void *y, void *preact, void *workspace, size_t ws_bytes, pz_stream_t stream) {
+	if (int rc = check_desc(d, "pz_linear_fwd")) return rc;
+	if (int rc = check_mask(mask, "pz_linear_fwd")) return rc;
+	if (d->m == 0) return PZ_OK;
+	PZ_REQUIRE(x && w && y, "pz_linear_fwd: null tensor");
+	PZ_REQUIRE((!residual || d->ldr >= d->n) && (!preact || d->ldp >= d->n), "pz_linear_fwd: row pitch too small");
+	const Operands o = forward_operands(d, x, w);
+	const size_t need = plan_product(d->dtype, o).bytes();
+	PZ_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "pz_linear_fwd: workspace needs %zu bytes", need);
+
+	const int size = d->dtype == PZ_F16 ? 2 : 4;
+	Epilogue e{};
+	e.out = y, e.preact = preact, e.residual = residual, e.bias = bias;
+	e.ldo = d->ldy, e.ldp = d->ldp, e.ldr = d->ldr;
+	e.kind = EPI_FORWARD, e.act = d->act, e.dropping = mask != nullptr, e.alpha = 1.f;
+	e.vec = runs_ok(y, d->ldy, size) && runs_ok(preact, d->ldp, size) && runs_ok(residual, d->ldr, size) && runs_ok(bias, 4, 4);
+	e.drop = key_of(mask);
+	return product(d->dtype, o, e, (char *)workspace, pz::as_stream(stream));
+}
+
+int pz_linear_bwd_workspace_bytes(const pz_linear_desc *d, const void *dy, const void *x, const void *w, int dropping, int want_dx, int want_dw,
+                                  int want_db, size_t *nbytes) {
+	if (int rc = check_desc(d, "pz_linear_bwd_workspace_bytes")) return rc;
+	PZ_REQUIRE(nbytes, "pz_linear_bwd_workspace_bytes: null output");
+	*nbytes = plan_backward(d, dy, x, w, dropping != 0, want_dx != 0, want_dw != 0, want_db != 0).bytes();
+	return PZ_OK;
+}
+
+int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const void *w, const void *preact, const pz_dropout_mask *mask,
+                  void *dx, void *dw, int dw_dtype, float *db, float alpha, float beta, void *workspace, size_t ws_bytes, pz_stream_t stream) {
+	if (int rc = check_desc(d, "pz_linear_bwd")) return rc;
+	if (int rc = check_mask(mask, "pz_linear_bwd")) return rc;
+	PZ_REQUIRE(dw_dtype == PZ_F32 || dw_dtype == d->dtype, "pz_linear_bwd: weight gradients are float32 or the operands' type");
+	PZ_REQUIRE(d->m == 0 || (dy && (!dx || w) && (!dw || x)), "pz_linear_bwd: null tensor");
+	PZ_REQUIRE(d->m == 0 || d->act == PZ_ACT_NONE || (preact && d->ldp >= d->n), "pz_linear_bwd: the activation's gradient needs the pre-activation");
+	PZ_REQUIRE(!dx || d->ldr >= d->k, "pz_linear_bwd: row pitch too small");
+	const BackPlan p = plan_backward(d, dy, x, w, mask != nullptr, dx != nullptr, dw != nullptr, db != nullptr);
+	const size_t need = p.bytes();
+	PZ_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "pz_linear_bwd: workspace needs %zu bytes", need);
+
+	hipStream_t st = pz::as_stream(stream);
+	const int size = d->dtype == PZ_F16 ? 2 : 4;
+	char *ws = (char *)workspace;
+	float *sums = (float *)(ws + p.dz_bytes);
+	const void *dz = p.write_dz ? (const void *)ws : dy;
+	const long lddz = p.write_dz ? padded(d->n) : d->ldy;
+	const int wide = p.write_dz ? padded(d->n) : d->n;
+
+	if (d->m > 0 && (p.write_dz || db)) {
+		Gate g{};
+		g.dy = dy, g.preact = preact, g.dz = p.write_dz ? ws : nullptr, g.sums = db ? sums : nullptr;
+		g.lddy = d->ldy, g.ldp = d->ldp, g.lddz = lddz;
+		g.m = d->m, g.n = d->n, g.act = d->act, g.dropping = mask != nullptr, g.rows_per_block = p.rows_per_block;
+		g.vec = runs_ok(dy, d->ldy, size) && (d->act == PZ_ACT_NONE || runs_ok(preact, d->ldp, size));
+		g.drop = key_of(mask);
+		const dim3 grid((unsigned)pz::ceil_div(d->n, 512), (unsigned)p.row_blocks);
+		if (d->dtype == PZ_F16) linear_gate_kernel<f16><<<grid, 256, 0, st>>>(g);
+		else linear_gate_kernel<float><<<grid, 256, 0, st>>>(g);
+		PZ_LAUNCH_CHECK();
+	}
+	if (db) {
+		linear_bias_grad_kernel<<<pz::ceil_div(d->n, 256), 256, 0, st>>>(sums, p.row_blocks, d->n, db, alpha, beta);
+		PZ_LAUNCH_CHECK();
+	}
+	ws += p.dz_bytes + p.sum_bytes;
+	if (dx) {
+		Epilogue e{};
+		e.out = dx, e.ldo = d->ldr, e.kind = EPI_ACCUMULATE, e.alpha = 1.f, e.vec = runs_ok(dx, d->ldr, size);
+		if (int rc = product(d->dtype, data_operands(d, dz, lddz, wide, w), e, ws, st)) return rc;
+	}
+	if (dw) {
+		Epilogue e{};
+		e.out = dw, e.ldo = d->trans_w ? d->k : d->n, e.kind = EPI_ACCUMULATE, e.alpha = alpha, e.beta = beta, e.out_f32 = dw_dtype == PZ_F32;
+		e.vec = runs_ok(dw, e.ldo, e.out_f32 ? 4 : 2) && (!e.out_f32 || e.ldo % (16 / size) == 0);
+		if (int rc = product(d->dtype, weight_operands(d, dz, lddz, wide, x), e, ws, st)) return rc;
+	}
+	return PZ_OK;
+}
+
+}  // extern "C"

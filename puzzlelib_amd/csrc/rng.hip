@@ -3,7 +3,7 @@
 // reference's stream is seeded from numpy (Cuda/GPUBackend.py:62-63) and is not reproducible across backends either.
 // Stateless kernels: word i of call #k is philox(key = seed, counter = {i/4, k}), so fills never need a state array
 // in HBM and every launch is a pure streaming write.
-#include "common.h"
+#include "philox.h"
 
 struct pz_rng {
 	uint64_t seed;
@@ -11,19 +11,6 @@ struct pz_rng {
 };
 
 namespace {
-
-__device__ __forceinline__ uint4 philox4x32_10(uint4 ctr, uint2 key) {
-	constexpr uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-	for (int r = 0; r < 10; ++r) {
-		const uint32_t hi0 = __umulhi(M0, ctr.x), lo0 = M0 * ctr.x;
-		const uint32_t hi1 = __umulhi(M1, ctr.z), lo1 = M1 * ctr.z;
-		ctr = make_uint4(hi1 ^ ctr.y ^ key.x, lo1, hi0 ^ ctr.w ^ key.y, lo0);
-		key.x += W0;
-		key.y += W1;
-	}
-	return ctr;
-}
 
 __device__ __forceinline__ float u01(uint32_t w) { return ((float)(w >> 8) + 1.0f) * (1.0f / 16777216.0f); }   // (0, 1]
 
@@ -83,6 +70,12 @@ int pz_rng_create(uint64_t seed, pz_rng_t *rng) {
 
 int pz_rng_destroy(pz_rng_t rng) {
 	delete rng;
+	return PZ_OK;
+}
+
+int pz_rng_reserve(pz_rng_t rng, uint64_t *seed, uint64_t *call) {
+	PZ_REQUIRE(rng && seed && call, "pz_rng_reserve: null argument");
+	*seed = rng->seed, *call = rng->calls++;
 	return PZ_OK;
 }
 

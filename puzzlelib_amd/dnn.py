@@ -21,7 +21,7 @@ from puzzlelib_amd.driver import streamHandle
 from puzzlelib_amd.gpuarray import GPUArray, prod, eltwise, contiguousStrides
 from puzzlelib_amd.common import (
 	ConvFwdAlgo, ConvBwdFilterAlgo, ConvBwdDataAlgo, PoolMode, SoftMaxMode, BatchNormMode, LRNMode, RNNMode, DirectionMode, RNNAlgo,
-	GroupFormat, ConvPerf, toAlgoId, pair, requireF32, rptrOf
+	GroupFormat, ConvPerf, FusedAct, toAlgoId, pair, requireF32, rptrOf, rowDtype, requireVector, requireDisjoint
 )
 
 
@@ -912,6 +912,114 @@ class DnnContext:
 			out.optr
 			thunk.run(out)
 		return out, savemean, saveinvvar
+
+
+	@staticmethod
+	def groupNormDesc(what, data, groups, scale, bias, epsilon, act):
+		"""data (batch, ..., channels): channels last"""
+		dtype = rowDtype(data, what)
+		if data.ndim < 2 or not data.contiguous:
+			raise ValueError("%s: contiguous data (batch, ..., channels) expected, got shape %s" % (what, data.shape))
+		n, c = data.shape[0], data.shape[-1]
+		if groups <= 0 or c == 0 or c % groups != 0:
+			raise ValueError("%s: %d channels do not form %d groups" % (what, c, groups))
+		requireVector(scale, c, what + ": scale")
+		requireVector(bias, c, what + ": bias")
+		pixels = prod(data.shape[1:-1])
+		if max(n, c, pixels) > 0x7fffffff:
+			raise ValueError("%s: shape %s is too large" % (what, data.shape))
+		return lib.GroupNormDesc(dtype, FusedAct(act).value, n, pixels, c, int(groups), float(epsilon))
+
+
+	@staticmethod
+	def groupNormStats(what, ary, desc):
+		if ary.shape != (desc.n, desc.groups) or ary.dtype != np.float32 or not ary.contiguous:
+			raise ValueError("%s: contiguous float32 %s expected, got %s %s" % (what, (desc.n, desc.groups), ary.dtype, ary.shape))
+
+
+	def groupNormNd(self, data, scale, bias, groups, epsilon=1e-5, act=FusedAct.none, test=False, out=None, savemean=None,
+					saveinvvar=None, allocator=None):
+		"""Group normalisation of channels-last data (batch, ..., channels) with an activation behind it (float32 or float16 data;
+		scale and bias, float32 or None, per channel): out, or (out, savemean, saveinvvar) unless `test` — the shape of batchNormNd's
+		answer, with statistics per (sample, group). `out` may be `data`."""
+		desc = self.groupNormDesc("groupNormNd", data, groups, scale, bias, epsilon, act)
+		if out is None:
+			out = GPUArray.empty(data.shape, dtype=data.dtype, allocator=allocator)
+		else:
+			if out.shape != data.shape or out.dtype != data.dtype or not out.contiguous:
+				raise ValueError("groupNormNd: out is %s %s, expected contiguous %s %s" % (out.shape, out.dtype, data.shape, data.dtype))
+			requireDisjoint("groupNormNd: out", out, None if lazy.sameBuffer(out, data) else data, scale, bias)
+		if not test:
+			stats = []
+			for name, ary in (("savemean", savemean), ("saveinvvar", saveinvvar)):
+				if ary is None:
+					ary = GPUArray.empty((desc.n, desc.groups), dtype=np.float32, allocator=allocator)
+				else:
+					self.groupNormStats("groupNormNd: " + name, ary, desc)
+					requireDisjoint("groupNormNd: " + name, ary, data, out, scale, bias, *stats)
+				stats.append(ary)
+			savemean, saveinvvar = stats
+		else:
+			savemean = saveinvvar = None
+
+		if data.size == 0:
+			for ary in () if test else (savemean, saveinvvar):
+				if ary.size > 0:
+					ary.fill(0)                                     # statistics of no values: defined, never read
+		else:
+			size = c_size_t(0)
+			lib.pz_groupnorm_workspace_bytes(byref(desc), 0, byref(size))
+			ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+			xptr, sptr, bptr = data.rptr, rptrOf(scale), rptrOf(bias)
+			lib.pz_groupnorm_fwd(
+				byref(desc), xptr, sptr, bptr, out.wptr if lazy.sameBuffer(out, data) else out.optr,
+				None if savemean is None else savemean.optr, None if saveinvvar is None else saveinvvar.optr,
+				None if ws is None else ws.optr, size.value, None
+			)
+		return out if test else (out, savemean, saveinvvar)
+
+
+	def groupNormNdBackward(self, grad, data, scale, bias, savemean, saveinvvar, groups, act=FusedAct.none, out=None, scalegrad=None,
+							bgrad=None, affine=True, allocator=None):
+		"""(ingrad, scalegrad, bgrad) of groupNormNd from its input and saved statistics (batchNormNdBackward's answer); ingrad alone
+		without `affine`. `out` may be `grad` or `data`."""
+		desc = self.groupNormDesc("groupNormNdBackward", data, groups, scale, bias, 0.0, act)
+		if grad.shape != data.shape or grad.dtype != data.dtype or not grad.contiguous:
+			raise ValueError("groupNormNdBackward: grad is %s %s, expected contiguous %s %s" % (grad.shape, grad.dtype, data.shape, data.dtype))
+		self.groupNormStats("groupNormNdBackward: savemean", savemean, desc)
+		self.groupNormStats("groupNormNdBackward: saveinvvar", saveinvvar, desc)
+		if out is None:
+			out = GPUArray.empty(data.shape, dtype=data.dtype, allocator=allocator)
+		else:
+			if out.shape != data.shape or out.dtype != data.dtype or not out.contiguous:
+				raise ValueError("groupNormNdBackward: out is %s %s, expected contiguous %s %s" % (out.shape, out.dtype, data.shape, data.dtype))
+			requireDisjoint("groupNormNdBackward: out", out, *[
+				None if lazy.sameBuffer(out, ary) else ary for ary in (grad, data)
+			], scale, bias, savemean, saveinvvar)
+		if affine:
+			grads = []
+			for name, ary in (("scalegrad", scalegrad), ("bgrad", bgrad)):
+				if ary is None:
+					ary = GPUArray.empty((desc.c, ), dtype=np.float32, allocator=allocator)
+				else:
+					requireVector(ary, desc.c, "groupNormNdBackward: " + name)
+					requireDisjoint("groupNormNdBackward: " + name, ary, grad, data, scale, bias, savemean, saveinvvar, out, *grads)
+				grads.append(ary)
+			scalegrad, bgrad = grads
+		else:
+			scalegrad = bgrad = None
+
+		size = c_size_t(0)
+		lib.pz_groupnorm_workspace_bytes(byref(desc), 1, byref(size))
+		ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+		gptr, xptr, sptr, bptr, mptr, vptr = grad.rptr, data.rptr, rptrOf(scale), rptrOf(bias), savemean.rptr, saveinvvar.rptr
+		inplace = lazy.sameBuffer(out, grad) or lazy.sameBuffer(out, data)
+		lib.pz_groupnorm_bwd(
+			byref(desc), gptr, xptr, sptr, bptr, mptr, vptr, out.wptr if inplace else out.optr,
+			None if scalegrad is None else scalegrad.optr, None if bgrad is None else bgrad.optr, None if ws is None else ws.optr,
+			size.value, None
+		)
+		return (out, scalegrad, bgrad) if affine else out
 
 
 	def batchNormNdBackward(self, grad, data, scale, savemean=None, saveinvvar=None, epsilon=1e-5,

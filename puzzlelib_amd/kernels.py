@@ -13,6 +13,7 @@ from puzzlelib_amd import lib, driver, lazy, fusion
 from puzzlelib_amd.lib import HipError, ConvDesc, PoolDesc
 from puzzlelib_amd.driver import streamHandle
 from puzzlelib_amd.gpuarray import GPUArray, prod, eltwise, contiguousStrides
+from puzzlelib_amd.common import DropoutMask, ROW_DTYPES, rowDtype, requireDisjoint
 
 
 def absorbRelu(arrays, scalars):
@@ -217,3 +218,46 @@ class AddKernelFactory:
 			lazy.deferAdd(out, x, y, alpha, beta)            # runs with its neighbours in one launch (lazy.flushSmall)
 			return
 		eltwise(lib.OP_ADD, out.size, (out, x, y), np.array([alpha, beta], dtype=np.float32), slc=slice, stream=stream)
+
+
+class CounterDropoutFactory:
+	"""counterDropoutKer(dtype)(outdata, indata, mask, residual=None): outdata = residual + indata * keep / (1 - p), the mask computed
+	from its key (common.DropoutMask) instead of read — beside dropoutKer (Cuda/Kernels/ElementWise.py:495-536), with the same words.
+	The backward pass is the same call with the gradients. outdata may be indata or residual; float32 and float16."""
+
+	def __call__(self, dtype):
+		if np.dtype(dtype) not in ROW_DTYPES:
+			raise NotImplementedError("counterDropoutKer: dtype %s" % dtype)
+		return self.launch
+
+	@staticmethod
+	def launch(outdata, indata, mask, residual=None, slice=None, stream=None):
+		if slice is not None:
+			raise ValueError("counterDropoutKer takes whole tensors")
+		if not isinstance(mask, DropoutMask):
+			raise ValueError("counterDropoutKer: a DropoutMask expected, got %r" % (mask, ))
+		dtype = rowDtype(outdata, "counterDropoutKer")
+		arrays = (indata, ) if residual is None else (indata, residual)
+		for ary in arrays + (outdata, ):
+			if ary.dtype != outdata.dtype or ary.size != outdata.size:
+				raise ValueError("counterDropoutKer: %s %s does not match %s %s" % (ary.dtype, ary.shape, outdata.dtype, outdata.shape))
+			if not ary.contiguous:
+				raise ValueError("gpuarray is not contiguous")
+		for ary in arrays:
+			if not lazy.sameBuffer(ary, outdata):
+				requireDisjoint("counterDropoutKer: outdata", outdata, ary)
+		if outdata.size == 0:
+			return
+
+		if stream is None:
+			ptrs = [ary.rptr for ary in arrays]
+			outptr = outdata.wptr if any(lazy.sameBuffer(ary, outdata) for ary in arrays) else outdata.optr
+		else:
+			ptrs = [ary.ptrOn(stream, False) for ary in arrays]
+			outptr = outdata.ptrOn(stream, True)
+			ready = lazy.foreignBegin(stream)
+		lib.pz_dropout(
+			dtype, ptrs[0], ptrs[1] if residual is not None else None, outptr, outdata.size, byref(mask.key), streamHandle(stream)
+		)
+		if stream is not None:
+			lazy.foreignEnd(stream, ready, reads=arrays, writes=(outdata, ))

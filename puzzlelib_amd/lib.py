@@ -41,6 +41,20 @@ class PoolDesc(ctypes.Structure):
 	)]
 
 
+class DropoutKey(ctypes.Structure):         # struct pz_dropout_mask
+	_fields_ = [("seed", c_uint64), ("call", c_uint64), ("threshold", c_uint32), ("keep", c_float)]
+
+
+class LinearDesc(ctypes.Structure):
+	_fields_ = [(name, c_int) for name in ("dtype", "act", "trans_w", "m", "n", "k")] + [
+		(name, c_int64) for name in ("ldx", "ldw", "ldy", "ldr", "ldp")
+	]
+
+
+class GroupNormDesc(ctypes.Structure):
+	_fields_ = [(name, c_int) for name in ("dtype", "act", "n", "pixels", "c", "groups")] + [("epsilon", c_float)]
+
+
 # Dry run (PUZZLE_MI355_DRYRUN=1, host-logic tests only): the library is loaded for its host-side queries (output shapes,
 # workspace sizes, kernel-family resolution) but nothing that needs a device is called — allocations hand out fake
 # addresses and every launch is appended to `trace` as (entry point, non-pointer arguments). Lets the whole Python side
@@ -231,6 +245,17 @@ _PROTOS = {
 	"pz_rng_fill_uniform": [P, P, c_size_t, P],
 	"pz_rng_fill_normal": [P, P, c_size_t, c_float, c_float, P],
 
+	"pz_rng_reserve": [P, POINTER(c_uint64), POINTER(c_uint64)],
+
+	"pz_dropout": [c_int, P, P, P, c_size_t, POINTER(DropoutKey), P],
+	"pz_linear_fwd_workspace_bytes": [POINTER(LinearDesc), P, P, POINTER(c_size_t)],
+	"pz_linear_fwd": [POINTER(LinearDesc), P, P, P, P, POINTER(DropoutKey), P, P, P, c_size_t, P],
+	"pz_linear_bwd_workspace_bytes": [POINTER(LinearDesc), P, P, P, c_int, c_int, c_int, c_int, POINTER(c_size_t)],
+	"pz_linear_bwd": [POINTER(LinearDesc), P, P, P, P, POINTER(DropoutKey), P, P, c_int, P, c_float, c_float, P, c_size_t, P],
+	"pz_groupnorm_workspace_bytes": [POINTER(GroupNormDesc), c_int, POINTER(c_size_t)],
+	"pz_groupnorm_fwd": [POINTER(GroupNormDesc), P, P, P, P, P, P, P, c_size_t, P],
+	"pz_groupnorm_bwd": [POINTER(GroupNormDesc), P, P, P, P, P, P, P, P, P, P, c_size_t, P],
+
 	"pz_rtc_compile": [c_char_p, c_char_p, POINTER(c_char_p), c_int, PP, POINTER(c_size_t), c_char_p, c_size_t],
 	"pz_rtc_free_code": [P],
 	"pz_module_load": [P, PP],
@@ -293,6 +318,7 @@ _HOST_ONLY = {
 	"pz_conv2d_bn_fold_supported", "pz_conv2d_bwd_data_bnstats_bytes", "pz_conv2d_xbn_supported", "pz_conv2d_fwd_bn_supported", "pz_bn_workspace_bytes", "pz_relu_mask_bytes",
 	"pz_pool2d_out_shape", "pz_pool2d_fwd_bn_supported", "pz_pool_oom_events", "pz_pool_driver_allocs", "pz_gemm_workspace_bytes", "pz_conv_math_set", "pz_conv_math_get",
 	"pz_conv_winograd_tile_set", "pz_conv_winograd_tile_get",
+	"pz_linear_fwd_workspace_bytes", "pz_linear_bwd_workspace_bytes", "pz_groupnorm_workspace_bytes",
 	"pz_rtc_compile", "pz_rtc_free_code"                  # (hiprtc compiles for gfx950 without a device)
 }
 _fake = {"next": 0x7000_0000_0000}
@@ -329,6 +355,10 @@ def _dry(name, argtypes):
 			_store(args[0], _fakeHandle())
 		elif name == "pz_rng_create":
 			_store(args[1], _fakeHandle())
+		elif name == "pz_rng_reserve":
+			_fake["calls"] = _fake.get("calls", -1) + 1
+			_store(args[1], 0)
+			_store(args[2], _fake["calls"])
 		elif name == "pz_comm_init_rank":
 			_store(args[0], _fakeHandle())
 			_fake["comm"] = (int(args[1]), int(args[3]))
@@ -474,6 +504,8 @@ COST_BCE, COST_HINGE, COST_SMOOTH_L1, COST_L1_HINGE = 0, 1, 2, 3
 CONV_ALGO_AUTO, CONV_ALGO_DIRECT, CONV_ALGO_WINOGRAD, CONV_ALGO_IMPLICIT_GEMM = -1, 1, 3, 5
 CONV_FWD, CONV_BWD_DATA, CONV_BWD_FILTER = 0, 1, 2
 BN_ACT_NONE, BN_ACT_RELU = 0, 1
+F32, F16 = 0, 1
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
 
 
 def declaredSymbols():

@@ -20,7 +20,382 @@ struct Norm {
 
 __device__ __forceinline__ float or_else(const float *p, int i, float v) { return p ? p[i] : v; }
 
-// One workgroup per (sample, group), three sweeps over its values: any shape. Threads take consecutive channels of consecutive pixels.
+// ---- where the values of a workgroup lie ----------------------------------------------------------------------------------------------
+// A workgroup holds `rows` rows of `width` consecutive values, `pitch` apart, as 16-byte vectors in registers: thread (tx, ty) the
+// vectors at tx * V of the rows ty, ty + TY, ... — its channels never change, so scale, bias and statistics are fetched once. Either
+//  - a row is a pixel's slab of channels (whole groups, at least a cache line where the shape gives one), pitch c; or
+//  - the pixels lie back to back: a row is lcm(c, V) values (`reps` pixels), whatever c is; what lies beyond `limit` does not exist.
+struct Slab {
+	int width, tx, reps, slabs, uniform;         // uniform: every vector lies inside one group
+	long pitch;
+	long rows, limit;                            // of one chunk (the last may be shorter); limit: values of one sample
+	int chunks;
+	int paired;                                  // workgroups b and b + 8 (one XCD, hence one L2) take the two halves of a cache line
+	int wd, period;                              // values of a group and of all channels in a row's cells (below)
+};
+
+template <typename T>
+struct Vec {
+	static constexpr int V = 16 / sizeof(T);
+	typedef T raw __attribute__((ext_vector_type(V), aligned(sizeof(T))));       // (any alignment of whole elements)
+};
+
+template <typename T>
+__device__ __forceinline__ typename Vec<T>::raw load_vec(const T *p, long left) {
+	constexpr int V = Vec<T>::V;
+	typename Vec<T>::raw v;
+	if (left >= V) return *reinterpret_cast<const typename Vec<T>::raw *>(p);
+#pragma unroll
+	for (int e = 0; e < V; ++e) v[e] = e < left ? p[e] : (T)0.f;
+	return v;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_vec(T *p, long left, const float (&v)[Vec<T>::V]) {
+	constexpr int V = Vec<T>::V;
+	if (left >= V) {
+		typename Vec<T>::raw x;
+#pragma unroll
+		for (int e = 0; e < V; ++e) x[e] = (T)v[e];
+		*reinterpret_cast<typename Vec<T>::raw *>(p) = x;
+	} else {
+#pragma unroll
+		for (int e = 0; e < V; ++e)
+			if (e < left) p[e] = (T)v[e];
+	}
+}
+
+// The vectors of a thread: rows ty, ty + TY, ...: `mine` of them, the last one with `last` values (V unless the data ends inside it)
+__device__ __forceinline__ void share(const Slab &s, bool active, int ty, int TY, int col, int v, long rows, long all, int most, int &mine, int &last) {
+	mine = active && ty < rows ? (int)min((long)most, (rows - ty + TY - 1) / TY) : 0;
+	last = v;
+	if (mine > 0 && s.slabs == 1) {
+		const long left = all - (ty + (long)(mine - 1) * TY) * s.pitch - col;
+		if (left <= 0) mine -= 1;                    // (only the last row ends early: the one before it is whole)
+		else if (left < v) last = (int)left;
+	}
+}
+
+// Sums of cells in LDS: red[row * across + cell], `rows` rows; output o takes the cells rep * period + o * wd ... + wd - 1, rep < reps, of
+// every row. Each output is added by up to 64 lanes in a fixed order; out[o] = sum * factor. All threads call it; the caller has synchronised.
+template <int NT>
+__device__ void sum_cells(const float *red, int across, int rows, int reps, int period, int wd, int outputs, float factor, float *out) {
+	int lanes = 64;
+	while (lanes > 1 && lanes * outputs > NT) lanes >>= 1;
+	const int items = rows * reps * wd, sub = threadIdx.x % lanes;
+	for (int o0 = 0; o0 < outputs; o0 += NT / lanes) {
+		const int o = o0 + threadIdx.x / lanes;
+		float s = 0.f;
+		if (o < outputs)
+			for (int t = sub; t < items; t += lanes) {
+				const int i = t % wd, rest = t / wd;
+				s += red[(rest / reps) * across + (rest % reps) * period + o * wd + i];
+			}
+		for (int l = lanes >> 1; l > 0; l >>= 1) s += __shfl_xor(s, l, 64);
+		if (o < outputs && sub == 0) out[o] = s * factor;
+	}
+}
+
+constexpr int kMaxWidth = 2048;                  // values of a row of a slab
+
+// ---- forward: statistics, and with FINISH the normalised values, from one read ---------------------------------------------------------
+// PART (FINISH = false): {mean, sum of centred squares} of the chunk's groups, for norm_join_kernel.
+template <typename T, int NT, int NV, bool UNI, bool FINISH>
+__global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *part) {
+	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
+	__shared__ float red[NT * CELLS];
+	__shared__ float smean[UNI ? NT : kMaxWidth], sinv[UNI ? NT : kMaxWidth];      // (vectors inside one group: no more groups than vectors in a row)
+	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = NT / s.tx;
+	const unsigned item = s.paired ? (blockIdx.x / 16 * 8 + blockIdx.x % 8) * 2 + blockIdx.x / 8 % 2 : blockIdx.x;
+	const int slab = item % s.slabs;
+	const long rest = item / s.slabs, sample = rest / s.chunks;
+	const int chunk = (int)(rest % s.chunks);
+	const int c0 = slab * s.width;                                              // (one slab: 0)
+	const int groups = s.slabs > 1 ? s.width / g.width : g.groups, group0 = c0 / g.width;
+	const size_t start = (size_t)sample * g.pixels * g.c + c0 + (size_t)chunk * s.rows * s.pitch;
+	const T *x = (const T *)g.x + start;
+	// one slab: values of the sample from this chunk on; several: every row is whole and there is one chunk
+	const long all = s.slabs > 1 ? (long)1 << 62 : s.limit - (long)chunk * s.rows * s.pitch;
+	const long rows = min(s.rows, s.slabs > 1 ? s.rows : (all + s.pitch - 1) / s.pitch);
+	const long count = s.slabs > 1 ? rows * g.width : min(all, s.rows * s.pitch) / g.c * g.width;        // values of a group here
+	const bool active = ty < TY;
+
+	typename Vec<T>::raw v[NV];
+	int mine, last;
+	share(s, active, ty, TY, tx * V, V, rows, all, NV, mine, last);
+#pragma unroll
+	for (int k = 0; k < NV; ++k)
+		if (k < mine) v[k] = load_vec(x + (ty + (long)k * TY) * s.pitch + tx * V, k + 1 < mine ? V : last);
+
+	float acc[CELLS];
+	auto cells = [&](auto value) {                                              // red <- per-thread sums of value(x, cell)
+#pragma unroll
+		for (int e = 0; e < CELLS; ++e) acc[e] = 0.f;
+#pragma unroll
+		for (int k = 0; k < NV; ++k) {
+			if (k + 1 < mine || (k < mine && last == V)) {
+#pragma unroll
+				for (int e = 0; e < V; ++e) acc[UNI ? 0 : e] += value((float)v[k][e], e);
+			} else if (k < mine) {
+#pragma unroll
+				for (int e = 0; e < V; ++e)
+					if (e < last) acc[UNI ? 0 : e] += value((float)v[k][e], e);
+			}
+		}
+		if (active) {
+#pragma unroll
+			for (int e = 0; e < CELLS; ++e) red[(ty * s.tx + tx) * CELLS + e] = acc[e];
+		}
+		__syncthreads();
+	};
+
+	cells([](float f, int) { return f; });
+	sum_cells<NT>(red, s.tx * CELLS, TY, s.reps, s.period, s.wd, groups, 1.f / (float)count, smean);
+	__syncthreads();
+
+	float mean[CELLS];
+#pragma unroll
+	for (int e = 0; e < CELLS; ++e) mean[e] = smean[(tx * V + e) % g.c / g.width];
+	cells([&](float f, int e) {
+		const float d = f - mean[UNI ? 0 : e];
+		return d * d;
+	});
+	sum_cells<NT>(red, s.tx * CELLS, TY, s.reps, s.period, s.wd, groups, 1.f, sinv);
+	__syncthreads();
+
+	if (!FINISH) {
+		for (int o = threadIdx.x; o < groups; o += NT)
+			part[((size_t)sample * s.chunks + chunk) * g.groups + group0 + o] = make_float2(smean[o], sinv[o]);
+		return;
+	}
+	for (int o = threadIdx.x; o < groups; o += NT) {
+		const float inv = 1.f / sqrtf(sinv[o] / (float)count + g.epsilon);
+		sinv[o] = inv;
+		if (g.mean) g.mean[(size_t)sample * g.groups + group0 + o] = smean[o];
+		if (g.invvar) g.invvar[(size_t)sample * g.groups + group0 + o] = inv;
+	}
+	__syncthreads();
+	if (!active) return;
+
+	float scale[V], bias[V];
+#pragma unroll
+	for (int e = 0; e < V; ++e) {
+		const int ch = (tx * V + e) % g.c;                                        // channel inside the slab
+		scale[e] = or_else(g.scale, c0 + ch, 1.f) * sinv[ch / g.width];
+		bias[e] = or_else(g.bias, c0 + ch, 0.f);
+	}
+	T *y = (T *)g.out + start;
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		if (k >= mine) continue;
+		float o[V];
+#pragma unroll
+		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], g.act);
+		store_vec(y + (ty + (long)k * TY) * s.pitch + tx * V, k + 1 < mine ? V : last, o);
+	}
+}
+
+// mean and 1 / sqrt(var + epsilon) of a (sample, group) from its chunks' {mean, centred squares}: a wave each, float64 sums
+__global__ void __launch_bounds__(256) norm_join_kernel(Norm g, Slab s, const float2 *part, float *mean, float *invvar) {
+	const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+	if (at >= (long)g.n * g.groups) return;
+	const int lane = threadIdx.x & 63;
+	const long sample = at / g.groups, group = at % g.groups, each = s.rows * s.pitch / g.c * g.width, total = (long)g.pixels * g.width;
+	auto sum = [](double v) {
+		for (int l = 32; l > 0; l >>= 1) v += __shfl_xor(v, l, 64);
+		return v;
+	};
+	double m = 0.0, q = 0.0;
+	for (int k = lane; k < s.chunks; k += 64) m += (double)min(each, total - k * each) * part[((size_t)sample * s.chunks + k) * g.groups + group].x;
+	m = sum(m) / (double)total;
+	for (int k = lane; k < s.chunks; k += 64) {
+		const float2 p = part[((size_t)sample * s.chunks + k) * g.groups + group];
+		const double d = p.x - m;
+		q += p.y + (double)min(each, total - k * each) * d * d;
+	}
+	q = sum(q) / (double)total;
+	if (lane == 0) mean[at] = (float)m, invvar[at] = (float)(1.0 / sqrt(q + (double)g.epsilon));
+}
+
+// y from x and the statistics, a chunk of rows back to back
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) norm_apply_kernel(Norm g, Slab s, const float *means, const float *invvars) {
+	constexpr int V = Vec<T>::V;
+	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = 256 / s.tx;
+	if (ty >= TY) return;
+	const long sample = blockIdx.x / s.chunks, row0 = (long)(blockIdx.x % s.chunks) * s.rows;
+	const size_t start = (size_t)sample * g.pixels * g.c;
+	const T *x = (const T *)g.x + start;
+	T *y = (T *)g.out + start;
+	float mean[V], scale[V], bias[V];
+#pragma unroll
+	for (int e = 0; e < V; ++e) {
+		const int ch = (tx * V + e) % g.c;
+		const size_t at = sample * g.groups + ch / g.width;
+		mean[e] = means[at], scale[e] = or_else(g.scale, ch, 1.f) * invvars[at], bias[e] = or_else(g.bias, ch, 0.f);
+	}
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		const long r = ty + (long)k * TY, at = (row0 + r) * s.pitch + tx * V, left = r < s.rows ? s.limit - at : 0;
+		if (left <= 0) continue;
+		const typename Vec<T>::raw v = load_vec(x + at, left);
+		float o[V];
+#pragma unroll
+		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[e] - mean[e]) * scale[e] + bias[e], g.act);
+		store_vec(y + at, left, o);
+	}
+}
+
+// ---- backward ---------------------------------------------------------------------------------------------------------------------------
+// Sums over a chunk's pixels per channel, sums[((sample * chunks + chunk) * 2 + {0: da, 1: da xhat}) * c + channel], and with FINISH dx from
+// the same registers.
+template <typename T, int NT, int NV, bool UNI, bool FINISH>
+__global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float *sums) {
+	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
+	__shared__ float red[2][NT * V];
+	__shared__ float chan[2][kMaxWidth];
+	__shared__ float sa[UNI ? NT : kMaxWidth], sb[UNI ? NT : kMaxWidth];
+	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = NT / s.tx;
+	const unsigned item = s.paired ? (blockIdx.x / 16 * 8 + blockIdx.x % 8) * 2 + blockIdx.x / 8 % 2 : blockIdx.x;
+	const int slab = item % s.slabs;
+	const long rest = item / s.slabs, sample = rest / s.chunks;
+	const int chunk = (int)(rest % s.chunks);
+	const int c0 = slab * s.width;
+	const int channels = s.slabs > 1 ? s.width : g.c, groups = channels / g.width, group0 = c0 / g.width;
+	const size_t start = (size_t)sample * g.pixels * g.c + c0 + (size_t)chunk * s.rows * s.pitch;
+	const T *x = (const T *)g.x + start, *dy = (const T *)g.dy + start;
+	const long all = s.slabs > 1 ? (long)1 << 62 : s.limit - (long)chunk * s.rows * s.pitch;
+	const long rows = min(s.rows, s.slabs > 1 ? s.rows : (all + s.pitch - 1) / s.pitch);
+	const bool active = ty < TY;
+
+	typename Vec<T>::raw v[NV], d[NV];
+	int mine, last;
+	share(s, active, ty, TY, tx * V, V, rows, all, NV, mine, last);
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		const long at = (ty + (long)k * TY) * s.pitch + tx * V;
+		const int left = k + 1 < mine ? V : last;
+		if (k < mine) v[k] = load_vec(x + at, left), d[k] = load_vec(dy + at, left);      // (beyond the end: zeros, which add nothing)
+	}
+	float mean[CELLS], inv[CELLS], scale[V], bias[V], da[V], db[V];
+#pragma unroll
+	for (int e = 0; e < V; ++e) {
+		const int ch = (tx * V + e) % g.c;
+		const size_t at = sample * g.groups + group0 + ch / g.width;
+		if (!UNI || e == 0) mean[UNI ? 0 : e] = g.mean[at], inv[UNI ? 0 : e] = g.invvar[at];
+		scale[e] = or_else(g.scale, c0 + ch, 1.f), bias[e] = or_else(g.bias, c0 + ch, 0.f);
+		da[e] = db[e] = 0.f;
+	}
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		if (k >= mine) continue;
+#pragma unroll
+		for (int e = 0; e < V; ++e) {
+			const float xhat = ((float)v[k][e] - mean[UNI ? 0 : e]) * inv[UNI ? 0 : e];
+			const float t = (float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act);
+			da[e] += t, db[e] += t * xhat;
+		}
+	}
+	if (active) {
+#pragma unroll
+		for (int e = 0; e < V; ++e) red[0][(ty * s.tx + tx) * V + e] = da[e], red[1][(ty * s.tx + tx) * V + e] = db[e];
+	}
+	__syncthreads();
+	for (int i = 0; i < 2; ++i) sum_cells<NT>(red[i], s.tx * V, TY, s.reps, g.c, 1, channels, 1.f, chan[i]);
+	__syncthreads();
+	if (sums)
+		for (int i = threadIdx.x; i < 2 * channels; i += NT)
+			sums[(((size_t)sample * s.chunks + chunk) * 2 + i / channels) * g.c + c0 + i % channels] = chan[i / channels][i % channels];
+	if (!FINISH) return;
+
+	__syncthreads();
+	for (int i = threadIdx.x; i < channels; i += NT) {
+		const float f = or_else(g.scale, c0 + i, 1.f);
+		chan[0][i] *= f, chan[1][i] *= f;
+	}
+	__syncthreads();
+	const float one = 1.f / ((float)g.pixels * (float)g.width);
+	sum_cells<NT>(chan[0], 0, 1, 1, 0, g.width, groups, one, sa);
+	sum_cells<NT>(chan[1], 0, 1, 1, 0, g.width, groups, one, sb);
+	__syncthreads();
+	if (!active) return;
+	float a[CELLS], b[CELLS];
+#pragma unroll
+	for (int e = 0; e < CELLS; ++e) {
+		const int group = (tx * V + e) % g.c / g.width;
+		a[e] = sa[group], b[e] = sb[group];
+	}
+	T *dx = (T *)g.out + start;
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		if (k >= mine) continue;
+		float o[V];
+#pragma unroll
+		for (int e = 0; e < V; ++e) {
+			const int u = UNI ? 0 : e;
+			const float xhat = ((float)v[k][e] - mean[u]) * inv[u];
+			const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act));
+			o[e] = inv[u] * (t - a[u] - xhat * b[u]);
+		}
+		store_vec(dx + (ty + (long)k * TY) * s.pitch + tx * V, k + 1 < mine ? V : last, o);
+	}
+}
+
+// A and B of the head, divided by m, of a (sample, group) from its chunks' channel sums: a wave each
+__global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, const float *sums, float2 *ab) {
+	const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+	if (at >= (long)g.n * g.groups) return;
+	const int lane = threadIdx.x & 63;
+	const long sample = at / g.groups;
+	const int c0 = (int)(at % g.groups) * g.width;
+	double a = 0.0, b = 0.0;
+	for (long i = lane; i < (long)s.chunks * g.width; i += 64) {
+		const int ch = c0 + (int)(i % g.width);
+		const float *p = sums + ((size_t)sample * s.chunks + i / g.width) * 2 * g.c + ch;
+		const double f = or_else(g.scale, ch, 1.f);
+		a += f * p[0], b += f * p[g.c];
+	}
+	for (int l = 32; l > 0; l >>= 1) a += __shfl_xor(a, l, 64), b += __shfl_xor(b, l, 64);
+	const double m = (double)g.pixels * g.width;
+	if (lane == 0) ab[at] = make_float2((float)(a / m), (float)(b / m));
+}
+
+template <typename T, int NV>
+__global__ void __launch_bounds__(256) norm_apply_bwd_kernel(Norm g, Slab s, const float2 *ab) {
+	constexpr int V = Vec<T>::V;
+	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = 256 / s.tx;
+	if (ty >= TY) return;
+	const long sample = blockIdx.x / s.chunks, row0 = (long)(blockIdx.x % s.chunks) * s.rows;
+	const size_t start = (size_t)sample * g.pixels * g.c;
+	const T *x = (const T *)g.x + start, *dy = (const T *)g.dy + start;
+	T *dx = (T *)g.out + start;
+	float mean[V], inv[V], scale[V], bias[V];
+	float2 sum[V];
+#pragma unroll
+	for (int e = 0; e < V; ++e) {
+		const int ch = (tx * V + e) % g.c;
+		const size_t at = sample * g.groups + ch / g.width;
+		mean[e] = g.mean[at], inv[e] = g.invvar[at], scale[e] = or_else(g.scale, ch, 1.f), bias[e] = or_else(g.bias, ch, 0.f), sum[e] = ab[at];
+	}
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		const long r = ty + (long)k * TY, at = (row0 + r) * s.pitch + tx * V, left = r < s.rows ? s.limit - at : 0;
+		if (left <= 0) continue;
+		const typename Vec<T>::raw v = load_vec(x + at, left), d = load_vec(dy + at, left);
+		float o[V];
+#pragma unroll
+		for (int e = 0; e < V; ++e) {
+			const float xhat = ((float)v[e] - mean[e]) * inv[e];
+			const float t = scale[e] * ((float)d[e] * act_slope(scale[e] * xhat + bias[e], g.act));
+			o[e] = inv[e] * (t - sum[e].x - xhat * sum[e].y);
+		}
+		store_vec(dx + at, left, o);
+	}
+}
+
+// ---- any shape: one workgroup per (sample, group), three sweeps over its values ----------------------------------------------------------
+// Threads take consecutive channels of consecutive pixels. Only rows that no workgroup holds come here (more than kMaxWidth values in a
+// group, or a channel count whose vectors repeat later than that).
 template <typename T>
 __global__ void __launch_bounds__(256) norm_fwd_kernel(Norm g) {
 	__shared__ float red[16];
@@ -79,44 +454,52 @@ __global__ void __launch_bounds__(256) norm_bwd_kernel(Norm g) {
 	}
 }
 
-// sums over the pixels of one sample, a thread per channel: part[(sample * 2 + {0: da, 1: da * xhat}) * c + channel]
+// sums over the pixels of one sample, a thread per channel, in the layout of norm_slab_bwd_kernel
 template <typename T>
-__global__ void __launch_bounds__(256) norm_channel_kernel(Norm g, float *part) {
-	const int ch = blockIdx.x * 256 + threadIdx.x;
-	if (ch >= g.c) return;
-	const size_t sample = blockIdx.y, at = sample * g.groups + ch / g.width;
+__global__ void __launch_bounds__(256) norm_channel_kernel(Norm g, float *sums) {
+	const long at = (long)blockIdx.x * 256 + threadIdx.x;
+	if (at >= (long)g.n * g.c) return;
+	const long sample = at / g.c;
+	const int ch = (int)(at % g.c);
 	const T *x = (const T *)g.x + sample * g.pixels * g.c + ch, *dy = (const T *)g.dy + sample * g.pixels * g.c + ch;
-	const float mean = g.mean[at], invvar = g.invvar[at], scale = or_else(g.scale, ch, 1.f), bias = or_else(g.bias, ch, 0.f);
-	float s = 0.f, b = 0.f;
+	const size_t stat = sample * g.groups + ch / g.width;
+	const float mean = g.mean[stat], invvar = g.invvar[stat], scale = or_else(g.scale, ch, 1.f), bias = or_else(g.bias, ch, 0.f);
+	double s = 0.0, b = 0.0;
 	for (int p = 0; p < g.pixels; ++p) {
 		const float xhat = ((float)x[(size_t)p * g.c] - mean) * invvar;
 		const float d = (float)dy[(size_t)p * g.c] * act_slope(scale * xhat + bias, g.act);
 		b += d, s += d * xhat;
 	}
-	part[(sample * 2) * g.c + ch] = b;
-	part[(sample * 2 + 1) * g.c + ch] = s;
+	sums[(sample * 2) * g.c + ch] = (float)b;
+	sums[(sample * 2 + 1) * g.c + ch] = (float)s;
 }
 
-// dbias, dscale: the samples' sums, added in order
-__global__ void __launch_bounds__(256) norm_param_kernel(const float *part, int rows, int c, float *dscale, float *dbias) {
-	const int ch = blockIdx.x * 256 + threadIdx.x;
-	if (ch >= c) return;
-	float s = 0.f, b = 0.f;
-	for (int i = 0; i < rows; ++i) {
-		b += part[((size_t)i * 2) * c + ch];
-		s += part[((size_t)i * 2 + 1) * c + ch];
-	}
-	if (dbias) dbias[ch] = b;
-	if (dscale) dscale[ch] = s;
+// dbias, dscale: the samples' (and chunks') sums, added in a fixed order in float64. A workgroup takes 64 channels, 16 rows at a time.
+__global__ void __launch_bounds__(1024) norm_param_kernel(const float *sums, long rows, int c, float *dscale, float *dbias) {
+	__shared__ double part[2][16][64];
+	const int ch = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x & 63, row = threadIdx.x >> 6;
+	double s = 0.0, b = 0.0;
+	if (ch < c)
+		for (long i = row; i < rows; i += 16) {
+			b += sums[(size_t)i * 2 * c + ch];
+			s += sums[((size_t)i * 2 + 1) * c + ch];
+		}
+	part[0][row][lane] = b, part[1][row][lane] = s;
+	__syncthreads();
+	if (row > 0 || ch >= c) return;
+	for (int i = 1; i < 16; ++i) b += part[0][i][lane], s += part[1][i][lane];
+	if (dbias) dbias[ch] = (float)b;
+	if (dscale) dscale[ch] = (float)s;
 }
 
+// ---- host --------------------------------------------------------------------------------------------------------------------------------
 int check(const pz_groupnorm_desc *d, const char *who) {
 	PZ_REQUIRE(d, "%s: null descriptor", who);
 	PZ_REQUIRE(d->dtype == PZ_F32 || d->dtype == PZ_F16, "%s: unknown dtype %d", who, d->dtype);
 	PZ_REQUIRE(d->act >= PZ_ACT_NONE && d->act <= PZ_ACT_SILU, "%s: unknown activation %d", who, d->act);
 	PZ_REQUIRE(d->n >= 0 && d->pixels >= 0 && d->c > 0 && d->groups > 0 && d->c % d->groups == 0, "%s: bad dimensions (%d, %d, %d) in %d groups", who,
 	           d->n, d->pixels, d->c, d->groups);
-	PZ_REQUIRE((long)d->n * d->groups < (1l << 31) && d->n <= 65535, "%s: %d samples of %d groups are too many", who, d->n, d->groups);
+	PZ_REQUIRE((long)d->n * d->groups < (1l << 31) && (long)d->n * d->c < (1l << 38), "%s: %d samples of %d channels are too many", who, d->n, d->c);
 	return PZ_OK;
 }
 
@@ -127,6 +510,160 @@ Norm args_of(const pz_groupnorm_desc *d) {
 	return g;
 }
 
+long gcd(long a, long b) { return b == 0 ? a : gcd(b, a % b); }
+
+enum { WAY_PLAIN, WAY_ONE, WAY_CHUNKS };
+
+struct Plan {
+	int way, nt, nv;                 // WAY_ONE: threads and vectors a thread of the kernel that holds a sample's slab
+	Slab slab;                       // WAY_CHUNKS: of the statistics
+	Slab apply;                      // WAY_CHUNKS: of the second read
+	size_t part_bytes, stat_bytes;
+};
+
+// vectors a thread holds at most: 16 forward (64 registers), 8 + 8 backward
+constexpr int kForwardVectors = 16, kBackwardVectors = 8;
+
+Slab back_to_back(const pz_groupnorm_desc *d, int v, int threads, int vectors) {
+	Slab s{};
+	const int width = d->c / d->groups, period = (int)(d->c / gcd(d->c, v) * v);          // lcm
+	s.width = period, s.tx = period / v, s.reps = period / d->c, s.slabs = 1, s.pitch = period;
+	s.uniform = s.reps == 1 && width % v == 0;
+	s.limit = (long)d->pixels * d->c;
+	s.wd = s.uniform ? width / v : width, s.period = s.uniform ? d->c / v : d->c;
+	const long rows = (s.limit + period - 1) / period, held = (long)(threads / s.tx) * vectors;
+	s.rows = rows < held ? rows : held;
+	s.chunks = (int)((rows + s.rows - 1) / s.rows);
+	return s;
+}
+
+Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
+	Plan p{};
+	const int v = d->dtype == PZ_F16 ? 8 : 4, size = d->dtype == PZ_F16 ? 2 : 4, width = d->c / d->groups;
+	const long period = d->c / gcd(d->c, v) * v, limit = (long)d->pixels * d->c;
+	const int vectors = backward ? kBackwardVectors : kForwardVectors;
+	if (d->n == 0 || d->pixels == 0) return p;
+
+	// whole groups of a channel count that vectors divide: the narrowest slab that is a cache line wide (half a line where that is all that fits)
+	const long unit = width / gcd(width, v) * v;
+	if (d->c % v == 0 && d->c % unit == 0 && unit <= kMaxWidth) {
+		for (const long bytes : {128l, 64l}) {
+			long slab = unit;
+			while (slab * size < bytes && slab < d->c) {
+				do slab += unit;
+				while (d->c % slab != 0);
+			}
+			if (slab > kMaxWidth) continue;
+			const int tx = (int)(slab / v);
+			const bool uniform = width % v == 0;
+			for (const int nt : {256, 1024})
+				for (const int nv : {4, vectors}) {
+					if (nt == 1024 && (!uniform || nv == 4) && !(backward && uniform)) continue;
+					if (tx > nt || (long)(nt / tx) * nv < d->pixels) continue;
+					p.way = WAY_ONE, p.nt = nt, p.nv = nv;
+					Slab s{};
+					s.width = (int)slab, s.tx = tx, s.reps = 1, s.slabs = (int)(d->c / slab), s.uniform = uniform, s.pitch = d->c;
+					s.rows = d->pixels, s.limit = limit, s.chunks = 1;
+					s.paired = slab * size < 128 && (long)d->n * s.slabs % 16 == 0;
+					s.wd = uniform ? width / v : width, s.period = 0;
+					if (s.slabs == 1) s.period = uniform ? d->c / v : d->c;
+					p.slab = s;
+					return p;
+				}
+		}
+	}
+	if (period > kMaxWidth || period / v > 256) return p;                                   // WAY_PLAIN
+	for (const int nv : {4, vectors}) {
+		const Slab s = back_to_back(d, v, 256, nv);
+		if (s.chunks > 1) continue;
+		p.way = WAY_ONE, p.nt = 256, p.nv = nv, p.slab = s;
+		return p;
+	}
+	p.way = WAY_CHUNKS, p.nt = 256, p.nv = vectors;
+	p.slab = back_to_back(d, v, 256, vectors);
+	p.apply = back_to_back(d, v, 256, 4);
+	p.part_bytes = backward ? 0 : (size_t)d->n * p.slab.chunks * d->groups * sizeof(float2);
+	p.stat_bytes = (size_t)d->n * d->groups * sizeof(float2);
+	return p;
+}
+
+size_t sum_rows(const pz_groupnorm_desc *d, const Plan &p) { return (size_t)d->n * (p.way == WAY_PLAIN ? 1 : p.slab.chunks); }
+
+template <typename T, int NT, int NV, bool UNI, bool FINISH>
+void slab_fwd(const Norm &g, const Plan &p, float2 *part, hipStream_t st) {
+	norm_slab_kernel<T, NT, NV, UNI, FINISH><<<(unsigned)((long)g.n * p.slab.chunks * p.slab.slabs), NT, 0, st>>>(g, p.slab, part);
+}
+
+template <typename T>
+int forward(const pz_groupnorm_desc *d, const Norm &g, char *ws, hipStream_t st) {
+	const Plan p = plan_norm(d, false);
+	if (p.way == WAY_PLAIN) {
+		norm_fwd_kernel<T><<<d->n * d->groups, 256, 0, st>>>(g);
+		PZ_LAUNCH_CHECK();
+		return PZ_OK;
+	}
+	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_fwd: too many workgroups");
+	if (p.way == WAY_ONE) {
+		if (p.slab.uniform) {
+			if (p.nt == 1024) slab_fwd<T, 1024, 16, true, true>(g, p, nullptr, st);
+			else if (p.nv == 4) slab_fwd<T, 256, 4, true, true>(g, p, nullptr, st);
+			else slab_fwd<T, 256, 16, true, true>(g, p, nullptr, st);
+		} else if (p.nv == 4) slab_fwd<T, 256, 4, false, true>(g, p, nullptr, st);
+		else slab_fwd<T, 256, 16, false, true>(g, p, nullptr, st);
+		PZ_LAUNCH_CHECK();
+		return PZ_OK;
+	}
+	float2 *part = (float2 *)ws;
+	float *stats = (float *)(ws + p.part_bytes);
+	float *mean = g.mean ? g.mean : stats, *invvar = g.invvar ? g.invvar : stats + (size_t)d->n * d->groups;
+	PZ_REQUIRE((long)d->n * p.apply.chunks < (1l << 31), "pz_groupnorm_fwd: too many workgroups");
+	if (p.slab.uniform) slab_fwd<T, 256, 16, true, false>(g, p, part, st);
+	else slab_fwd<T, 256, 16, false, false>(g, p, part, st);
+	PZ_LAUNCH_CHECK();
+	norm_join_kernel<<<pz::ceil_div((long)d->n * d->groups, 4), 256, 0, st>>>(g, p.slab, part, mean, invvar);
+	PZ_LAUNCH_CHECK();
+	norm_apply_kernel<T, 4><<<(unsigned)((long)d->n * p.apply.chunks), 256, 0, st>>>(g, p.apply, mean, invvar);
+	PZ_LAUNCH_CHECK();
+	return PZ_OK;
+}
+
+template <typename T, int NT, int NV, bool UNI, bool FINISH>
+void slab_bwd(const Norm &g, const Plan &p, float *sums, hipStream_t st) {
+	norm_slab_bwd_kernel<T, NT, NV, UNI, FINISH><<<(unsigned)((long)g.n * p.slab.chunks * p.slab.slabs), NT, 0, st>>>(g, p.slab, sums);
+}
+
+template <typename T>
+int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, hipStream_t st) {
+	const Plan p = plan_norm(d, true);
+	if (p.way == WAY_PLAIN) {
+		if (sums) {
+			norm_channel_kernel<T><<<pz::ceil_div((long)d->n * d->c, 256), 256, 0, st>>>(g, sums);
+			PZ_LAUNCH_CHECK();
+		}
+		norm_bwd_kernel<T><<<d->n * d->groups, 256, 0, st>>>(g);
+		PZ_LAUNCH_CHECK();
+		return PZ_OK;
+	}
+	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_bwd: too many workgroups");
+	if (p.way == WAY_ONE) {
+		if (p.slab.uniform) {
+			if (p.nt == 1024) p.nv == 4 ? slab_bwd<T, 1024, 4, true, true>(g, p, sums, st) : slab_bwd<T, 1024, 8, true, true>(g, p, sums, st);
+			else p.nv == 4 ? slab_bwd<T, 256, 4, true, true>(g, p, sums, st) : slab_bwd<T, 256, 8, true, true>(g, p, sums, st);
+		} else p.nv == 4 ? slab_bwd<T, 256, 4, false, true>(g, p, sums, st) : slab_bwd<T, 256, 8, false, true>(g, p, sums, st);
+		PZ_LAUNCH_CHECK();
+		return PZ_OK;
+	}
+	PZ_REQUIRE((long)d->n * p.apply.chunks < (1l << 31), "pz_groupnorm_bwd: too many workgroups");
+	if (p.slab.uniform) slab_bwd<T, 256, 8, true, false>(g, p, sums, st);
+	else slab_bwd<T, 256, 8, false, false>(g, p, sums, st);
+	PZ_LAUNCH_CHECK();
+	norm_join_bwd_kernel<<<pz::ceil_div((long)d->n * d->groups, 4), 256, 0, st>>>(g, p.slab, sums, (float2 *)ws);
+	PZ_LAUNCH_CHECK();
+	norm_apply_bwd_kernel<T, 4><<<(unsigned)((long)d->n * p.apply.chunks), 256, 0, st>>>(g, p.apply, (const float2 *)ws);
+	PZ_LAUNCH_CHECK();
+	return PZ_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -134,7 +671,8 @@ extern "C" {
 int pz_groupnorm_workspace_bytes(const pz_groupnorm_desc *d, int backward, size_t *nbytes) {
 	if (int rc = check(d, "pz_groupnorm_workspace_bytes")) return rc;
 	PZ_REQUIRE(nbytes, "pz_groupnorm_workspace_bytes: null output");
-	*nbytes = backward ? (size_t)d->n * 2 * d->c * sizeof(float) : 0;
+	const Plan p = plan_norm(d, backward != 0);
+	*nbytes = backward ? sum_rows(d, p) * 2 * d->c * sizeof(float) + p.stat_bytes : p.part_bytes + p.stat_bytes;
 	return PZ_OK;
 }
 
@@ -142,14 +680,14 @@ int pz_groupnorm_fwd(const pz_groupnorm_desc *d, const void *x, const float *sca
                      void *workspace, size_t ws_bytes, pz_stream_t stream) {
 	if (int rc = check(d, "pz_groupnorm_fwd")) return rc;
 	if (d->n == 0 || d->pixels == 0) return PZ_OK;
+	size_t need = 0;
+	if (int rc = pz_groupnorm_workspace_bytes(d, 0, &need)) return rc;
 	PZ_REQUIRE(x && y, "pz_groupnorm_fwd: null tensor");
+	PZ_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "pz_groupnorm_fwd: workspace needs %zu bytes", need);
 	Norm g = args_of(d);
 	g.x = x, g.out = y, g.scale = scale, g.bias = bias, g.mean = savemean, g.invvar = saveinvvar;
 	hipStream_t st = pz::as_stream(stream);
-	if (d->dtype == PZ_F16) norm_fwd_kernel<f16><<<d->n * d->groups, 256, 0, st>>>(g);
-	else norm_fwd_kernel<float><<<d->n * d->groups, 256, 0, st>>>(g);
-	PZ_LAUNCH_CHECK();
-	return PZ_OK;
+	return d->dtype == PZ_F16 ? forward<f16>(d, g, (char *)workspace, st) : forward<float>(d, g, (char *)workspace, st);
 }
 
 int pz_groupnorm_bwd(const pz_groupnorm_desc *d, const void *dy, const void *x, const float *scale, const float *bias, const float *savemean,
@@ -163,20 +701,15 @@ int pz_groupnorm_bwd(const pz_groupnorm_desc *d, const void *dy, const void *x, 
 	PZ_REQUIRE(empty || (workspace && ws_bytes >= need), "pz_groupnorm_bwd: workspace needs %zu bytes", need);
 	Norm g = args_of(d);
 	g.x = x, g.dy = dy, g.out = dx, g.scale = scale, g.bias = bias, g.mean = (float *)savemean, g.invvar = (float *)saveinvvar;
-	float *part = (float *)workspace;
+	const Plan p = plan_norm(d, true);
+	float *sums = (float *)workspace;
+	const size_t rows = empty ? 0 : sum_rows(d, p);
 	if (!empty) {
-		if (dscale || dbias) {
-			const dim3 grid((unsigned)pz::ceil_div(d->c, 256), (unsigned)d->n);
-			if (d->dtype == PZ_F16) norm_channel_kernel<f16><<<grid, 256, 0, st>>>(g, part);
-			else norm_channel_kernel<float><<<grid, 256, 0, st>>>(g, part);
-			PZ_LAUNCH_CHECK();
-		}
-		if (d->dtype == PZ_F16) norm_bwd_kernel<f16><<<d->n * d->groups, 256, 0, st>>>(g);
-		else norm_bwd_kernel<float><<<d->n * d->groups, 256, 0, st>>>(g);
-		PZ_LAUNCH_CHECK();
+		char *ws = (char *)workspace + rows * 2 * d->c * sizeof(float);
+		if (int rc = d->dtype == PZ_F16 ? backward<f16>(d, g, sums, ws, st) : backward<float>(d, g, sums, ws, st)) return rc;
 	}
 	if (dscale || dbias) {
-		norm_param_kernel<<<pz::ceil_div(d->c, 256), 256, 0, st>>>(part, empty ? 0 : d->n, d->c, dscale, dbias);
+		norm_param_kernel<<<pz::ceil_div(d->c, 64), 1024, 0, st>>>(sums, (long)rows, d->c, dscale, dbias);
 		PZ_LAUNCH_CHECK();
 	}
 	return PZ_OK;

@@ -27,7 +27,7 @@ struct Epilogue {
 	long ldo, ldp, ldr;              // row pitches in elements
 	int m, n;
 	int kind, act, dropping, out_f32;
-	float alpha, beta;
+	float alpha, beta, inv_keep;
 	int vec;                         // every pitch and base of the tensors above takes runs of COUNT (16 bytes of T, 32 of float32)
 	DropKey drop;
 };
@@ -71,7 +71,7 @@ __device__ __forceinline__ void finish_run(const Epilogue &e, int row, int col, 
 	if (e.dropping) {
 		const unsigned bits = drop_bits<COUNT>(e.drop, (uint64_t)row * e.n + col);
 #pragma unroll
-		for (int i = 0; i < COUNT; ++i) s[i] = bits >> i & 1u ? s[i] / e.drop.keep : 0.f;
+		for (int i = 0; i < COUNT; ++i) s[i] = bits >> i & 1u ? s[i] * e.inv_keep : 0.f;
 	}
 	if (e.residual) {
 		float r[COUNT];
@@ -417,6 +417,7 @@ struct Gate {
 	float *sums;                     // [row blocks][n], optional
 	long lddy, ldp, lddz;
 	int m, n, act, dropping, vec, rows_per_block;
+	float inv_keep;
 	DropKey drop;
 };
 
@@ -440,7 +441,7 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 			if (g.dropping) {
 				const unsigned bits = drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col);
 #pragma unroll
-				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] / g.drop.keep : 0.f;
+				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] * g.inv_keep : 0.f;
 			}
 			if (g.act != PZ_ACT_NONE) {
 				float z[COUNT];
@@ -463,14 +464,19 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 	}
 }
 
-// db = beta * db + alpha * (sums of the row blocks, in order)
-__global__ void __launch_bounds__(256) linear_bias_grad_kernel(const float *__restrict__ sums, int blocks, int n, float *__restrict__ db,
-                                                                float alpha, float beta) {
-	const int c = blockIdx.x * 256 + threadIdx.x;
-	if (c >= n) return;
-	float s = 0.f;
-	for (int i = 0; i < blocks; ++i) s += sums[(size_t)i * n + c];
-	db[c] = (beta == 0.f ? 0.f : beta * db[c]) + alpha * s;
+// db = beta * db + alpha * (sums of the row blocks, in a fixed order, float64). 64 columns a workgroup, 16 row blocks at a time.
+__global__ void __launch_bounds__(1024) linear_bias_grad_kernel(const float *__restrict__ sums, int blocks, int n, float *__restrict__ db,
+                                                                 float alpha, float beta) {
+	__shared__ double part[16][64];
+	const int lane = threadIdx.x & 63, row = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+	double s = 0.0;
+	if (c < n)
+		for (int i = row; i < blocks; i += 16) s += sums[(size_t)i * n + c];
+	part[row][lane] = s;
+	__syncthreads();
+	if (row > 0 || c >= n) return;
+	for (int i = 1; i < 16; ++i) s += part[i][lane];
+	db[c] = (beta == 0.f ? 0.f : beta * db[c]) + alpha * (float)s;
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------------
@@ -696,7 +702,7 @@ int pz_linear_fwd(const pz_linear_desc *d, const void *x, const void *w, const f
 	e.ldo = d->ldy, e.ldp = d->ldp, e.ldr = d->ldr;
 	e.kind = EPI_FORWARD, e.act = d->act, e.dropping = mask != nullptr, e.alpha = 1.f;
 	e.vec = runs_ok(y, d->ldy, size) && runs_ok(preact, d->ldp, size) && runs_ok(residual, d->ldr, size) && runs_ok(bias, 4, 4);
-	e.drop = key_of(mask);
+	e.drop = key_of(mask), e.inv_keep = 1.f / e.drop.keep;
 	return product(d->dtype, o, e, (char *)workspace, pz::as_stream(stream));
 }
 
@@ -734,14 +740,14 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 		g.lddy = d->ldy, g.ldp = d->ldp, g.lddz = lddz;
 		g.m = d->m, g.n = d->n, g.act = d->act, g.dropping = mask != nullptr, g.rows_per_block = p.rows_per_block;
 		g.vec = runs_ok(dy, d->ldy, size) && (d->act == PZ_ACT_NONE || runs_ok(preact, d->ldp, size));
-		g.drop = key_of(mask);
+		g.drop = key_of(mask), g.inv_keep = 1.f / g.drop.keep;
 		const dim3 grid((unsigned)pz::ceil_div(d->n, 512), (unsigned)p.row_blocks);
 		if (d->dtype == PZ_F16) linear_gate_kernel<f16><<<grid, 256, 0, st>>>(g);
 		else linear_gate_kernel<float><<<grid, 256, 0, st>>>(g);
 		PZ_LAUNCH_CHECK();
 	}
 	if (db) {
-		linear_bias_grad_kernel<<<pz::ceil_div(d->n, 256), 256, 0, st>>>(sums, p.row_blocks, d->n, db, alpha, beta);
+		linear_bias_grad_kernel<<<pz::ceil_div(d->n, 64), 1024, 0, st>>>(sums, p.row_blocks, d->n, db, alpha, beta);
 		PZ_LAUNCH_CHECK();
 	}
 	ws += p.dz_bytes + p.sum_bytes;

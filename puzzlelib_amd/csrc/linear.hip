@@ -226,7 +226,10 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 }
 
 // ---- float16: v_mfma_f32_32x32x16_f16, operands straight into LDS --------------------------------------------------------------------
-constexpr int HK = 64;               // reduction steps per LDS tile
+// LDS holds a ring of four tiles of HK = 32 reduction steps. While tile t is multiplied, t + 1 is there already, t + 2 is on its way and
+// t + 3 is asked for: a fragment is fetched one multiplication ahead, across the tiles' border too, so that neither LDS nor global
+// latency stands between matrix instructions, and the one barrier a tile needs meets waves that have work in hand.
+constexpr int HK = 32, kRing = 4;
 
 __device__ __forceinline__ unsigned lds_address(const void *p) {
 	return (unsigned)(size_t)(__attribute__((address_space(3))) const void *)p;
@@ -238,36 +241,38 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned lds, u
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rs) : "memory");
 }
 
-__device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ void meet() { asm volatile("s_barrier" ::: "memory"); }
+// all but the last LEFT of this wave's dma16 have landed, its LDS reads are done, and so for every wave behind the barrier
+template <int LEFT>
+__device__ __forceinline__ void meet() {
+	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
+}
 
-// One operand of the tile: ROWS x HK, staged by WAVES waves.
-// KMAJOR = false: [row][k] in memory, so 128 bytes of k per row in LDS; the 16-byte pieces of row r stand at piece ^ (r & 7) — a
-//   fragment read (32 rows, one piece each) then touches all 64 banks evenly.
-// KMAJOR = true: [k][row] in memory, so ROWS * 2 bytes per k in LDS; the 32-byte pieces of step k stand at piece ^ turn(k), and
-//   fragments are read with ds_read_b64_tr_b16, which hands 16 lanes the 4 x 16 block of 4 steps x 16 rows transposed; turn() puts
-//   the 16 steps that one such instruction reads onto 8 different piece positions (256 bytes: all banks).
+// One operand of the tile: ROWS x HK, staged by WAVES waves. LDS has 64 banks of 4 bytes; a read is spread so that 16 neighbouring lanes of
+// a ds_read_b128, or 32 of a ds_read_b64, touch each bank once.
+// KMAJOR = false: [row][k] in memory, so 64 bytes of k per row in LDS, four rows to all banks; the 16-byte pieces of row r stand at
+//   piece ^ (r / 4 mod 4), so the fragment's 16 rows at one piece land on 16 different places.
+// KMAJOR = true: [k][row] in memory, so ROWS * 2 bytes per k in LDS; fragments are read with ds_read_b64_tr_b16, which hands 16 lanes
+//   the 4 x 16 block of 4 steps x 16 rows transposed. 32 lanes take 64 bytes (two 32-byte pieces) of each of 4 steps: the pieces of
+//   step k stand at piece ^ turn(k), which gives the 4 steps 4 different pairs of pieces.
 template <int ROWS, bool KMAJOR, int WAVES>
 struct Stage {
 	static constexpr int HALVES = ROWS * HK;
-	static constexpr int PIECES = ROWS / 8 / WAVES;            // dma16 per wave and tile
-	static_assert(PIECES >= 1 && PIECES * WAVES * 8 == ROWS, "tile / waves");
-	static constexpr int TURNS = ROWS / 16 < 8 ? ROWS / 16 : 8;
+	static constexpr int PIECES = ROWS / 16 / WAVES;           // dma16 per wave and tile
+	static_assert(PIECES >= 1 && PIECES * WAVES * 16 == ROWS, "tile / waves");
 
-	__device__ __forceinline__ static int turn(int k) { return ((k & 3) | (k >> 3 & 1) << 2) & (TURNS - 1); }
+	__device__ __forceinline__ static int turn(int k) { return ROWS == 64 ? k & 2 : (k & 3) << 1; }      // (64 rows: two steps to all banks)
+	__device__ __forceinline__ static int spot(int r) { return r >> 2 & 3; }
 
-	size_t base, bytes;              // start of the tile in the operand at the next k step, and what is left of the operand from there
-	size_t step;                     // advance per k step
-	const char *p;
-	unsigned off[PIECES];            // a lane's byte offsets from the start
-	int kpiece;                      // KMAJOR = false: first k of the lane's piece
+	long bytes, step;                // what is left of the operand from the next tile on (negative: nothing); advance per tile
+	const char *p;                   // the next tile
+	unsigned off[PIECES];            // a lane's byte offsets from there
+	int kpiece[PIECES];              // KMAJOR = false: first k of the lane's pieces
 
 	__device__ __forceinline__ void init(const void *src, size_t extent, long ld, int row0, int kbeg, int wave, int lane) {
 		const size_t start = KMAJOR ? ((size_t)kbeg * ld + row0) * 2 : ((size_t)row0 * ld + kbeg) * 2;
 		p = (const char *)src + start;
-		bytes = extent > start ? extent - start : 0;
-		step = KMAJOR ? (size_t)HK * ld * 2 : (size_t)HK * 2;
-		kpiece = 0;
+		bytes = (long)(extent - start);
+		step = KMAJOR ? HK * ld * 2 : HK * 2;
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
 			const int o = ((wave * PIECES + i) * 64 + lane) * 16;                // place in the LDS tile
@@ -275,29 +280,30 @@ struct Stage {
 				const int k = o / (ROWS * 2), at = o % (ROWS * 2) / 16;
 				off[i] = (unsigned)((size_t)k * ld * 2) + (((at >> 1) ^ turn(k)) * 2 + (at & 1)) * 16;
 			} else {
-				const int r = o / 128, piece = (o / 16 & 7) ^ (r & 7);
-				kpiece = piece * 8;                                               // (r & 7 is lane >> 3 for every i)
+				const int r = o / (HK * 2), piece = (o / 16 % (HK / 8)) ^ spot(r);
+				kpiece[i] = piece * 8;
 				off[i] = (unsigned)((size_t)r * ld * 2) + piece * 16;
 			}
 		}
 	}
 
-	// k steps [k, k + HK) into the tile at LDS address `lds`; moves on
+	// k steps [k, k + HK) into the tile at LDS address `lds`; moves on. Steps from kend on are zeros (or another split's, never multiplied).
 	__device__ __forceinline__ void issue(unsigned lds, int k, int kend, int wave) {
-		const unsigned span = bytes > 0xfffff000ull ? 0xfffff000u : (unsigned)bytes;
-		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, __builtin_amdgcn_readfirstlane(span), 0x00020000);
-		const bool in = KMAJOR || k + kpiece < kend;
+		const int high = (int)(bytes >> 32);                                 // (32-bit tests: they stay in the scalar unit)
+		const unsigned span = high > 0 ? 0xfffff000u : high < 0 ? 0u : min((unsigned)bytes, 0xfffff000u);
+		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, span, 0x00020000);
 #pragma unroll
-		for (int i = 0; i < PIECES; ++i) dma16(rs, lds + (wave * PIECES + i) * 1024, in ? off[i] : 0xfffffff0u);
+		for (int i = 0; i < PIECES; ++i)
+			dma16(rs, lds + (wave * PIECES + i) * 1024, KMAJOR || k + kpiece[i] < kend ? off[i] : 0xfffffff0u);
 		p += step;
-		bytes = bytes > step ? bytes - step : 0;
+		bytes -= step;
 	}
 
 	// fragment of v_mfma_f32_32x32x16_f16: rows row0 + (lane & 31), steps 16 s + 8 (lane >> 5) ... + 7
 	__device__ __forceinline__ static f16x8 fragment(const f16 *tile, int row0, int s, int lane) {
 		if (!KMAJOR) {
 			const int r = row0 + (lane & 31), piece = s * 2 + (lane >> 5);
-			return *reinterpret_cast<const f16x8 *>(tile + r * HK + ((piece ^ (r & 7)) * 8));
+			return *reinterpret_cast<const f16x8 *>(tile + r * HK + ((piece ^ spot(r)) * 8));
 		}
 		// 16 lanes: rows base ... base + 15; lane j of them points at step (j >> 2), rows 4 (j & 3) ... + 3 of the block
 		const int j = lane & 15, base = row0 + (lane >> 4 & 1) * 16, k = s * 16 + (lane >> 5) * 8 + (j >> 2);
@@ -319,7 +325,8 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	using SB = Stage<BN, !TB, WAVES>;
 	using Out = Drain<f16, TM, TN>;
 	constexpr int TILE = SA::HALVES + SB::HALVES, SLABS = 2 * WAVES * Out::FLOATS;
-	__shared__ __attribute__((aligned(1024))) f16 lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
+	constexpr int FLIGHT = SA::PIECES + SB::PIECES;              // dma16 per wave and tile
+	__shared__ __attribute__((aligned(1024))) f16 lds[kRing * TILE > SLABS ? kRing * TILE : SLABS];
 
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -344,35 +351,53 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	sa.init(g.a, g.a_bytes, g.lda, m0, kbeg, wave, lane);
 	sb.init(g.b, g.b_bytes, g.ldb, n0, kbeg, wave, lane);
 	const unsigned at = lds_address(lds);
-	if (kbeg < kend) {
-		sa.issue(at, kbeg, kend, wave);
-		sb.issue(at + SA::HALVES * 2, kbeg, kend, wave);
-	}
+	auto ask = [&](int tile) {
+		const unsigned to = at + (tile % kRing) * (TILE * 2);
+		sa.issue(to, kbeg + tile * HK, kend, wave);
+		sb.issue(to + SA::HALVES * 2, kbeg + tile * HK, kend, wave);
+	};
+	f16x8 av[2][TM], bv[2][TN];
+	auto fetch = [&](int tile, int s, f16x8 (&a)[TM], f16x8 (&b)[TN]) {
+		const f16 *as = lds + (tile % kRing) * TILE, *bs = as + SA::HALVES;
+#pragma unroll
+		for (int j = 0; j < TN; ++j) b[j] = SB::fragment(bs, wn * (BN / WN) + j * 32, s, lane);
+#pragma unroll
+		for (int i = 0; i < TM; ++i) a[i] = SA::fragment(as, wm * (BM / WM) + i * 32, s, lane);
+	};
+	auto multiply = [&](const f16x8 (&a)[TM], const f16x8 (&b)[TN]) {
+#pragma unroll
+		for (int i = 0; i < TM; ++i)
+#pragma unroll
+			for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[j], a[i], acc[i][j], 0, 0, 0);
+	};
 
-	int buf = 0;
-	for (int k0 = kbeg; k0 < kend; k0 += HK, buf ^= 1) {
-		dma_landed();                // this wave's share of tile k0 is in LDS; behind the barrier everybody's is,
-		meet();                      // and everybody is done reading the other half
-		if (k0 + HK < kend) {
-			const unsigned next = at + (buf ^ 1) * (TILE * 2);
-			sa.issue(next, k0 + HK, kend, wave);
-			sb.issue(next + SA::HALVES * 2, k0 + HK, kend, wave);
+	// the scheduler would sink each fetch to its use: two reads behind each of the first matrix instructions, so that they are back
+	// before the last one is through
+	auto interleave = [&]() {
+#pragma unroll
+		for (int i = 0; i < TM * TN; ++i) {
+			__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+			__builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
 		}
-		const f16 *as = lds + buf * TILE, *bs = as + SA::HALVES;
-#pragma unroll
-		for (int s = 0; s < HK / 16; ++s) {
-			f16x8 av[TM], bv[TN];
-#pragma unroll
-			for (int i = 0; i < TM; ++i) av[i] = SA::fragment(as, wm * (BM / WM) + i * 32, s, lane);
-#pragma unroll
-			for (int j = 0; j < TN; ++j) bv[j] = SB::fragment(bs, wn * (BN / WN) + j * 32, s, lane);
-#pragma unroll
-			for (int i = 0; i < TM; ++i)
-#pragma unroll
-				for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bv[j], av[i], acc[i][j], 0, 0, 0);
-		}
+		__builtin_amdgcn_sched_barrier(0);
+	};
+
+	const int tiles = (kend - kbeg + HK - 1) / HK;
+	for (int t = 0; t < kRing - 1; ++t) ask(t);
+	meet<2 * FLIGHT>();
+	fetch(0, 0, av[0], bv[0]);
+	for (int t = 0; t < tiles; ++t) {
+		meet<FLIGHT>();              // tile t + 1 is there for everybody, and everybody is done with tile t - 1, whose place t + 3 takes
+		ask(t + kRing - 1);
+		__builtin_amdgcn_sched_barrier(0);
+		fetch(t, 1, av[1], bv[1]);
+		multiply(av[0], bv[0]);
+		interleave();
+		fetch(t + 1, 0, av[0], bv[0]);
+		multiply(av[1], bv[1]);
+		interleave();
 	}
-	__syncthreads();                 // the slabs below lie over the tiles
+	meet<0>();                       // the slabs below lie over the tiles
 	Out::run(g, acc, reinterpret_cast<float *>(lds) + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);
 }
 

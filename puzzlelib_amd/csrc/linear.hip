@@ -226,10 +226,11 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 }
 
 // ---- float16: v_mfma_f32_32x32x16_f16, operands straight into LDS --------------------------------------------------------------------
-// LDS holds a ring of four tiles of HK = 32 reduction steps. While tile t is multiplied, t + 1 is there already, t + 2 is on its way and
-// t + 3 is asked for: a fragment is fetched one multiplication ahead, across the tiles' border too, so that neither LDS nor global
-// latency stands between matrix instructions, and the one barrier a tile needs meets waves that have work in hand.
-constexpr int HK = 32, kRing = 4;
+// LDS holds two tiles of HK = 64 reduction steps: 128 bytes of a row whose contiguous axis is k, one L2 request each (a ring of four
+// tiles of 32 steps asked twice as often and ran 8 % slower: 247 instead of 229 us for 8192 x 8192 x 2048). Fragments are fetched one
+// block of matrix instructions ahead, across the tiles' border too: the one barrier a tile needs stands in front of its LAST block, when
+// its fragments are all in registers. Behind it the next tile is there for everybody and this one's place is free for the next but one.
+constexpr int HK = 64;
 
 __device__ __forceinline__ unsigned lds_address(const void *p) {
 	return (unsigned)(size_t)(__attribute__((address_space(3))) const void *)p;
@@ -241,7 +242,7 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, unsigned lds, u
 	asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rs) : "memory");
 }
 
-// all but the last LEFT of this wave's dma16 have landed, its LDS reads are done, and so for every wave behind the barrier
+// all but the last LEFT of this wave's dma16 have landed (they do in order), its LDS reads are back, and so for every wave behind the barrier
 template <int LEFT>
 __device__ __forceinline__ void meet() {
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
@@ -249,19 +250,19 @@ __device__ __forceinline__ void meet() {
 
 // One operand of the tile: ROWS x HK, staged by WAVES waves. LDS has 64 banks of 4 bytes; a read is spread so that 16 neighbouring lanes of
 // a ds_read_b128, or 32 of a ds_read_b64, touch each bank once.
-// KMAJOR = false: [row][k] in memory, so 64 bytes of k per row in LDS, four rows to all banks; the 16-byte pieces of row r stand at
-//   piece ^ (r / 4 mod 4), so the fragment's 16 rows at one piece land on 16 different places.
+// KMAJOR = false: [row][k] in memory, so 128 bytes of k per row in LDS, two rows to all banks; the 16-byte pieces of row r stand at
+//   piece ^ (r / 2 mod 8), so the fragment's 16 rows at one piece land on 16 different places.
 // KMAJOR = true: [k][row] in memory, so ROWS * 2 bytes per k in LDS; fragments are read with ds_read_b64_tr_b16, which hands 16 lanes
 //   the 4 x 16 block of 4 steps x 16 rows transposed. 32 lanes take 64 bytes (two 32-byte pieces) of each of 4 steps: the pieces of
 //   step k stand at piece ^ turn(k), which gives the 4 steps 4 different pairs of pieces.
 template <int ROWS, bool KMAJOR, int WAVES>
 struct Stage {
 	static constexpr int HALVES = ROWS * HK;
-	static constexpr int PIECES = ROWS / 16 / WAVES;           // dma16 per wave and tile
-	static_assert(PIECES >= 1 && PIECES * WAVES * 16 == ROWS, "tile / waves");
+	static constexpr int PIECES = ROWS / 8 / WAVES;            // dma16 per wave and tile
+	static_assert(PIECES >= 1 && PIECES * WAVES * 8 == ROWS, "tile / waves");
 
 	__device__ __forceinline__ static int turn(int k) { return ROWS == 64 ? k & 2 : (k & 3) << 1; }      // (64 rows: two steps to all banks)
-	__device__ __forceinline__ static int spot(int r) { return r >> 2 & 3; }
+	__device__ __forceinline__ static int spot(int r) { return r >> 1 & 7; }
 
 	long bytes, step;                // what is left of the operand from the next tile on (negative: nothing); advance per tile
 	const char *p;                   // the next tile
@@ -287,17 +288,15 @@ struct Stage {
 		}
 	}
 
-	// k steps [k, k + HK) into the tile at LDS address `lds`; moves on. Steps from kend on are zeros (or another split's, never multiplied).
-	__device__ __forceinline__ void issue(unsigned lds, int k, int kend, int wave) {
+	// piece i of k steps [k, k + HK) into the tile at LDS address `lds`. Steps from kend on are zeros (or another split's, never multiplied).
+	__device__ __forceinline__ void issue(int i, unsigned lds, int k, int kend, int wave) {
 		const int high = (int)(bytes >> 32);                                 // (32-bit tests: they stay in the scalar unit)
 		const unsigned span = high > 0 ? 0xfffff000u : high < 0 ? 0u : min((unsigned)bytes, 0xfffff000u);
 		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, span, 0x00020000);
-#pragma unroll
-		for (int i = 0; i < PIECES; ++i)
-			dma16(rs, lds + (wave * PIECES + i) * 1024, KMAJOR || k + kpiece[i] < kend ? off[i] : 0xfffffff0u);
-		p += step;
-		bytes -= step;
+		dma16(rs, lds + (wave * PIECES + i) * 1024, KMAJOR || k + kpiece[i] < kend ? off[i] : 0xfffffff0u);
 	}
+
+	__device__ __forceinline__ void advance() { p += step, bytes -= step; }
 
 	// fragment of v_mfma_f32_32x32x16_f16: rows row0 + (lane & 31), steps 16 s + 8 (lane >> 5) ... + 7
 	__device__ __forceinline__ static f16x8 fragment(const f16 *tile, int row0, int s, int lane) {
@@ -326,7 +325,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	using Out = Drain<f16, TM, TN>;
 	constexpr int TILE = SA::HALVES + SB::HALVES, SLABS = 2 * WAVES * Out::FLOATS;
 	constexpr int FLIGHT = SA::PIECES + SB::PIECES;              // dma16 per wave and tile
-	__shared__ __attribute__((aligned(1024))) f16 lds[kRing * TILE > SLABS ? kRing * TILE : SLABS];
+	__shared__ __attribute__((aligned(1024))) f16 lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
 
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -351,51 +350,55 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	sa.init(g.a, g.a_bytes, g.lda, m0, kbeg, wave, lane);
 	sb.init(g.b, g.b_bytes, g.ldb, n0, kbeg, wave, lane);
 	const unsigned at = lds_address(lds);
-	auto ask = [&](int tile) {
-		const unsigned to = at + (tile % kRing) * (TILE * 2);
-		sa.issue(to, kbeg + tile * HK, kend, wave);
-		sb.issue(to + SA::HALVES * 2, kbeg + tile * HK, kend, wave);
+	// piece i of what a tile takes: the first operand's, then the second's
+	auto ask = [&](int tile, int i) {
+		const unsigned to = at + (tile & 1) * (TILE * 2);
+		if (i < SA::PIECES) {
+			sa.issue(i, to, kbeg + tile * HK, kend, wave);
+			if (i == SA::PIECES - 1) sa.advance();
+		} else {
+			sb.issue(i - SA::PIECES, to + SA::HALVES * 2, kbeg + tile * HK, kend, wave);
+			if (i == FLIGHT - 1) sb.advance();
+		}
 	};
 	f16x8 av[2][TM], bv[2][TN];
-	auto fetch = [&](int tile, int s, f16x8 (&a)[TM], f16x8 (&b)[TN]) {
-		const f16 *as = lds + (tile % kRing) * TILE, *bs = as + SA::HALVES;
-#pragma unroll
-		for (int j = 0; j < TN; ++j) b[j] = SB::fragment(bs, wn * (BN / WN) + j * 32, s, lane);
-#pragma unroll
-		for (int i = 0; i < TM; ++i) a[i] = SA::fragment(as, wm * (BM / WM) + i * 32, s, lane);
+	auto fetch = [&](int tile, int s, int i, int half) {          // fragment i of step s
+		const f16 *as = lds + (tile & 1) * TILE, *bs = as + SA::HALVES;
+		if (i < TN) bv[half][i] = SB::fragment(bs, wn * (BN / WN) + i * 32, s, lane);
+		else av[half][i - TN] = SA::fragment(as, wm * (BM / WM) + (i - TN) * 32, s, lane);
 	};
-	auto multiply = [&](const f16x8 (&a)[TM], const f16x8 (&b)[TN]) {
+	// the TM x TN matrix instructions on fragments `half`, each followed by a share of what else the wave has to issue: the next
+	// fragments, the next tile's requests. Left alone, the scheduler collects them between the blocks, where the matrix pipe stands.
+	constexpr int OPS = TM * TN, FRAGMENTS = TM + TN;
+	auto block = [&](int half, int tile, int s, int asked) {
 #pragma unroll
-		for (int i = 0; i < TM; ++i)
+		for (int x = 0; x < OPS; ++x) {
+			const int i = x / TN, j = x % TN;
+			acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bv[half][j], av[half][i], acc[i][j], 0, 0, 0);
 #pragma unroll
-			for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(b[j], a[i], acc[i][j], 0, 0, 0);
-	};
-
-	// the scheduler would sink each fetch to its use: two reads behind each of the first matrix instructions, so that they are back
-	// before the last one is through
-	auto interleave = [&]() {
+			for (int f = x * FRAGMENTS / OPS; f < (x + 1) * FRAGMENTS / OPS; ++f) fetch(tile, s, f, half ^ 1);
+			if (asked >= 0) {
 #pragma unroll
-		for (int i = 0; i < TM * TN; ++i) {
-			__builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-			__builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+				for (int f = x * FLIGHT / OPS; f < (x + 1) * FLIGHT / OPS; ++f) ask(asked, f);
+			}
+			__builtin_amdgcn_sched_barrier(0);
 		}
-		__builtin_amdgcn_sched_barrier(0);
 	};
 
 	const int tiles = (kend - kbeg + HK - 1) / HK;
-	for (int t = 0; t < kRing - 1; ++t) ask(t);
-	meet<2 * FLIGHT>();
-	fetch(0, 0, av[0], bv[0]);
+#pragma unroll
+	for (int t = 0; t < 2; ++t)
+#pragma unroll
+		for (int i = 0; i < FLIGHT; ++i) ask(t, i);
+	meet<FLIGHT>();
+#pragma unroll
+	for (int i = 0; i < FRAGMENTS; ++i) fetch(0, 0, i, 0);
 	for (int t = 0; t < tiles; ++t) {
-		meet<FLIGHT>();              // tile t + 1 is there for everybody, and everybody is done with tile t - 1, whose place t + 3 takes
-		ask(t + kRing - 1);
-		__builtin_amdgcn_sched_barrier(0);
-		fetch(t, 1, av[1], bv[1]);
-		multiply(av[0], bv[0]);
-		interleave();
-		fetch(t + 1, 0, av[0], bv[0]);
-		multiply(av[1], bv[1]);
-		interleave();
+		block(0, t, 1, -1);
+		block(1, t, 2, -1);
+		block(0, t, 3, -1);
+		meet<0>();
+		block(1, t + 1, 0, t + 2);
 	}
 	meet<0>();                       // the slabs below lie over the tiles
 	Out::run(g, acc, reinterpret_cast<float *>(lds) + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);

@@ -106,25 +106,40 @@ __device__ __forceinline__ void tile_of(const Product &g, int &tm, int &tn) {
 	tn = rest / rows;
 }
 
-// A wave's accumulators -> rows. The matrix instruction took the operand of the n side first, so a lane holds, of row m = lane & 31,
-// the columns 8 q + 4 (lane >> 5) ... + 3 in registers 4 q ... 4 q + 3. They go through LDS in slabs of 32 rows x 32 TN columns (the wave's own,
-// no barrier), so that consecutive lanes store consecutive runs of a row: whole 128-byte lines instead of 32 pieces of 16 bytes.
-template <typename T, int TM, int TN>
+// A wave's accumulators -> rows. The matrix instruction took the operand of the n side first, so a lane holds 4 consecutive columns of one
+// row at a time: 32 x 32 tiles, row lane & 31, columns 8 q + 4 (lane >> 5) in registers 4 q ...; 16 x 16 tiles, row lane & 15, columns
+// 4 (lane >> 4). They go through LDS in slabs of 32 rows (the wave's own, no barrier), so that consecutive lanes store consecutive runs
+// of a row: whole 128-byte lines instead of pieces of 16 bytes.
+template <typename T, int ROWS, int COLS>
 struct Drain {
 	static constexpr int COUNT = 16 / sizeof(T);                 // values a lane stores at once
-	static constexpr int COLS = 32 * TN, PITCH = COLS + 4;       // (+4: the rows of a store start 4 banks apart)
+	static constexpr int PITCH = COLS + 4;                       // (+4: the rows of a store start 4 banks apart)
 	static constexpr int FLOATS = 32 * PITCH;
 
-	static __device__ __forceinline__ void run(const Product &g, const f32x16 (&acc)[TM][TN], float *lds, int row0, int col0, int split, int lane) {
-		const int l31 = lane & 31, lhi = lane >> 5;
+	template <int TM, int TN>
+	static __device__ __forceinline__ void park(const f32x16 (&acc)[TM][TN], int i, float *lds, int lane) {
 #pragma unroll
-		for (int i = 0; i < TM; ++i) {
+		for (int j = 0; j < TN; ++j)
+#pragma unroll
+			for (int q = 0; q < 4; ++q)
+				*reinterpret_cast<f32x4 *>(lds + (lane & 31) * PITCH + j * 32 + q * 8 + (lane >> 5) * 4) =
+				    (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+	}
+
+	template <int TM, int TN>
+	static __device__ __forceinline__ void park(const f32x4 (&acc)[TM][TN], int i, float *lds, int lane) {
+#pragma unroll
+		for (int h = 0; h < 2; ++h)
 #pragma unroll
 			for (int j = 0; j < TN; ++j)
+				*reinterpret_cast<f32x4 *>(lds + (h * 16 + (lane & 15)) * PITCH + j * 16 + (lane >> 4) * 4) = acc[2 * i + h][j];
+	}
+
+	template <typename ACC>
+	static __device__ __forceinline__ void run(const Product &g, const ACC &acc, float *lds, int row0, int col0, int split, int lane) {
 #pragma unroll
-				for (int q = 0; q < 4; ++q)
-					*reinterpret_cast<f32x4 *>(lds + l31 * PITCH + j * 32 + q * 8 + lhi * 4) =
-					    (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+		for (int i = 0; i < ROWS / 32; ++i) {
+			park(acc, i, lds, lane);
 			__builtin_amdgcn_wave_barrier();
 			constexpr int RUNS = COLS / COUNT, STEP = 64 / RUNS;         // runs in a row, rows a wave handles at once
 			static_assert(64 % RUNS == 0, "runs of a row over lanes");
@@ -157,7 +172,7 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 	constexpr int NT = 64 * WM * WN, TM = BM / (32 * WM), TN = BN / (32 * WN);
 	using LA = Loader<NT, BM, TA, VEC>;
 	using LB = Loader<NT, BN, !TB, VEC>;
-	using Out = Drain<float, TM, TN>;
+	using Out = Drain<float, BM / WM, BN / WN>;
 	constexpr int TILES = 2 * BK * (LA::LD + LB::LD), SLABS = WM * WN * Out::FLOATS;
 	__shared__ __attribute__((aligned(16))) float lds[TILES > SLABS ? TILES : SLABS];
 	float *const As = lds, *const Bs = lds + 2 * BK * LA::LD;
@@ -225,11 +240,12 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 	Out::run(g, acc, lds + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);
 }
 
-// ---- float16: v_mfma_f32_32x32x16_f16, operands straight into LDS --------------------------------------------------------------------
-// LDS holds two tiles of HK = 64 reduction steps: 128 bytes of a row whose contiguous axis is k, one L2 request each (a ring of four
-// tiles of 32 steps asked twice as often and ran 8 % slower: 247 instead of 229 us for 8192 x 8192 x 2048). Fragments are fetched one
-// block of matrix instructions ahead, across the tiles' border too: the one barrier a tile needs stands in front of its LAST block, when
-// its fragments are all in registers. Behind it the next tile is there for everybody and this one's place is free for the next but one.
+// ---- float16: v_mfma_f32_16x16x32_f16, operands straight into LDS --------------------------------------------------------------------
+// LDS holds two tiles of HK = 64 reduction steps: 128 bytes of a row whose contiguous axis is k, one L2 request each. A wave keeps the n
+// side's fragments of a whole tile in registers and walks over its rows, so that a tile's place in LDS frees in pieces: the n side and
+// the first half of the m side's rows ("half 0") in the tile's middle, the other rows at its end. What the tile after the next one puts
+// there is asked for at once and not needed for one and a half tiles — about 1.5 us, the time a line takes that no L2 holds. (Asked for
+// a tile at a time, behind its last block, the same kernel waited 40 % of its time: 465000 instead of 380000 cycles for 8192 x 8192 x 2048.)
 constexpr int HK = 64;
 
 __device__ __forceinline__ unsigned lds_address(const void *p) {
@@ -248,24 +264,28 @@ __device__ __forceinline__ void meet() {
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-// One operand of the tile: ROWS x HK, staged by WAVES waves. LDS has 64 banks of 4 bytes; a read is spread so that 16 neighbouring lanes of
+// ROWS rows of one operand x HK, staged by WAVES waves: rows row0 + (q / RUN) 2 RUN + half RUN + q mod RUN, q < ROWS — half of the rows of
+// every wave, or all rows (RUN = ROWS, half 0). LDS has 64 banks of 4 bytes; a read is spread so that 16 neighbouring lanes of
 // a ds_read_b128, or 32 of a ds_read_b64, touch each bank once.
 // KMAJOR = false: [row][k] in memory, so 128 bytes of k per row in LDS, two rows to all banks; the 16-byte pieces of row r stand at
 //   piece ^ (r / 2 mod 8), so the fragment's 16 rows at one piece land on 16 different places.
 // KMAJOR = true: [k][row] in memory, so ROWS * 2 bytes per k in LDS; fragments are read with ds_read_b64_tr_b16, which hands 16 lanes
-//   the 4 x 16 block of 4 steps x 16 rows transposed. 32 lanes take 64 bytes (two 32-byte pieces) of each of 4 steps: the pieces of
-//   step k stand at piece ^ turn(k), which gives the 4 steps 4 different pairs of pieces.
-template <int ROWS, bool KMAJOR, int WAVES>
+//   the 4 x 16 block of 4 steps x 16 rows transposed. 32 lanes take one 32-byte piece of each of 8 steps (k mod 4 and k / 8 mod 2 tell
+//   them apart): the pieces of step k stand at piece ^ turn(k), which gives the 8 steps 8 different places.
+template <int ROWS, int RUN, bool KMAJOR, int WAVES>
 struct Stage {
 	static constexpr int HALVES = ROWS * HK;
 	static constexpr int PIECES = ROWS / 8 / WAVES;            // dma16 per wave and tile
 	static_assert(PIECES >= 1 && PIECES * WAVES * 8 == ROWS, "tile / waves");
 
-	__device__ __forceinline__ static int turn(int k) { return ROWS == 64 ? k & 2 : (k & 3) << 1; }      // (64 rows: two steps to all banks)
+	__device__ __forceinline__ static int turn(int k) {                   // (64 rows: two steps to all banks, 32: four)
+		return ROWS == 32 ? k >> 3 & 1 : ROWS == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2;
+	}
 	__device__ __forceinline__ static int spot(int r) { return r >> 1 & 7; }
 
 	long bytes, step;                // what is left of the operand from the next tile on (negative: nothing); advance per tile
 	const char *p;                   // the next tile
+	long shift;                      // from half 0 to half 1
 	unsigned off[PIECES];            // a lane's byte offsets from there
 	int kpiece[PIECES];              // KMAJOR = false: first k of the lane's pieces
 
@@ -274,43 +294,46 @@ struct Stage {
 		p = (const char *)src + start;
 		bytes = (long)(extent - start);
 		step = KMAJOR ? HK * ld * 2 : HK * 2;
+		shift = KMAJOR ? RUN * 2 : RUN * ld * 2;
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
 			const int o = ((wave * PIECES + i) * 64 + lane) * 16;                // place in the LDS tile
 			if (KMAJOR) {
-				const int k = o / (ROWS * 2), at = o % (ROWS * 2) / 16;
-				off[i] = (unsigned)((size_t)k * ld * 2) + (((at >> 1) ^ turn(k)) * 2 + (at & 1)) * 16;
+				const int k = o / (ROWS * 2), at = o % (ROWS * 2) / 16, q = (((at >> 1) ^ turn(k)) * 2 + (at & 1)) * 8;
+				off[i] = (unsigned)((size_t)k * ld * 2) + (q / RUN * (2 * RUN) + q % RUN) * 2;
 			} else {
-				const int r = o / (HK * 2), piece = (o / 16 % (HK / 8)) ^ spot(r);
+				const int q = o / (HK * 2), piece = (o / 16 % (HK / 8)) ^ spot(q);
 				kpiece[i] = piece * 8;
-				off[i] = (unsigned)((size_t)r * ld * 2) + piece * 16;
+				off[i] = (unsigned)((size_t)(q / RUN * (2 * RUN) + q % RUN) * ld * 2) + piece * 16;
 			}
 		}
 	}
 
-	// piece i of k steps [k, k + HK) into the tile at LDS address `lds`. Steps from kend on are zeros (or another split's, never multiplied).
-	__device__ __forceinline__ void issue(int i, unsigned lds, int k, int kend, int wave) {
-		const int high = (int)(bytes >> 32);                                 // (32-bit tests: they stay in the scalar unit)
-		const unsigned span = high > 0 ? 0xfffff000u : high < 0 ? 0u : min((unsigned)bytes, 0xfffff000u);
-		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)p, 0, span, 0x00020000);
+	// piece i of k steps [k, k + HK) to LDS address `lds`. Steps from kend on are zeros (or another split's, never multiplied).
+	__device__ __forceinline__ void issue(int i, unsigned lds, int k, int kend, int wave, int half) {
+		const long left = bytes - half * shift;
+		const int high = (int)(left >> 32);                                  // (32-bit tests: they stay in the scalar unit)
+		const unsigned span = high > 0 ? 0xfffff000u : high < 0 ? 0u : min((unsigned)left, 0xfffff000u);
+		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(p + half * shift), 0, span, 0x00020000);
 		dma16(rs, lds + (wave * PIECES + i) * 1024, KMAJOR || k + kpiece[i] < kend ? off[i] : 0xfffffff0u);
 	}
 
 	__device__ __forceinline__ void advance() { p += step, bytes -= step; }
 
-	// fragment of v_mfma_f32_32x32x16_f16: rows row0 + (lane & 31), steps 16 s + 8 (lane >> 5) ... + 7
+	// fragment of v_mfma_f32_16x16x32_f16: rows row0 + (lane & 15), steps 32 s + 8 (lane >> 4) ... + 7
 	__device__ __forceinline__ static f16x8 fragment(const f16 *tile, int row0, int s, int lane) {
+		const int j = lane & 15;
 		if (!KMAJOR) {
-			const int r = row0 + (lane & 31), piece = s * 2 + (lane >> 5);
+			const int r = row0 + j, piece = s * 4 + (lane >> 4);
 			return *reinterpret_cast<const f16x8 *>(tile + r * HK + ((piece ^ spot(r)) * 8));
 		}
-		// 16 lanes: rows base ... base + 15; lane j of them points at step (j >> 2), rows 4 (j & 3) ... + 3 of the block
-		const int j = lane & 15, base = row0 + (lane >> 4 & 1) * 16, k = s * 16 + (lane >> 5) * 8 + (j >> 2);
+		// lane j of the 16 that share 8 steps points at step (j >> 2), rows 4 (j & 3) ... + 3 of their 4 x 16 block
+		const int k = s * 32 + (lane >> 4) * 8 + (j >> 2);
 		union { f16x8 v; tr16x4 h[2]; } f;
 #pragma unroll
 		for (int half = 0; half < 2; ++half) {
 			const int kk = k + half * 4;
-			const f16 *at = tile + kk * ROWS + ((base / 16) ^ turn(kk)) * 16 + (j & 3) * 4;
+			const f16 *at = tile + kk * ROWS + ((row0 / 16) ^ turn(kk)) * 16 + (j & 3) * 4;
 			f.h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr16x4 *)at);
 		}
 		return f.v;
@@ -319,12 +342,12 @@ struct Stage {
 
 template <int BM, int BN, int WM, int WN, bool TA, bool TB>
 __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
-	constexpr int WAVES = WM * WN, TM = BM / (32 * WM), TN = BN / (32 * WN);
-	using SA = Stage<BM, TA, WAVES>;
-	using SB = Stage<BN, !TB, WAVES>;
-	using Out = Drain<f16, TM, TN>;
-	constexpr int TILE = SA::HALVES + SB::HALVES, SLABS = 2 * WAVES * Out::FLOATS;
-	constexpr int FLIGHT = SA::PIECES + SB::PIECES;              // dma16 per wave and tile
+	constexpr int WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN);
+	using SA = Stage<BM / 2, BM / WM / 2, TA, WAVES>;            // a half of the rows
+	using SB = Stage<BN, BN, !TB, WAVES>;
+	using Out = Drain<f16, BM / WM, BN / WN>;
+	constexpr int TILE = 2 * SA::HALVES + SB::HALVES, SLABS = 2 * WAVES * Out::FLOATS;
+	constexpr int NH = SA::PIECES, NB = SB::PIECES;              // dma16 per wave: a half of the m side, the n side
 	__shared__ __attribute__((aligned(1024))) f16 lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
 
 	const int lane = threadIdx.x & 63;
@@ -337,68 +360,84 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	const int kbeg = split * g.ksteps_per_split * HK;
 	const int kend = min(g.k, kbeg + g.ksteps_per_split * HK);
 
-	f32x16 acc[TM][TN];
+	f32x4 acc[TM][TN];
 #pragma unroll
 	for (int i = 0; i < TM; ++i)
 #pragma unroll
-		for (int j = 0; j < TN; ++j)
-#pragma unroll
-			for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+		for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
 	SA sa;
 	SB sb;
 	sa.init(g.a, g.a_bytes, g.lda, m0, kbeg, wave, lane);
 	sb.init(g.b, g.b_bytes, g.ldb, n0, kbeg, wave, lane);
 	const unsigned at = lds_address(lds);
-	// piece i of what a tile takes: the first operand's, then the second's
-	auto ask = [&](int tile, int i) {
-		const unsigned to = at + (tile & 1) * (TILE * 2);
-		if (i < SA::PIECES) {
-			sa.issue(i, to, kbeg + tile * HK, kend, wave);
-			if (i == SA::PIECES - 1) sa.advance();
-		} else {
-			sb.issue(i - SA::PIECES, to + SA::HALVES * 2, kbeg + tile * HK, kend, wave);
-			if (i == FLIGHT - 1) sb.advance();
-		}
+	auto ask_a = [&](int tile, int half, int i) {
+		sa.issue(i, at + ((tile & 1) * TILE + half * SA::HALVES) * 2, kbeg + tile * HK, kend, wave, half);
+		if (half == 1 && i == NH - 1) sa.advance();
 	};
-	f16x8 av[2][TM], bv[2][TN];
-	auto fetch = [&](int tile, int s, int i, int half) {          // fragment i of step s
-		const f16 *as = lds + (tile & 1) * TILE, *bs = as + SA::HALVES;
-		if (i < TN) bv[half][i] = SB::fragment(bs, wn * (BN / WN) + i * 32, s, lane);
-		else av[half][i - TN] = SA::fragment(as, wm * (BM / WM) + (i - TN) * 32, s, lane);
+	auto ask_b = [&](int tile, int i) {
+		sb.issue(i, at + ((tile & 1) * TILE + 2 * SA::HALVES) * 2, kbeg + tile * HK, kend, wave, 0);
+		if (i == NB - 1) sb.advance();
 	};
-	// the TM x TN matrix instructions on fragments `half`, each followed by a share of what else the wave has to issue: the next
-	// fragments, the next tile's requests. Left alone, the scheduler collects them between the blocks, where the matrix pipe stands.
-	constexpr int OPS = TM * TN, FRAGMENTS = TM + TN;
-	auto block = [&](int half, int tile, int s, int asked) {
+	// a tile is 2 TM steps: step y multiplies the fragment of rows 16 (y / 2) at reduction half y mod 2 with TN fragments of the other
+	// operand. Each step also issues a share of what else there is to issue; left alone, the scheduler collects that between the steps,
+	// where the matrix pipe stands.
+	constexpr int STEPS = 2 * TM, AHEAD = 3;
+	static_assert(STEPS % 4 == 0 && TM >= 4, "fragments are fetched three steps ahead, inside a half or into the next one");
+	f16x8 av[4], bv[2][TN];
+	auto fetch_a = [&](int tile, int y) {
+		const int i = y / 2, half = i / (TM / 2);
+		av[y % 4] = SA::fragment(lds + (tile & 1) * TILE + half * SA::HALVES, wm * (BM / WM / 2) + i % (TM / 2) * 16, y % 2, lane);
+	};
+	auto fetch_b = [&](int tile, int s) {
 #pragma unroll
-		for (int x = 0; x < OPS; ++x) {
-			const int i = x / TN, j = x % TN;
-			acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(bv[half][j], av[half][i], acc[i][j], 0, 0, 0);
+		for (int j = 0; j < TN; ++j) bv[s][j] = SB::fragment(lds + (tile & 1) * TILE + 2 * SA::HALVES, wn * (BN / WN) + j * 16, s, lane);
+	};
+	const int tiles = (kend - kbeg + HK - 1) / HK;
 #pragma unroll
-			for (int f = x * FRAGMENTS / OPS; f < (x + 1) * FRAGMENTS / OPS; ++f) fetch(tile, s, f, half ^ 1);
-			if (asked >= 0) {
+	for (int t = 0; t < 2; ++t) {
 #pragma unroll
-				for (int f = x * FLIGHT / OPS; f < (x + 1) * FLIGHT / OPS; ++f) ask(asked, f);
+		for (int i = 0; i < NH; ++i) ask_a(t, 0, i);
+#pragma unroll
+		for (int i = 0; i < NB; ++i) ask_b(t, i);
+#pragma unroll
+		for (int i = 0; i < NH; ++i) ask_a(t, 1, i);
+	}
+	meet<3 * NH + NB>();
+	fetch_b(0, 0);
+#pragma unroll
+	for (int y = 0; y < AHEAD; ++y) fetch_a(0, y);
+	for (int t = 0; t < tiles; ++t) {
+#pragma unroll
+		for (int y = 0; y < STEPS; ++y) {
+			// behind step TM - 3 every wave has read half 0 and the n side of this tile, and half 1 is there; behind step 2 TM - 3 it has read
+			// half 1, and half 0 and the n side of the next tile are there. What was asked for since may still be on its way.
+			const bool middle = y >= TM - AHEAD && y < TM, end = y >= STEPS - AHEAD, border = y == TM - AHEAD || y == STEPS - AHEAD;
+			auto fetch = [&]() { y + AHEAD < STEPS ? fetch_a(t, y + AHEAD) : fetch_a(t + 1, y + AHEAD - STEPS); };
+			if (!border) fetch();
+			if (y == 0) fetch_b(t, 1);
+			if (y == STEPS - 1) fetch_b(t + 1, 0);
+#pragma unroll
+			for (int j = 0; j < TN; ++j) acc[y / 2][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[y % 2][j], av[y % 4], acc[y / 2][j], 0, 0, 0);
+			__builtin_amdgcn_sched_barrier(0);
+			if (border) {
+				meet<2 * NH + NB>();
+				fetch();
+			}
+			if (middle) {
+				constexpr int SHARE = (NH + NB + AHEAD - 1) / AHEAD;
+				const int from = (y - (TM - AHEAD)) * SHARE;
+#pragma unroll
+				for (int i = from; i < from + SHARE && i < NH + NB; ++i) i < NH ? ask_a(t + 2, 0, i) : ask_b(t + 2, i - NH);
+			}
+			if (end) {
+				constexpr int SHARE = (NH + AHEAD - 1) / AHEAD;
+				const int from = (y - (STEPS - AHEAD)) * SHARE;
+#pragma unroll
+				for (int i = from; i < from + SHARE && i < NH; ++i) ask_a(t + 2, 1, i);
 			}
 			__builtin_amdgcn_sched_barrier(0);
 		}
-	};
-
-	const int tiles = (kend - kbeg + HK - 1) / HK;
-#pragma unroll
-	for (int t = 0; t < 2; ++t)
-#pragma unroll
-		for (int i = 0; i < FLIGHT; ++i) ask(t, i);
-	meet<FLIGHT>();
-#pragma unroll
-	for (int i = 0; i < FRAGMENTS; ++i) fetch(0, 0, i, 0);
-	for (int t = 0; t < tiles; ++t) {
-		block(0, t, 1, -1);
-		block(1, t, 2, -1);
-		block(0, t, 3, -1);
-		meet<0>();
-		block(1, t + 1, 0, t + 2);
 	}
 	meet<0>();                       // the slabs below lie over the tiles
 	Out::run(g, acc, reinterpret_cast<float *>(lds) + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);

@@ -379,20 +379,57 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 		sb.issue(i, at + ((tile & 1) * TILE + 2 * SA::HALVES) * 2, kbeg + tile * HK, kend, wave, 0);
 		if (i == NB - 1) sb.advance();
 	};
-	// a tile is 2 TM steps: step y multiplies the fragment of rows 16 (y / 2) at reduction half y mod 2 with TN fragments of the other
-	// operand. Each step also issues a share of what else there is to issue; left alone, the scheduler collects that between the steps,
-	// where the matrix pipe stands.
+	// a tile is 2 TM steps, TM for each half of the rows: step y multiplies the fragment of 16 rows at one reduction half s with TN fragments
+	// of the other operand. The halves s turn back in a half's middle (0 1 1 0, then 1 0 0 1 in the next tile), so that each set of the
+	// other operand's fragments is free, and the next one fetched, half a tile's quarter before its use. Each step also issues a share
+	// of what else there is to issue; left alone, the scheduler collects that between the steps, where the matrix pipe stands.
 	constexpr int STEPS = 2 * TM, AHEAD = 3;
-	static_assert(STEPS % 4 == 0 && TM >= 4, "fragments are fetched three steps ahead, inside a half or into the next one");
+	static_assert(TM % 4 == 0 && TN <= 4, "shares of a step");
 	f16x8 av[4], bv[2][TN];
-	auto fetch_a = [&](int tile, int y) {
-		const int i = y / 2, half = i / (TM / 2);
-		av[y % 4] = SA::fragment(lds + (tile & 1) * TILE + half * SA::HALVES, wm * (BM / WM / 2) + i % (TM / 2) * 16, y % 2, lane);
+	auto side = [](int odd, int y) { return odd ^ y / TM ^ y % TM / (TM / 2); };
+	auto fetch_a = [&](int tile, int odd, int y) {
+		av[y % 4] = SA::fragment(lds + (tile & 1) * TILE + y / TM * SA::HALVES, wm * (BM / WM / 2) + y % (TM / 2) * 16, side(odd, y), lane);
 	};
-	auto fetch_b = [&](int tile, int s) {
+	auto fetch_b = [&](int tile, int s, int j) {
+		if (j < TN) bv[s][j] = SB::fragment(lds + (tile & 1) * TILE + 2 * SA::HALVES, wn * (BN / WN) + j * 16, s, lane);
+	};
+	auto multiply = [&](auto parity, int t) {
+		constexpr int odd = decltype(parity)::value;
 #pragma unroll
-		for (int j = 0; j < TN; ++j) bv[s][j] = SB::fragment(lds + (tile & 1) * TILE + 2 * SA::HALVES, wn * (BN / WN) + j * 16, s, lane);
+		for (int y = 0; y < STEPS; ++y) {
+			// behind step TM - 3 every wave has read half 0 and the n side of this tile, and half 1 is there; behind step 2 TM - 3 it has read
+			// half 1, and half 0 and the n side of the next tile are there. What was asked for since may still be on its way.
+			const bool middle = y >= TM - AHEAD && y < TM, end = y >= STEPS - AHEAD, border = y == TM - AHEAD || y == STEPS - AHEAD;
+			auto fetch = [&]() { y + AHEAD < STEPS ? fetch_a(t, odd, y + AHEAD) : fetch_a(t + 1, odd ^ 1, y + AHEAD - STEPS); };
+			if (!border) fetch();
+			if (y < 2) fetch_b(t, odd ^ 1, 2 * y), fetch_b(t, odd ^ 1, 2 * y + 1);
+			const int i = y / TM * (TM / 2) + y % (TM / 2);
+#pragma unroll
+			for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[side(odd, y)][j], av[y % 4], acc[i][j], 0, 0, 0);
+			if (border) {
+				meet<2 * NH + NB>();
+				fetch();
+			}
+			if (end && y < STEPS - 1) {
+				const int j = 2 * (y - (STEPS - AHEAD));
+				fetch_b(t + 1, odd ^ 1, j), fetch_b(t + 1, odd ^ 1, j + 1);
+			}
+			if (middle) {
+				constexpr int SHARE = (NH + NB + AHEAD - 1) / AHEAD;
+				const int from = (y - (TM - AHEAD)) * SHARE;
+#pragma unroll
+				for (int q = from; q < from + SHARE && q < NH + NB; ++q) q < NH ? ask_a(t + 2, 0, q) : ask_b(t + 2, q - NH);
+			}
+			if (end) {
+				constexpr int SHARE = (NH + AHEAD - 1) / AHEAD;
+				const int from = (y - (STEPS - AHEAD)) * SHARE;
+#pragma unroll
+				for (int q = from; q < from + SHARE && q < NH; ++q) ask_a(t + 2, 1, q);
+			}
+			__builtin_amdgcn_sched_barrier(0);
+		}
 	};
+
 	const int tiles = (kend - kbeg + HK - 1) / HK;
 #pragma unroll
 	for (int t = 0; t < 2; ++t) {
@@ -404,40 +441,13 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 		for (int i = 0; i < NH; ++i) ask_a(t, 1, i);
 	}
 	meet<3 * NH + NB>();
-	fetch_b(0, 0);
 #pragma unroll
-	for (int y = 0; y < AHEAD; ++y) fetch_a(0, y);
-	for (int t = 0; t < tiles; ++t) {
+	for (int j = 0; j < TN; ++j) fetch_b(0, 0, j);
 #pragma unroll
-		for (int y = 0; y < STEPS; ++y) {
-			// behind step TM - 3 every wave has read half 0 and the n side of this tile, and half 1 is there; behind step 2 TM - 3 it has read
-			// half 1, and half 0 and the n side of the next tile are there. What was asked for since may still be on its way.
-			const bool middle = y >= TM - AHEAD && y < TM, end = y >= STEPS - AHEAD, border = y == TM - AHEAD || y == STEPS - AHEAD;
-			auto fetch = [&]() { y + AHEAD < STEPS ? fetch_a(t, y + AHEAD) : fetch_a(t + 1, y + AHEAD - STEPS); };
-			if (!border) fetch();
-			if (y == 0) fetch_b(t, 1);
-			if (y == STEPS - 1) fetch_b(t + 1, 0);
-#pragma unroll
-			for (int j = 0; j < TN; ++j) acc[y / 2][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[y % 2][j], av[y % 4], acc[y / 2][j], 0, 0, 0);
-			__builtin_amdgcn_sched_barrier(0);
-			if (border) {
-				meet<2 * NH + NB>();
-				fetch();
-			}
-			if (middle) {
-				constexpr int SHARE = (NH + NB + AHEAD - 1) / AHEAD;
-				const int from = (y - (TM - AHEAD)) * SHARE;
-#pragma unroll
-				for (int i = from; i < from + SHARE && i < NH + NB; ++i) i < NH ? ask_a(t + 2, 0, i) : ask_b(t + 2, i - NH);
-			}
-			if (end) {
-				constexpr int SHARE = (NH + AHEAD - 1) / AHEAD;
-				const int from = (y - (STEPS - AHEAD)) * SHARE;
-#pragma unroll
-				for (int i = from; i < from + SHARE && i < NH; ++i) ask_a(t + 2, 1, i);
-			}
-			__builtin_amdgcn_sched_barrier(0);
-		}
+	for (int y = 0; y < AHEAD; ++y) fetch_a(0, 0, y);
+	for (int t = 0; t < tiles; t += 2) {
+		multiply(std::integral_constant<int, 0>{}, t);
+		if (t + 1 < tiles) multiply(std::integral_constant<int, 1>{}, t + 1);
 	}
 	meet<0>();                       // the slabs below lie over the tiles
 	Out::run(g, acc, reinterpret_cast<float *>(lds) + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);

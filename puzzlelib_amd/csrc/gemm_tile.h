@@ -1,5 +1,5 @@
 // The operand loader of the fp32 matrix products (gemm.hip, linear.hip): one tile of rows x BK reduction steps, through registers
-// into LDS, reduction-major with a row stride of ROWS + 32 floats (why: gemm.hip).
+// into LDS, reduction-major.
 #pragma once
 #include "common.h"
 
@@ -12,10 +12,11 @@ constexpr int BK = 16;
 constexpr unsigned kOOB = 0xfffffff0u;      // buffer-load byte offset beyond every matrix: the hardware returns 0
 
 // Loads one operand tile (ROWS x BK, ROWS = BM or BN) into registers and parks it in LDS as [k][row].
-// KMAJOR: the source is stored [k][row] (row contiguous); else [row][k] (k contiguous). VEC: 16-byte buffer loads.
-template <int NT, int ROWS, bool KMAJOR, bool VEC>
+// KMAJOR: the source is stored [k][row] (row contiguous); else [row][k] (k contiguous). VEC: 16-byte buffer loads. PAD: the row stride
+// in LDS is ROWS + PAD floats.
+template <int NT, int ROWS, bool KMAJOR, bool VEC, int BK = ::BK, int PAD = 32>
 struct Loader {
-	static constexpr int LD = ROWS + 32;
+	static constexpr int LD = ROWS + PAD;
 	static constexpr int NV = ROWS * BK / 4 / NT;             // float4 per thread per tile
 	static_assert(NV >= 1 && NV * NT * 4 == ROWS * BK, "operand tile / thread count");
 	f32x4 reg[NV];

@@ -106,25 +106,14 @@ __device__ __forceinline__ void tile_of(const Product &g, int &tm, int &tn) {
 	tn = rest / rows;
 }
 
-// A wave's accumulators -> rows. The matrix instruction took the operand of the n side first, so a lane holds 4 consecutive columns of one
-// row at a time: 32 x 32 tiles, row lane & 31, columns 8 q + 4 (lane >> 5) in registers 4 q ...; 16 x 16 tiles, row lane & 15, columns
-// 4 (lane >> 4). They go through LDS in slabs of 32 rows (the wave's own, no barrier), so that consecutive lanes store consecutive runs
+// A wave's accumulators -> rows. The matrix instruction took the operand of the n side first, so a lane holds, of each 16 x 16 tile, 4
+// consecutive columns 4 (lane >> 4) of row lane & 15. They go through LDS in slabs of 32 rows (the wave's own, no barrier), so that consecutive lanes store consecutive runs
 // of a row: whole 128-byte lines instead of pieces of 16 bytes.
 template <typename T, int ROWS, int COLS>
 struct Drain {
 	static constexpr int COUNT = 16 / sizeof(T);                 // values a lane stores at once
 	static constexpr int PITCH = COLS + 4;                       // (+4: the rows of a store start 4 banks apart)
 	static constexpr int FLOATS = 32 * PITCH;
-
-	template <int TM, int TN>
-	static __device__ __forceinline__ void park(const f32x16 (&acc)[TM][TN], int i, float *lds, int lane) {
-#pragma unroll
-		for (int j = 0; j < TN; ++j)
-#pragma unroll
-			for (int q = 0; q < 4; ++q)
-				*reinterpret_cast<f32x4 *>(lds + (lane & 31) * PITCH + j * 32 + q * 8 + (lane >> 5) * 4) =
-				    (f32x4){acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-	}
 
 	template <int TM, int TN>
 	static __device__ __forceinline__ void park(const f32x4 (&acc)[TM][TN], int i, float *lds, int lane) {
@@ -166,17 +155,18 @@ struct Drain {
 	}
 };
 
-// ---- float32: v_mfma_f32_32x32x2_f32, operands through registers (gemm_tile.h) -----------------------------------------------------
-template <int BM, int BN, int WM, int WN, bool TA, bool TB, bool VEC>
+// ---- float32: v_mfma_f32_16x16x4_f32, operands through registers (gemm_tile.h) -----------------------------------------------------
+// A row stride of ROWS + 16 floats puts the four steps of a fragment on four different quarters of the 64 banks. KB: reduction steps a tile.
+template <int BM, int BN, int WM, int WN, int KB, bool TA, bool TB, bool VEC>
 __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(4, 8))) linear_f32_kernel(Product g) {
-	constexpr int NT = 64 * WM * WN, TM = BM / (32 * WM), TN = BN / (32 * WN);
-	using LA = Loader<NT, BM, TA, VEC>;
-	using LB = Loader<NT, BN, !TB, VEC>;
+	constexpr int NT = 64 * WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN);
+	using LA = Loader<NT, BM, TA, VEC, KB, 16>;
+	using LB = Loader<NT, BN, !TB, VEC, KB, 16>;
 	using Out = Drain<float, BM / WM, BN / WN>;
-	constexpr int TILES = 2 * BK * (LA::LD + LB::LD), SLABS = WM * WN * Out::FLOATS;
+	constexpr int TILES = 2 * KB * (LA::LD + LB::LD), SLABS = WM * WN * Out::FLOATS;
 	__shared__ __attribute__((aligned(16))) float lds[TILES > SLABS ? TILES : SLABS];
-	float *const As = lds, *const Bs = lds + 2 * BK * LA::LD;
-	constexpr int A = BK * LA::LD, B = BK * LB::LD;
+	float *const As = lds, *const Bs = lds + 2 * KB * LA::LD;
+	constexpr int A = KB * LA::LD, B = KB * LB::LD;
 
 	const int tid = threadIdx.x, lane = tid & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -187,19 +177,17 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 	const int split = blockIdx.z;
 	const int kbeg = split * g.ksteps_per_split * BK;
 	const int kend = min(g.k, kbeg + g.ksteps_per_split * BK);
-	const int l31 = lane & 31, lhi = lane >> 5;
+	const int l15 = lane & 15, lq = lane >> 4;
 
 	const float *a = (const float *)g.a, *b = (const float *)g.b;
 	const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc((void *)a, 0, VEC ? (unsigned)g.a_bytes : 0u, 0x00020000);
 	const __amdgpu_buffer_rsrc_t br = __builtin_amdgcn_make_buffer_rsrc((void *)b, 0, VEC ? (unsigned)g.b_bytes : 0u, 0x00020000);
 
-	f32x16 acc[TM][TN];
+	f32x4 acc[TM][TN];
 #pragma unroll
 	for (int i = 0; i < TM; ++i)
 #pragma unroll
-		for (int j = 0; j < TN; ++j)
-#pragma unroll
-			for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+		for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
 
 	LA la;
 	LB lb;
@@ -212,24 +200,24 @@ __global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_
 	__syncthreads();
 
 	int buf = 0;
-	for (int k0 = kbeg; k0 < kend; k0 += BK, buf ^= 1) {
-		const bool more = k0 + BK < kend;
+	for (int k0 = kbeg; k0 < kend; k0 += KB, buf ^= 1) {
+		const bool more = k0 + KB < kend;
 		if (more) {
-			la.load(a, ar, (int)g.lda, m0, g.m, k0 + BK, kend, tid);
-			lb.load(b, br, (int)g.ldb, n0, g.n, k0 + BK, kend, tid);
+			la.load(a, ar, (int)g.lda, m0, g.m, k0 + KB, kend, tid);
+			lb.load(b, br, (int)g.ldb, n0, g.n, k0 + KB, kend, tid);
 		}
-		const float *as = As + buf * A + wm * (BM / WM) + l31, *bs = Bs + buf * B + wn * (BN / WN) + l31;
+		const float *as = As + buf * A + wm * (BM / WM) + l15, *bs = Bs + buf * B + wn * (BN / WN) + l15;
 #pragma unroll
-		for (int ks = 0; ks < BK; ks += 2) {
+		for (int ks = 0; ks < KB; ks += 4) {
 			float av[TM], bv[TN];
 #pragma unroll
-			for (int i = 0; i < TM; ++i) av[i] = as[(ks + lhi) * LA::LD + i * 32];
+			for (int i = 0; i < TM; ++i) av[i] = as[(ks + lq) * LA::LD + i * 16];
 #pragma unroll
-			for (int j = 0; j < TN; ++j) bv[j] = bs[(ks + lhi) * LB::LD + j * 32];
+			for (int j = 0; j < TN; ++j) bv[j] = bs[(ks + lq) * LB::LD + j * 16];
 #pragma unroll
 			for (int i = 0; i < TM; ++i)
 #pragma unroll
-				for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(bv[j], av[i], acc[i][j], 0, 0, 0);
+				for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[j], av[i], acc[i][j], 0, 0, 0);
 		}
 		if (more) {
 			la.park(As + (buf ^ 1) * A, tid);
@@ -633,11 +621,11 @@ void launch_f16(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
 
 template <bool TA, bool TB, bool VEC>
 void launch_f32(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
-	if (p.bm == 256) linear_f32_kernel<256, 256, 4, 4, TA, TB, VEC><<<grid, 1024, 0, st>>>(g);
-	else if (p.bm == 128 && p.bn == 128) linear_f32_kernel<128, 128, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
-	else if (p.bm == 128) linear_f32_kernel<128, 64, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
-	else if (p.bn == 128) linear_f32_kernel<64, 128, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
-	else linear_f32_kernel<64, 64, 2, 2, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	if (p.bm == 256) linear_f32_kernel<256, 256, 4, 4, 32, TA, TB, VEC><<<grid, 1024, 0, st>>>(g);
+	else if (p.bm == 128 && p.bn == 128) linear_f32_kernel<128, 128, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	else if (p.bm == 128) linear_f32_kernel<128, 64, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	else if (p.bn == 128) linear_f32_kernel<64, 128, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+	else linear_f32_kernel<64, 64, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
 }
 
 size_t extent_of(int rows, int wide, long ld, int size) { return rows > 0 ? ((size_t)(rows - 1) * ld + wide) * size : 0; }

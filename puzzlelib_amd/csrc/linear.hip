@@ -5,12 +5,12 @@
 // Every product is C[m][n] = sum_k A(m, k) B(k, n) with A stored [m][k] or [k][m] and B stored [k][n] or [n][k]; the forward pass is
 // x W, the backward pass dz W^T and x^T dz with dz = dy * keep / (1 - p) * act'(z) written once by linear_gate_kernel, which also
 // leaves the column sums that become db.
-#include "gemm_tile.h"
 #include "philox.h"
 #include "rows.h"
 
 #include <type_traits>
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __fp16 tr16x4 __attribute__((ext_vector_type(4)));
 
@@ -155,86 +155,19 @@ struct Drain {
 	}
 };
 
-// ---- float32: v_mfma_f32_16x16x4_f32, operands through registers (gemm_tile.h) -----------------------------------------------------
-// A row stride of ROWS + 16 floats puts the four steps of a fragment on four different quarters of the 64 banks. KB: reduction steps a tile.
-template <int BM, int BN, int WM, int WN, int KB, bool TA, bool TB, bool VEC>
-__global__ void __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(4, 8))) linear_f32_kernel(Product g) {
-	constexpr int NT = 64 * WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN);
-	using LA = Loader<NT, BM, TA, VEC, KB, 16>;
-	using LB = Loader<NT, BN, !TB, VEC, KB, 16>;
-	using Out = Drain<float, BM / WM, BN / WN>;
-	constexpr int TILES = 2 * KB * (LA::LD + LB::LD), SLABS = WM * WN * Out::FLOATS;
-	__shared__ __attribute__((aligned(16))) float lds[TILES > SLABS ? TILES : SLABS];
-	float *const As = lds, *const Bs = lds + 2 * KB * LA::LD;
-	constexpr int A = KB * LA::LD, B = KB * LB::LD;
-
-	const int tid = threadIdx.x, lane = tid & 63;
-	const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-	const int wm = wave / WN, wn = wave % WN;
-	int tm, tn;
-	tile_of(g, tm, tn);
-	const int m0 = tm * BM, n0 = tn * BN;
-	const int split = blockIdx.z;
-	const int kbeg = split * g.ksteps_per_split * BK;
-	const int kend = min(g.k, kbeg + g.ksteps_per_split * BK);
-	const int l15 = lane & 15, lq = lane >> 4;
-
-	const float *a = (const float *)g.a, *b = (const float *)g.b;
-	const __amdgpu_buffer_rsrc_t ar = __builtin_amdgcn_make_buffer_rsrc((void *)a, 0, VEC ? (unsigned)g.a_bytes : 0u, 0x00020000);
-	const __amdgpu_buffer_rsrc_t br = __builtin_amdgcn_make_buffer_rsrc((void *)b, 0, VEC ? (unsigned)g.b_bytes : 0u, 0x00020000);
-
-	f32x4 acc[TM][TN];
-#pragma unroll
-	for (int i = 0; i < TM; ++i)
-#pragma unroll
-		for (int j = 0; j < TN; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-
-	LA la;
-	LB lb;
-	la.init((int)g.lda, m0, g.m, kbeg, tid);
-	lb.init((int)g.ldb, n0, g.n, kbeg, tid);
-	la.load(a, ar, (int)g.lda, m0, g.m, kbeg, kend, tid);
-	lb.load(b, br, (int)g.ldb, n0, g.n, kbeg, kend, tid);
-	la.park(As, tid);
-	lb.park(Bs, tid);
-	__syncthreads();
-
-	int buf = 0;
-	for (int k0 = kbeg; k0 < kend; k0 += KB, buf ^= 1) {
-		const bool more = k0 + KB < kend;
-		if (more) {
-			la.load(a, ar, (int)g.lda, m0, g.m, k0 + KB, kend, tid);
-			lb.load(b, br, (int)g.ldb, n0, g.n, k0 + KB, kend, tid);
-		}
-		const float *as = As + buf * A + wm * (BM / WM) + l15, *bs = Bs + buf * B + wn * (BN / WN) + l15;
-#pragma unroll
-		for (int ks = 0; ks < KB; ks += 4) {
-			float av[TM], bv[TN];
-#pragma unroll
-			for (int i = 0; i < TM; ++i) av[i] = as[(ks + lq) * LA::LD + i * 16];
-#pragma unroll
-			for (int j = 0; j < TN; ++j) bv[j] = bs[(ks + lq) * LB::LD + j * 16];
-#pragma unroll
-			for (int i = 0; i < TM; ++i)
-#pragma unroll
-				for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(bv[j], av[i], acc[i][j], 0, 0, 0);
-		}
-		if (more) {
-			la.park(As + (buf ^ 1) * A, tid);
-			lb.park(Bs + (buf ^ 1) * B, tid);
-		}
-		__syncthreads();
-	}
-	Out::run(g, acc, lds + wave * Out::FLOATS, m0 + wm * (BM / WM), n0 + wn * (BN / WN), split, lane);
-}
-
-// ---- float16: v_mfma_f32_16x16x32_f16, operands straight into LDS --------------------------------------------------------------------
-// LDS holds two tiles of HK = 64 reduction steps: 128 bytes of a row whose contiguous axis is k, one L2 request each. A wave keeps the n
-// side's fragments of a whole tile in registers and walks over its rows, so that a tile's place in LDS frees in pieces: the n side and
-// the first half of the m side's rows ("half 0") in the tile's middle, the other rows at its end. What the tile after the next one puts
-// there is asked for at once and not needed for one and a half tiles — about 1.5 us, the time a line takes that no L2 holds. (Asked for
-// a tile at a time, behind its last block, the same kernel waited 40 % of its time: 465000 instead of 380000 cycles for 8192 x 8192 x 2048.)
-constexpr int HK = 64;
+// ---- the product: operands straight into LDS, v_mfma_f32_16x16x32_f16 or v_mfma_f32_16x16x4_f32 -----------------------------------------
+// LDS holds two tiles of 128 bytes of reduction steps (64 float16, 32 float32): of a row whose contiguous axis is k that is one L2 request.
+// A wave keeps the n side's fragments of half a tile in registers and walks over its rows, so that a tile's place in LDS frees in pieces:
+// the n side and the first half of the m side's rows ("half 0") in the tile's middle, the other rows at its end. What the tile after
+// the next one puts there is asked for at once and not needed for one and a half tiles — about 1.5 us, the time a line takes that no L2
+// holds. Per-step costs matter as much as waits: 8192 x 8192 x 2048 in float16 runs into the card's power limit (1.9 of 2.4 GHz, the matrix
+// pipes busy 60 % of the cycles). 16 x 16 instructions move half the accumulator bytes of 32 x 32 ones and hold a higher clock: 248
+// instead of 263 us.
+// A fragment is 16 bytes a lane: row lane & 15, steps (lane >> 4) C ... + C - 1 of 4 C, C = 16 / sizeof(T). In float16 that is one matrix
+// instruction's operand; in float32 element e feeds the e-th of four instructions, each of which sums the steps 4 q + e — any four will
+// do, as long as both operands take the same ones.
+template <typename T>
+constexpr int kSteps = 128 / sizeof(T);
 
 __device__ __forceinline__ unsigned lds_address(const void *p) {
 	return (unsigned)(size_t)(__attribute__((address_space(3))) const void *)p;
@@ -252,22 +185,25 @@ __device__ __forceinline__ void meet() {
 	asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LEFT) : "memory");
 }
 
-// ROWS rows of one operand x HK, staged by WAVES waves: rows row0 + (q / RUN) 2 RUN + half RUN + q mod RUN, q < ROWS — half of the rows of
-// every wave, or all rows (RUN = ROWS, half 0). LDS has 64 banks of 4 bytes; a read is spread so that 16 neighbouring lanes of
-// a ds_read_b128, or 32 of a ds_read_b64, touch each bank once.
+// ROWS rows of one operand x 128 bytes of steps, staged by WAVES waves: rows row0 + (q / RUN) 2 RUN + half RUN + q mod RUN, q < ROWS — half of
+// the rows of every wave, or all rows (RUN = ROWS, half 0). LDS has 64 banks of 4 bytes; a read is spread so that 16 neighbouring lanes
+// of a ds_read_b128, 32 of a ds_read_b64 or 64 of a ds_read_b32 touch each bank once.
 // KMAJOR = false: [row][k] in memory, so 128 bytes of k per row in LDS, two rows to all banks; the 16-byte pieces of row r stand at
 //   piece ^ (r / 2 mod 8), so the fragment's 16 rows at one piece land on 16 different places.
-// KMAJOR = true: [k][row] in memory, so ROWS * 2 bytes per k in LDS; fragments are read with ds_read_b64_tr_b16, which hands 16 lanes
-//   the 4 x 16 block of 4 steps x 16 rows transposed. 32 lanes take one 32-byte piece of each of 8 steps (k mod 4 and k / 8 mod 2 tell
-//   them apart): the pieces of step k stand at piece ^ turn(k), which gives the 8 steps 8 different places.
-template <int ROWS, int RUN, bool KMAJOR, int WAVES>
+// KMAJOR = true: [k][row] in memory, so a row of ROWS values per k in LDS, in pieces of 16 rows; the pieces of step k stand at
+//   piece ^ turn(k). Float16 fragments are read with ds_read_b64_tr_b16, which hands 16 lanes the 4 x 16 block of 4 steps x 16 rows
+//   transposed: 32 lanes take one piece of each of 8 steps (k mod 4 and k / 8 mod 2 tell them apart). Float32 fragments are read element
+//   by element: 64 lanes take one piece of each of 4 steps (k / 4 mod 4).
+template <typename T, int ROWS, int RUN, bool KMAJOR, int WAVES>
 struct Stage {
-	static constexpr int HALVES = ROWS * HK;
+	static constexpr int SIZE = sizeof(T), HK = kSteps<T>, C = 16 / SIZE;
+	static constexpr int VALUES = ROWS * HK;
 	static constexpr int PIECES = ROWS / 8 / WAVES;            // dma16 per wave and tile
 	static_assert(PIECES >= 1 && PIECES * WAVES * 8 == ROWS, "tile / waves");
 
-	__device__ __forceinline__ static int turn(int k) {                   // (64 rows: two steps to all banks, 32: four)
-		return ROWS == 32 ? k >> 3 & 1 : ROWS == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2;
+	__device__ __forceinline__ static int turn(int k) {
+		if (SIZE == 4) return k >> 2 & (ROWS == 32 ? 1 : 3);
+		return ROWS == 32 ? k >> 3 & 1 : ROWS == 64 ? (k >> 1 & 1) | (k >> 3 & 1) << 1 : (k & 3) | (k >> 3 & 1) << 2;      // (64 rows: two steps to all banks, 32: four)
 	}
 	__device__ __forceinline__ static int spot(int r) { return r >> 1 & 7; }
 
@@ -278,21 +214,21 @@ struct Stage {
 	int kpiece[PIECES];              // KMAJOR = false: first k of the lane's pieces
 
 	__device__ __forceinline__ void init(const void *src, size_t extent, long ld, int row0, int kbeg, int wave, int lane) {
-		const size_t start = KMAJOR ? ((size_t)kbeg * ld + row0) * 2 : ((size_t)row0 * ld + kbeg) * 2;
+		const size_t start = KMAJOR ? ((size_t)kbeg * ld + row0) * SIZE : ((size_t)row0 * ld + kbeg) * SIZE;
 		p = (const char *)src + start;
 		bytes = (long)(extent - start);
-		step = KMAJOR ? HK * ld * 2 : HK * 2;
-		shift = KMAJOR ? RUN * 2 : RUN * ld * 2;
+		step = KMAJOR ? HK * ld * SIZE : HK * SIZE;
+		shift = KMAJOR ? RUN * SIZE : RUN * ld * SIZE;
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
 			const int o = ((wave * PIECES + i) * 64 + lane) * 16;                // place in the LDS tile
 			if (KMAJOR) {
-				const int k = o / (ROWS * 2), at = o % (ROWS * 2) / 16, q = (((at >> 1) ^ turn(k)) * 2 + (at & 1)) * 8;
-				off[i] = (unsigned)((size_t)k * ld * 2) + (q / RUN * (2 * RUN) + q % RUN) * 2;
+				const int k = o / (ROWS * SIZE), at = o % (ROWS * SIZE) / 16, q = ((at / SIZE) ^ turn(k)) * 16 + at % SIZE * C;
+				off[i] = (unsigned)((size_t)k * ld * SIZE) + (q / RUN * (2 * RUN) + q % RUN) * SIZE;
 			} else {
-				const int q = o / (HK * 2), piece = (o / 16 % (HK / 8)) ^ spot(q);
-				kpiece[i] = piece * 8;
-				off[i] = (unsigned)((size_t)(q / RUN * (2 * RUN) + q % RUN) * ld * 2) + piece * 16;
+				const int q = o / 128, piece = (o / 16 % 8) ^ spot(q);
+				kpiece[i] = piece * C;
+				off[i] = (unsigned)((size_t)(q / RUN * (2 * RUN) + q % RUN) * ld * SIZE) + piece * 16;
 			}
 		}
 	}
@@ -308,35 +244,59 @@ struct Stage {
 
 	__device__ __forceinline__ void advance() { p += step, bytes -= step; }
 
-	// fragment of v_mfma_f32_16x16x32_f16: rows row0 + (lane & 15), steps 32 s + 8 (lane >> 4) ... + 7
-	__device__ __forceinline__ static f16x8 fragment(const f16 *tile, int row0, int s, int lane) {
+	// fragment s of rows row0 + (lane & 15)
+	__device__ __forceinline__ static f32x4 fragment(const T *tile, int row0, int s, int lane) {
 		const int j = lane & 15;
 		if (!KMAJOR) {
 			const int r = row0 + j, piece = s * 4 + (lane >> 4);
-			return *reinterpret_cast<const f16x8 *>(tile + r * HK + ((piece ^ spot(r)) * 8));
+			return *reinterpret_cast<const f32x4 *>(tile + r * HK + ((piece ^ spot(r)) * C));
+		}
+		if (SIZE == 4) {
+			f32x4 f;
+#pragma unroll
+			for (int e = 0; e < 4; ++e) {
+				const int k = s * 16 + (lane >> 4) * 4 + e;
+				f[e] = (float)tile[k * ROWS + ((row0 / 16) ^ turn(k)) * 16 + j];
+			}
+			return f;
 		}
 		// lane j of the 16 that share 8 steps points at step (j >> 2), rows 4 (j & 3) ... + 3 of their 4 x 16 block
 		const int k = s * 32 + (lane >> 4) * 8 + (j >> 2);
-		union { f16x8 v; tr16x4 h[2]; } f;
+		union { f32x4 v; tr16x4 h[2]; } f;
 #pragma unroll
 		for (int half = 0; half < 2; ++half) {
 			const int kk = k + half * 4;
-			const f16 *at = tile + kk * ROWS + ((row0 / 16) ^ turn(kk)) * 16 + (j & 3) * 4;
+			const T *at = tile + kk * ROWS + ((row0 / 16) ^ turn(kk)) * 16 + (j & 3) * 4;
 			f.h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4f16((__attribute__((address_space(3))) tr16x4 *)at);
 		}
 		return f.v;
 	}
 };
 
-template <int BM, int BN, int WM, int WN, bool TA, bool TB>
-__global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
-	constexpr int WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN);
-	using SA = Stage<BM / 2, BM / WM / 2, TA, WAVES>;            // a half of the rows
-	using SB = Stage<BN, BN, !TB, WAVES>;
-	using Out = Drain<f16, BM / WM, BN / WN>;
-	constexpr int TILE = 2 * SA::HALVES + SB::HALVES, SLABS = 2 * WAVES * Out::FLOATS;
+// acc[j] += a b[j]; in float32 the instructions on one accumulator stand N apart
+template <typename T, int N>
+__device__ __forceinline__ void multiply_add(f32x4 (&acc)[N], const f32x4 &a, const f32x4 (&b)[N]) {
+	if (sizeof(T) == 2) {
+#pragma unroll
+		for (int j = 0; j < N; ++j)
+			acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, b[j]), __builtin_bit_cast(f16x8, a), acc[j], 0, 0, 0);
+	} else {
+#pragma unroll
+		for (int e = 0; e < 4; ++e)
+#pragma unroll
+			for (int j = 0; j < N; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(b[j][e], a[e], acc[j], 0, 0, 0);
+	}
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB>
+__global__ void __launch_bounds__(64 * WM * WN) linear_kernel(Product g) {
+	constexpr int HK = kSteps<T>, WAVES = WM * WN, TM = BM / (16 * WM), TN = BN / (16 * WN);
+	using SA = Stage<T, BM / 2, BM / WM / 2, TA, WAVES>;            // a half of the rows
+	using SB = Stage<T, BN, BN, !TB, WAVES>;
+	using Out = Drain<T, BM / WM, BN / WN>;
+	constexpr int TILE = 2 * SA::VALUES + SB::VALUES, SLABS = WAVES * Out::FLOATS * 4 / (int)sizeof(T);
 	constexpr int NH = SA::PIECES, NB = SB::PIECES;              // dma16 per wave: a half of the m side, the n side
-	__shared__ __attribute__((aligned(1024))) f16 lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
+	__shared__ __attribute__((aligned(1024))) T lds[2 * TILE > SLABS ? 2 * TILE : SLABS];
 
 	const int lane = threadIdx.x & 63;
 	const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -360,11 +320,11 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	sb.init(g.b, g.b_bytes, g.ldb, n0, kbeg, wave, lane);
 	const unsigned at = lds_address(lds);
 	auto ask_a = [&](int tile, int half, int i) {
-		sa.issue(i, at + ((tile & 1) * TILE + half * SA::HALVES) * 2, kbeg + tile * HK, kend, wave, half);
+		sa.issue(i, at + ((tile & 1) * TILE + half * SA::VALUES) * (int)sizeof(T), kbeg + tile * HK, kend, wave, half);
 		if (half == 1 && i == NH - 1) sa.advance();
 	};
 	auto ask_b = [&](int tile, int i) {
-		sb.issue(i, at + ((tile & 1) * TILE + 2 * SA::HALVES) * 2, kbeg + tile * HK, kend, wave, 0);
+		sb.issue(i, at + ((tile & 1) * TILE + 2 * SA::VALUES) * (int)sizeof(T), kbeg + tile * HK, kend, wave, 0);
 		if (i == NB - 1) sb.advance();
 	};
 	// a tile is 2 TM steps, TM for each half of the rows: step y multiplies the fragment of 16 rows at one reduction half s with TN fragments
@@ -373,13 +333,13 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 	// of what else there is to issue; left alone, the scheduler collects that between the steps, where the matrix pipe stands.
 	constexpr int STEPS = 2 * TM, AHEAD = 3;
 	static_assert(TM % 4 == 0 && TN <= 4, "shares of a step");
-	f16x8 av[4], bv[2][TN];
+	f32x4 av[4], bv[2][TN];
 	auto side = [](int odd, int y) { return odd ^ y / TM ^ y % TM / (TM / 2); };
 	auto fetch_a = [&](int tile, int odd, int y) {
-		av[y % 4] = SA::fragment(lds + (tile & 1) * TILE + y / TM * SA::HALVES, wm * (BM / WM / 2) + y % (TM / 2) * 16, side(odd, y), lane);
+		av[y % 4] = SA::fragment(lds + (tile & 1) * TILE + y / TM * SA::VALUES, wm * (BM / WM / 2) + y % (TM / 2) * 16, side(odd, y), lane);
 	};
 	auto fetch_b = [&](int tile, int s, int j) {
-		if (j < TN) bv[s][j] = SB::fragment(lds + (tile & 1) * TILE + 2 * SA::HALVES, wn * (BN / WN) + j * 16, s, lane);
+		if (j < TN) bv[s][j] = SB::fragment(lds + (tile & 1) * TILE + 2 * SA::VALUES, wn * (BN / WN) + j * 16, s, lane);
 	};
 	auto multiply = [&](auto parity, int t) {
 		constexpr int odd = decltype(parity)::value;
@@ -392,8 +352,7 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_f16_kernel(Product g) {
 			if (!border) fetch();
 			if (y < 2) fetch_b(t, odd ^ 1, 2 * y), fetch_b(t, odd ^ 1, 2 * y + 1);
 			const int i = y / TM * (TM / 2) + y % (TM / 2);
-#pragma unroll
-			for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(bv[side(odd, y)][j], av[y % 4], acc[i][j], 0, 0, 0);
+			multiply_add<T>(acc[i], av[y % 4], bv[side(odd, y)]);
 			if (border) {
 				meet<2 * NH + NB>();
 				fetch();
@@ -575,7 +534,7 @@ Plan plan_product(int dtype, const Operands &o) {
 	Plan p{};
 	if (o.m == 0 || o.n == 0) return p;                                 // (no output, nothing runs)
 	const int size = dtype == PZ_F16 ? 2 : 4;
-	p.bk = dtype == PZ_F16 ? HK : BK;
+	p.bk = dtype == PZ_F16 ? kSteps<f16> : kSteps<float>;
 	p.bm = o.m > 64 ? 128 : 64, p.bn = o.n > 64 ? 128 : 64;
 	const long tiles256 = (long)pz::ceil_div(o.m, 256) * pz::ceil_div(o.n, 256);
 	if (o.k >= (dtype == PZ_F16 ? 256 : 1024) && tiles256 >= pz::kNumCU) p.bm = p.bn = 256;
@@ -610,22 +569,20 @@ int align_operand(const void *&src, long &ld, int rows, int cols, char *at, hipS
 	return PZ_OK;
 }
 
-template <bool TA, bool TB>
-void launch_f16(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
-	if (p.bm == 256) linear_f16_kernel<256, 256, 2, 4, TA, TB><<<grid, 512, 0, st>>>(g);
-	else if (p.bm == 128 && p.bn == 128) linear_f16_kernel<128, 128, 2, 2, TA, TB><<<grid, 256, 0, st>>>(g);
-	else if (p.bm == 128) linear_f16_kernel<128, 64, 2, 1, TA, TB><<<grid, 128, 0, st>>>(g);
-	else if (p.bn == 128) linear_f16_kernel<64, 128, 1, 2, TA, TB><<<grid, 128, 0, st>>>(g);
-	else linear_f16_kernel<64, 64, 1, 1, TA, TB><<<grid, 64, 0, st>>>(g);
+template <typename T, bool TA, bool TB>
+void launch(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
+	if (p.bm == 256) linear_kernel<T, 256, 256, 2, 4, TA, TB><<<grid, 512, 0, st>>>(g);
+	else if (p.bm == 128 && p.bn == 128) linear_kernel<T, 128, 128, 2, 2, TA, TB><<<grid, 256, 0, st>>>(g);
+	else if (p.bm == 128) linear_kernel<T, 128, 64, 2, 1, TA, TB><<<grid, 128, 0, st>>>(g);
+	else if (p.bn == 128) linear_kernel<T, 64, 128, 1, 2, TA, TB><<<grid, 128, 0, st>>>(g);
+	else linear_kernel<T, 64, 64, 1, 1, TA, TB><<<grid, 64, 0, st>>>(g);
 }
 
-template <bool TA, bool TB, bool VEC>
-void launch_f32(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
-	if (p.bm == 256) linear_f32_kernel<256, 256, 4, 4, 32, TA, TB, VEC><<<grid, 1024, 0, st>>>(g);
-	else if (p.bm == 128 && p.bn == 128) linear_f32_kernel<128, 128, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
-	else if (p.bm == 128) linear_f32_kernel<128, 64, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
-	else if (p.bn == 128) linear_f32_kernel<64, 128, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
-	else linear_f32_kernel<64, 64, 2, 2, 16, TA, TB, VEC><<<grid, 256, 0, st>>>(g);
+template <typename T>
+void launch(const Plan &p, const Product &g, bool ta, bool tb, dim3 grid, hipStream_t st) {
+	if (ta) launch<T, true, false>(p, g, grid, st);
+	else if (tb) launch<T, false, true>(p, g, grid, st);
+	else launch<T, false, false>(p, g, grid, st);
 }
 
 size_t extent_of(int rows, int wide, long ld, int size) { return rows > 0 ? ((size_t)(rows - 1) * ld + wide) * size : 0; }
@@ -656,16 +613,8 @@ int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st
 	g.epi.m = o.m, g.epi.n = o.n;
 
 	const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)p.splits);
-	if (dtype == PZ_F16) {
-		if (o.ta) launch_f16<true, false>(p, g, grid, st);
-		else if (o.tb) launch_f16<false, true>(p, g, grid, st);
-		else launch_f16<false, false>(p, g, grid, st);
-	} else {
-		const bool vec = g.a_bytes < 0xffff0000ull && g.b_bytes < 0xffff0000ull;       // 16-byte buffer loads reach 4 GiB
-		if (o.ta) vec ? launch_f32<true, false, true>(p, g, grid, st) : launch_f32<true, false, false>(p, g, grid, st);
-		else if (o.tb) vec ? launch_f32<false, true, true>(p, g, grid, st) : launch_f32<false, true, false>(p, g, grid, st);
-		else vec ? launch_f32<false, false, true>(p, g, grid, st) : launch_f32<false, false, false>(p, g, grid, st);
-	}
+	if (dtype == PZ_F16) launch<f16>(p, g, o.ta, o.tb, grid, st);
+	else launch<float>(p, g, o.ta, o.tb, grid, st);
 	PZ_LAUNCH_CHECK();
 	if (p.splits > 1) {
 		const size_t items = (size_t)o.m * pz::ceil_div(o.n, 16 / size);

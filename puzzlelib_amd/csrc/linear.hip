@@ -32,59 +32,96 @@ struct Epilogue {
 	DropKey drop;
 };
 
-// COUNT sums of row `row`, columns col ... (col + COUNT - 1 may lie beyond the matrix)
-template <typename T, int COUNT>
-__device__ __forceinline__ void finish_run(const Epilogue &e, int row, int col, float (&s)[COUNT]) {
-	const int left = e.n - col;
-	if (row >= e.m || left <= 0) return;
-	const bool whole = e.vec && left >= COUNT;
-
+// COUNT finished sums of a row, whose first is element `index` of the (m, n) tensor; the callers say how runs are loaded and stored
+template <int COUNT, typename LoadOld, typename LoadResidual, typename StorePreact, typename StoreOut>
+__device__ __forceinline__ void finish(const Epilogue &e, float (&s)[COUNT], const float (&bias)[COUNT], uint64_t index, LoadOld load_old,
+                                       LoadResidual load_residual, StorePreact store_preact, StoreOut store_out) {
 	if (e.kind == EPI_ACCUMULATE) {
 #pragma unroll
 		for (int i = 0; i < COUNT; ++i) s[i] *= e.alpha;
-		auto add = [&](auto *c) {
-			if (e.beta != 0.f) {
-				float old[COUNT];
-				load_run(c, whole, left, old);
+		if (e.beta != 0.f) {
+			float old[COUNT];
+			load_old(old);
 #pragma unroll
-				for (int i = 0; i < COUNT; ++i) s[i] += e.beta * old[i];
-			}
-			store_run(c, whole, left, s);
-		};
-		const size_t at = (size_t)row * e.ldo + col;
-		if (e.out_f32) add((float *)e.out + at);
-		else add((T *)e.out + at);
+			for (int i = 0; i < COUNT; ++i) s[i] += e.beta * old[i];
+		}
+		store_out(s);
 		return;
 	}
-
-	if (e.bias) {
-		float b[COUNT];
-		load_run(e.bias + col, whole, left, b);
 #pragma unroll
-		for (int i = 0; i < COUNT; ++i) s[i] += b[i];
-	}
-	if (e.preact) store_run((T *)e.preact + (size_t)row * e.ldp + col, whole, left, s);
+	for (int i = 0; i < COUNT; ++i) s[i] += bias[i];
+	if (e.preact) store_preact(s);
 	if (e.act != PZ_ACT_NONE) {
 #pragma unroll
 		for (int i = 0; i < COUNT; ++i) s[i] = act_value(s[i], e.act);
 	}
 	if (e.dropping) {
-		const unsigned bits = drop_bits<COUNT>(e.drop, (uint64_t)row * e.n + col);
+		const unsigned bits = drop_bits<COUNT>(e.drop, index);
 #pragma unroll
 		for (int i = 0; i < COUNT; ++i) s[i] = bits >> i & 1u ? s[i] * e.inv_keep : 0.f;
 	}
 	if (e.residual) {
 		float r[COUNT];
-		load_run((const T *)e.residual + (size_t)row * e.ldr + col, whole, left, r);
+		load_residual(r);
 #pragma unroll
 		for (int i = 0; i < COUNT; ++i) s[i] += r[i];
 	}
-	store_run((T *)e.out + (size_t)row * e.ldo + col, whole, left, s);
+	store_out(s);
 }
+
+template <int COUNT>
+__device__ __forceinline__ void load_bias(const Epilogue &e, int col, float (&bias)[COUNT]) {
+#pragma unroll
+	for (int i = 0; i < COUNT; ++i) bias[i] = 0.f;
+	if (e.kind == EPI_FORWARD && e.bias && col < e.n) load_run(e.bias + col, e.vec && col + COUNT <= e.n, e.n - col, bias);
+}
+
+// the run at (row, col), any part of which may lie beyond the matrix
+template <typename T, int COUNT>
+__device__ __forceinline__ void finish_at(const Epilogue &e, int row, int col, float (&s)[COUNT], const float (&bias)[COUNT]) {
+	const int left = e.n - col;
+	if (row >= e.m || left <= 0) return;
+	const bool whole = e.vec && left >= COUNT;
+	const size_t at = (size_t)row * e.ldo + col;
+	finish(
+	    e, s, bias, (uint64_t)row * e.n + col,
+	    [&](float (&v)[COUNT]) { e.out_f32 ? load_run((const float *)e.out + at, whole, left, v) : load_run((const T *)e.out + at, whole, left, v); },
+	    [&](float (&v)[COUNT]) { load_run((const T *)e.residual + (size_t)row * e.ldr + col, whole, left, v); },
+	    [&](const float (&v)[COUNT]) { store_run((T *)e.preact + (size_t)row * e.ldp + col, whole, left, v); },
+	    [&](const float (&v)[COUNT]) { e.out_f32 ? store_run((float *)e.out + at, whole, left, v) : store_run((T *)e.out + at, whole, left, v); });
+}
+
+// the runs at (row, col), (row + step, col), ...: all inside, all aligned. Addresses move by additions.
+template <typename T, int COUNT>
+struct Column {
+	char *out;
+	T *preact;
+	const T *residual;
+	long out_step, preact_step, residual_step;
+	uint64_t index, index_step;
+
+	__device__ __forceinline__ void init(const Epilogue &e, int row, int col, int step) {
+		const int size = e.out_f32 ? 4 : sizeof(T);
+		out = (char *)e.out + ((size_t)row * e.ldo + col) * size, out_step = step * e.ldo * size;
+		preact = (T *)e.preact + (size_t)row * e.ldp + col, preact_step = step * e.ldp;
+		residual = (const T *)e.residual + (size_t)row * e.ldr + col, residual_step = step * e.ldr;
+		index = (uint64_t)row * e.n + col, index_step = (uint64_t)step * e.n;
+	}
+
+	__device__ __forceinline__ void next(const Epilogue &e, float (&s)[COUNT], const float (&bias)[COUNT]) {
+		finish(
+		    e, s, bias, index,
+		    [&](float (&v)[COUNT]) { e.out_f32 ? load_run((const float *)out, true, COUNT, v) : load_run((const T *)out, true, COUNT, v); },
+		    [&](float (&v)[COUNT]) { load_run(residual, true, COUNT, v); }, [&](const float (&v)[COUNT]) { store_run(preact, true, COUNT, v); },
+		    [&](const float (&v)[COUNT]) { e.out_f32 ? store_run((float *)out, true, COUNT, v) : store_run((T *)out, true, COUNT, v); });
+		out += out_step, preact += preact_step, residual += residual_step, index += index_step;
+	}
+};
 
 struct Product {
 	const void *a, *b;
-	float *slabs;                    // partial sums [split][m][n] when splits > 1
+	float *slabs;                    // partial sums [split][m][slab_n] when splits > 1
+	int slab_n;                      // n up to whole runs
 	long lda, ldb;
 	int m, n, k;
 	int tiles_m, tiles_n, splits, ksteps_per_split;
@@ -126,15 +163,20 @@ struct Drain {
 
 	template <typename ACC>
 	static __device__ __forceinline__ void run(const Product &g, const ACC &acc, float *lds, int row0, int col0, int split, int lane) {
+		constexpr int RUNS = COLS / COUNT, STEP = 64 / RUNS;             // runs in a row, rows a wave handles at once
+		static_assert(64 % RUNS == 0, "runs of a row over lanes");
+		const int run = lane % RUNS, first = lane / RUNS, col = col0 + run * COUNT;
+		const bool inside = g.epi.vec && row0 + ROWS <= g.m && col0 + COLS <= g.n;
+		float bias[COUNT];
+		load_bias(g.epi, col, bias);
+		Column<T, COUNT> column;
+		column.init(g.epi, row0 + first, col, STEP);
 #pragma unroll
 		for (int i = 0; i < ROWS / 32; ++i) {
 			park(acc, i, lds, lane);
 			__builtin_amdgcn_wave_barrier();
-			constexpr int RUNS = COLS / COUNT, STEP = 64 / RUNS;         // runs in a row, rows a wave handles at once
-			static_assert(64 % RUNS == 0, "runs of a row over lanes");
-			const int run = lane % RUNS;
 #pragma unroll 2
-			for (int r = lane / RUNS; r < 32; r += STEP) {
+			for (int r = first; r < 32; r += STEP) {
 				float s[COUNT];
 #pragma unroll
 				for (int v = 0; v < COUNT; v += 4) {
@@ -142,12 +184,13 @@ struct Drain {
 #pragma unroll
 					for (int e = 0; e < 4; ++e) s[v + e] = x[e];
 				}
-				const int row = row0 + i * 32 + r, col = col0 + run * COUNT;
-				if (g.splits == 1) {
-					finish_run<T>(g.epi, row, col, s);
-				} else if (row < g.m && col < g.n) {
-					float *o = g.slabs + ((size_t)split * g.m + row) * g.n + col;
-					store_run(o, g.n % 4 == 0 && col + COUNT <= g.n, g.n - col, s);
+				const int row = row0 + i * 32 + r;
+				if (g.splits > 1) {
+					if (row < g.m && col < g.n) store_run(g.slabs + ((size_t)split * g.m + row) * g.slab_n + col, true, COUNT, s);
+				} else if (inside) {
+					column.next(g.epi, s, bias);
+				} else {
+					finish_at<T>(g.epi, row, col, s, bias);
 				}
 			}
 			__builtin_amdgcn_wave_barrier();
@@ -404,34 +447,52 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_kernel(Product g) {
 template <typename T>
 __global__ void __launch_bounds__(256) linear_join_kernel(Product g) {
 	constexpr int COUNT = 16 / sizeof(T);
-	const int runs = (g.n + COUNT - 1) / COUNT;
-	const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
+	const int runs = g.slab_n / COUNT;
+	const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x, each = (size_t)g.m * g.slab_n;
 	if (idx >= (size_t)runs * g.m) return;
-	const int row = (int)(idx / runs), col = (int)(idx % runs) * COUNT, left = g.n - col;
-	const bool whole = g.n % 4 == 0 && left >= COUNT;
-	float s[COUNT];
-	const float *p = g.slabs + (size_t)row * g.n + col;
-	load_run(p, whole, left, s);
+	const int row = (int)(idx / runs), col = (int)(idx % runs) * COUNT;
+	const float *p = g.slabs + (size_t)row * g.slab_n + col;
+	float s[COUNT], bias[COUNT];
+	load_bias(g.epi, col, bias);
+	load_run(p, true, COUNT, s);
+#pragma unroll 4
 	for (int i = 1; i < g.splits; ++i) {
 		float more[COUNT];
-		load_run(p + (size_t)i * g.m * g.n, whole, left, more);
+		load_run(p + i * each, true, COUNT, more);
 #pragma unroll
 		for (int e = 0; e < COUNT; ++e) s[e] += more[e];
 	}
-	finish_run<T>(g.epi, row, col, s);
+	finish_at<T>(g.epi, row, col, s, bias);
 }
 
 // ---- operands whose rows do not start on 16 bytes: a copy whose pitch is a multiple of 8 elements, the rest of each row zero -----------
+struct Aligned {
+	const void *src;
+	void *dst;                       // null: the operand stays where it is
+	int rows, cols, pitch;
+	long ld;
+};
+
 template <typename T>
-__global__ void __launch_bounds__(256) linear_align_kernel(const T *__restrict__ src, T *__restrict__ dst, int rows, int cols, long ld, int pitch) {
+__global__ void __launch_bounds__(256) linear_align_kernel(Aligned a, Aligned b, unsigned a_blocks) {
 	constexpr int COUNT = 16 / sizeof(T);
-	const int runs = pitch / COUNT;
-	const size_t idx = (size_t)blockIdx.x * 256 + threadIdx.x;
-	if (idx >= (size_t)runs * rows) return;
+	typedef T vec __attribute__((ext_vector_type(COUNT), aligned(sizeof(T))));
+	const bool second = blockIdx.x >= a_blocks;
+	const Aligned &o = second ? b : a;
+	const int runs = o.pitch / COUNT;
+	const size_t idx = (size_t)(blockIdx.x - (second ? a_blocks : 0)) * 256 + threadIdx.x;
+	if (idx >= (size_t)runs * o.rows) return;
 	const int row = (int)(idx / runs), col = (int)(idx % runs) * COUNT;
+	const T *p = (const T *)o.src + (size_t)row * o.ld + col;
 	float v[COUNT];
-	load_run(src + (size_t)row * ld + col, false, cols - col, v);
-	store_run(dst + (size_t)row * pitch + col, true, COUNT, v);
+	if (col + COUNT <= o.cols) {
+		const vec x = *reinterpret_cast<const vec *>(p);                  // (whole elements, no better alignment)
+#pragma unroll
+		for (int e = 0; e < COUNT; ++e) v[e] = (float)x[e];
+	} else {
+		load_run(p, false, o.cols - col, v);
+	}
+	store_run((T *)o.dst + (size_t)row * o.pitch + col, true, COUNT, v);
 }
 
 // ---- dz = dy * keep / (1 - p) * act'(z), and partial column sums -----------------------------------------------------------------------
@@ -445,10 +506,10 @@ struct Gate {
 	DropKey drop;
 };
 
-// block = 4 waves x (64 lanes x 8 columns), rows dealt out over the waves
+// block = 4 waves x (64 lanes x 16 bytes of columns), rows dealt out over the waves
 template <typename T>
 __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
-	constexpr int COUNT = 8;
+	constexpr int COUNT = 16 / sizeof(T);
 	__shared__ float part[4][64][COUNT + 1];
 	const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 	const int col = (blockIdx.x * 64 + lane) * COUNT, left = g.n - col;
@@ -553,20 +614,8 @@ Plan plan_product(int dtype, const Operands &o) {
 	p.copy_b = !aligned(o.b, o.ldb, o.wide_b, size);
 	p.a_bytes = p.copy_a ? rounded((size_t)(o.ta ? o.k : o.m) * padded(o.ta ? o.m : o.k) * size) : 0;
 	p.b_bytes = p.copy_b ? rounded((size_t)(o.tb ? o.n : o.k) * padded(o.tb ? o.k : o.n) * size) : 0;
-	p.slab_bytes = p.splits > 1 ? rounded((size_t)p.splits * o.m * o.n * sizeof(float)) : 0;
+	p.slab_bytes = p.splits > 1 ? rounded((size_t)p.splits * o.m * padded(o.n) * sizeof(float)) : 0;
 	return p;
-}
-
-template <typename T>
-int align_operand(const void *&src, long &ld, int rows, int cols, char *at, hipStream_t st) {
-	const int pitch = padded(cols), runs = pitch / (16 / (int)sizeof(T));
-	const size_t items = (size_t)rows * runs;
-	if (items > 0) {
-		linear_align_kernel<T><<<(unsigned)((items + 255) / 256), 256, 0, st>>>((const T *)src, (T *)at, rows, cols, ld, pitch);
-		PZ_LAUNCH_CHECK();
-	}
-	src = at, ld = pitch;
-	return PZ_OK;
 }
 
 template <typename T, bool TA, bool TB>
@@ -592,20 +641,24 @@ int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st
 	if (o.m == 0 || o.n == 0) return PZ_OK;
 	const Plan p = plan_product(dtype, o);
 	const int size = dtype == PZ_F16 ? 2 : 4;
-	if (p.copy_a) {
-		const int rows = o.ta ? o.k : o.m, cols = o.ta ? o.m : o.k;
-		if (int rc = dtype == PZ_F16 ? align_operand<f16>(o.a, o.lda, rows, cols, ws, st) : align_operand<float>(o.a, o.lda, rows, cols, ws, st)) return rc;
-	}
-	if (p.copy_b) {
-		const int rows = o.tb ? o.n : o.k, cols = o.tb ? o.k : o.n;
-		char *at = ws + p.a_bytes;
-		if (int rc = dtype == PZ_F16 ? align_operand<f16>(o.b, o.ldb, rows, cols, at, st) : align_operand<float>(o.b, o.ldb, rows, cols, at, st)) return rc;
+	if (p.copy_a || p.copy_b) {
+		Aligned a{o.a, nullptr, 0, 0, 0, o.lda}, b{o.b, nullptr, 0, 0, 0, o.ldb};
+		if (p.copy_a) a.dst = ws, a.rows = o.ta ? o.k : o.m, a.cols = o.ta ? o.m : o.k, a.pitch = padded(a.cols), o.a = ws, o.lda = a.pitch;
+		if (p.copy_b) b.dst = ws + p.a_bytes, b.rows = o.tb ? o.n : o.k, b.cols = o.tb ? o.k : o.n, b.pitch = padded(b.cols), o.b = b.dst, o.ldb = b.pitch;
+		auto blocks = [&](const Aligned &x) { return ((size_t)x.rows * (x.pitch * size / 16) + 255) / 256; };
+		const size_t total = blocks(a) + blocks(b);
+		PZ_REQUIRE(total < (1ull << 31), "linear: an unaligned operand of %d x %d is too large", o.m, o.k);
+		if (total > 0) {
+			if (dtype == PZ_F16) linear_align_kernel<f16><<<(unsigned)total, 256, 0, st>>>(a, b, (unsigned)blocks(a));
+			else linear_align_kernel<float><<<(unsigned)total, 256, 0, st>>>(a, b, (unsigned)blocks(a));
+			PZ_LAUNCH_CHECK();
+		}
 	}
 
 	Product g;
 	g.a = o.a, g.b = o.b, g.lda = o.lda, g.ldb = o.ldb;
 	g.slabs = (float *)(ws + p.a_bytes + p.b_bytes);
-	g.m = o.m, g.n = o.n, g.k = o.k;
+	g.m = o.m, g.n = o.n, g.k = o.k, g.slab_n = padded(o.n);
 	g.tiles_m = p.tiles_m, g.tiles_n = p.tiles_n, g.splits = p.splits, g.ksteps_per_split = p.ksteps_per_split;
 	g.a_bytes = extent_of(o.ta ? o.k : o.m, p.copy_a ? (int)o.lda : o.wide_a, o.lda, size);
 	g.b_bytes = extent_of(o.tb ? o.n : o.k, p.copy_b ? (int)o.ldb : o.wide_b, o.ldb, size);
@@ -617,7 +670,8 @@ int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st
 	else launch<float>(p, g, o.ta, o.tb, grid, st);
 	PZ_LAUNCH_CHECK();
 	if (p.splits > 1) {
-		const size_t items = (size_t)o.m * pz::ceil_div(o.n, 16 / size);
+		const size_t items = (size_t)o.m * (padded(o.n) * size / 16);
+		PZ_REQUIRE(items < (1ull << 38), "linear: %d rows are too many", o.m);
 		const unsigned blocks = (unsigned)((items + 255) / 256);
 		if (dtype == PZ_F16) linear_join_kernel<f16><<<blocks, 256, 0, st>>>(g);
 		else linear_join_kernel<float><<<blocks, 256, 0, st>>>(g);
@@ -668,9 +722,9 @@ BackPlan plan_backward(const pz_linear_desc *d, const void *dy, const void *x, c
 	const int size = d->dtype == PZ_F16 ? 2 : 4;
 	p.write_dz = (want_dx || want_dw) && (d->act != PZ_ACT_NONE || dropping || !aligned(dy, d->ldy, d->n, size));
 	p.dz_bytes = p.write_dz ? rounded((size_t)d->m * padded(d->n) * size) : 0;
-	const int strips = pz::ceil_div(d->n, 512);
+	const int strips = pz::ceil_div(d->n, 1024 / size);                  // (a workgroup takes 1 KiB of columns)
 	p.rows_per_block = 128;                                              // fewer rows a block where there are few blocks
-	while (p.rows_per_block > 8 && (long)strips * pz::ceil_div(d->m, p.rows_per_block) < 4 * pz::kNumCU) p.rows_per_block /= 2;
+	while (p.rows_per_block > 4 && (long)strips * pz::ceil_div(d->m, p.rows_per_block) < 4 * pz::kNumCU) p.rows_per_block /= 2;
 	while (pz::ceil_div(d->m, p.rows_per_block) > 65535) p.rows_per_block *= 2;
 	p.row_blocks = pz::ceil_div(d->m, p.rows_per_block);
 	p.sum_bytes = want_db ? rounded((size_t)p.row_blocks * d->n * sizeof(float)) : 0;
@@ -755,7 +809,7 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 		g.m = d->m, g.n = d->n, g.act = d->act, g.dropping = mask != nullptr, g.rows_per_block = p.rows_per_block;
 		g.vec = runs_ok(dy, d->ldy, size) && (d->act == PZ_ACT_NONE || runs_ok(preact, d->ldp, size));
 		g.drop = key_of(mask), g.inv_keep = 1.f / g.drop.keep;
-		const dim3 grid((unsigned)pz::ceil_div(d->n, 512), (unsigned)p.row_blocks);
+		const dim3 grid((unsigned)pz::ceil_div(d->n, 1024 / size), (unsigned)p.row_blocks);
 		if (d->dtype == PZ_F16) linear_gate_kernel<f16><<<grid, 256, 0, st>>>(g);
 		else linear_gate_kernel<float><<<grid, 256, 0, st>>>(g);
 		PZ_LAUNCH_CHECK();

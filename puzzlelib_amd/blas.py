@@ -18,11 +18,49 @@ from puzzlelib_amd.common import (
 )
 
 
+class LinearPlan:
+	"""A checked call of linear / linearBackward: its descriptor and the workspace it takes. `shared` descriptors are not written to."""
+	__slots__ = ("desc", "ref", "shape", "shared", "sizes")
+
+	def __init__(self, desc, shape, shared):
+		self.desc, self.ref, self.shape, self.shared, self.sizes = desc, byref(desc), shape, shared, {}
+
+	def private(self):
+		if not self.shared:
+			return self
+		desc = lib.LinearDesc()
+		ctypes.pointer(desc)[0] = self.desc
+		return LinearPlan(desc, self.shape, False)
+
+	def forwardBytes(self, x, w):
+		key = (x & 15, w & 15)
+		nbytes = self.sizes.get(key)
+		if nbytes is None:
+			size = c_size_t(0)
+			lib.pz_linear_fwd_workspace_bytes(self.ref, x, w, byref(size))
+			nbytes = size.value
+			if self.shared:
+				self.sizes[key] = nbytes
+		return nbytes
+
+	def backwardBytes(self, dy, x, w, *wants):
+		key = (dy & 15, x & 15, w & 15) + wants
+		nbytes = self.sizes.get(key)
+		if nbytes is None:
+			size = c_size_t(0)
+			lib.pz_linear_bwd_workspace_bytes(self.ref, dy, x, w, *map(int, wants), byref(size))
+			nbytes = size.value
+			if self.shared:
+				self.sizes[key] = nbytes
+		return nbytes
+
+
 class BlasContext:
 	"""gemm / dot / l1norm / l2norm — BlasContext of Cuda/Source/Libs/CuBlas.c:486-499 (RocBlas on HIP)."""
 
 	def __init__(self, backend):
 		self.backend = backend
+		self.linearPlans = {}
 
 
 	def enableTensorOps(self, _):
@@ -110,9 +148,18 @@ class BlasContext:
 		return out
 
 
-	@staticmethod
-	def linearDesc(what, data, W, transpW, act, dropout):
-		"""descriptor of data (..., k) times W (k, n), or (n, k) with transpW; (desc, rows' shape, dropout key or None)"""
+	# What a call of linear / linearBackward on dense operands of given shapes comes to is kept: the checked descriptor (never written to
+	# again) and the workspace size per alignment of the addresses. A small product takes less time on the device than its checks.
+	plansKept = 1024
+
+	def linearPlan(self, what, data, W, transpW, act, backward):
+		"""data (..., k) times W (k, n), or (n, k) with transpW -> LinearPlan (whose `ldr` is the pitch of the residual, or of the input
+		gradient)"""
+		dense = data.contiguous and W.contiguous
+		key = (data.shape, W.shape, data.dtype, W.dtype, transpW, act, backward)
+		plan = self.linearPlans.get(key) if dense else None
+		if plan is not None:
+			return plan
 		dtype = rowDtype(data, what)
 		if data.ndim < 2 or W.ndim != 2:
 			raise ValueError("%s: data of two axes or more and a matrix W expected, got %s and %s" % (what, data.shape, W.shape))
@@ -121,20 +168,52 @@ class BlasContext:
 		k, n = (W.shape[1], W.shape[0]) if transpW else W.shape
 		if data.shape[-1] != k or k == 0 or n == 0:
 			raise ValueError("%s: data %s does not fit W %s%s" % (what, data.shape, W.shape, " (transposed)" if transpW else ""))
-		if dropout is not None and not isinstance(dropout, DropoutMask):
-			raise ValueError("%s: dropout is a DropoutMask, got %r" % (what, dropout))
 		m = prod(data.shape[:-1])
 		if max(m, n, k) > 0x7fffffff:
 			raise ValueError("%s: %d rows are too many" % (what, m))
-		desc = lib.LinearDesc(dtype, FusedAct(act).value, int(transpW), m, n, k, rowPitch(data, what + ": data"), rowPitch(W, what + ": W"), n, n, n)
-		return desc, data.shape[:-1], None if dropout is None or dropout.p == 0.0 else byref(dropout.key)
+		plan = LinearPlan(lib.LinearDesc(
+			dtype, FusedAct(act).value, int(transpW), m, n, k, rowPitch(data, what + ": data"), rowPitch(W, what + ": W"), n, k if backward else n, n
+		), data.shape[:-1] + (n, ), dense)
+		if dense:
+			if len(self.linearPlans) >= self.plansKept:
+				self.linearPlans.clear()
+			self.linearPlans[key] = plan
+		return plan
 
 
 	@staticmethod
-	def linearOperand(what, ary, shape, dtype):
-		if tuple(ary.shape) != tuple(shape) or ary.dtype != dtype:
-			raise ValueError("%s is %s %s, expected %s %s" % (what, ary.shape, ary.dtype, tuple(shape), dtype))
-		return rowPitch(ary, what)
+	def linearOperand(what, ary, shape, dtype, plan, field, dense):
+		"""checks an operand of the given shape; a row pitch other than the dense one goes into the plan's descriptor (a private copy)"""
+		if ary.shape != shape or ary.dtype != dtype:
+			raise ValueError("%s is %s %s, expected %s %s" % (what, ary.shape, ary.dtype, shape, dtype))
+		if not ary.contiguous:
+			pitch = rowPitch(ary, what)
+			if pitch != dense:
+				plan = plan.private()
+				setattr(plan.desc, field, pitch)
+		return plan
+
+
+	@staticmethod
+	def linearMask(what, dropout):
+		if dropout is None:
+			return None
+		if not isinstance(dropout, DropoutMask):
+			raise ValueError("%s: dropout is a DropoutMask, got %r" % (what, dropout))
+		return None if dropout.p == 0.0 else byref(dropout.key)
+
+
+	@staticmethod
+	def workspace(nbytes, allocator):
+		"""(owner, address) of scratch memory; the owner goes back to the pool behind the launches that use it"""
+		if nbytes == 0:
+			return None, None
+		if GPUArray.debugFill:
+			ws = GPUArray.empty((nbytes, ), dtype=np.uint8, allocator=allocator)
+			return ws, ws.gpudata.ptr
+		allocator = GPUArray.defaultAllocator if allocator is None else allocator
+		ws = driver.Buffer.allocate(nbytes) if allocator is None else allocator.allocate(nbytes)
+		return ws, ws.ptr
 
 
 	def linear(self, data, W, bias=None, act=FusedAct.none, residual=None, dropout=None, preact=None, transpW=False, out=None,
@@ -144,34 +223,33 @@ class BlasContext:
 		Add.py:15-22). data is (..., k) in rows of one pitch, W (k, n), or (n, k) with transpW. `preact`: an array for
 		data W + bias (linearBackward needs it behind an activation), or True to have one made; the call then returns (out, preact).
 		`out` may be `residual` (in place)."""
-		what = "linear"
-		desc, rows, key = self.linearDesc(what, data, W, transpW, act, dropout)
-		shape = rows + (desc.n, )
-		requireVector(bias, desc.n, "linear: bias")
+		plan = self.linearPlan("linear", data, W, transpW, act, False)
+		key = self.linearMask("linear", dropout)
+		n, shape, dtype = plan.desc.n, plan.shape, data.dtype
+		requireVector(bias, n, "linear: bias")
 		if residual is not None:
-			desc.ldr = self.linearOperand("linear: residual", residual, shape, data.dtype)
+			plan = self.linearOperand("linear: residual", residual, shape, dtype, plan, "ldr", n)
 		if out is None:
-			out = GPUArray.empty(shape, dtype=data.dtype, allocator=allocator)
+			out = GPUArray.empty(shape, dtype=dtype, allocator=allocator)
 		else:
-			desc.ldy = self.linearOperand("linear: out", out, shape, data.dtype)
+			plan = self.linearOperand("linear: out", out, shape, dtype, plan, "ldy", n)
 			inplace = residual is not None and lazy.sameBuffer(out, residual) and out.strides == residual.strides
 			requireDisjoint("linear: out", out, data, W, bias, None if inplace else residual)
 		if preact is True:
-			preact = GPUArray.empty(shape, dtype=data.dtype, allocator=allocator)
+			preact = GPUArray.empty(shape, dtype=dtype, allocator=allocator)
 		elif preact is not None:
-			desc.ldp = self.linearOperand("linear: preact", preact, shape, data.dtype)
+			plan = self.linearOperand("linear: preact", preact, shape, dtype, plan, "ldp", n)
 			requireDisjoint("linear: preact", preact, data, W, bias, residual, out)
 
+		desc = plan.desc
 		if desc.m > 0:
 			xptr, wptr, bptr, rptr = data.rptr, W.rptr, rptrOf(bias), rptrOf(residual)
-			size = c_size_t(0)
-			lib.pz_linear_fwd_workspace_bytes(byref(desc), xptr, wptr, byref(size))
-			ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+			nbytes = plan.forwardBytes(xptr, wptr)
+			ws, wsptr = self.workspace(nbytes, allocator)
 			if desc.dtype == lib.F16:
 				lazy.matrixBegin()
 			lib.pz_linear_fwd(
-				byref(desc), xptr, wptr, bptr, rptr, key, out.optr, None if preact is None else preact.optr,
-				None if ws is None else ws.optr, size.value, None
+				plan.ref, xptr, wptr, bptr, rptr, key, out.optr, None if preact is None else preact.optr, wsptr, nbytes, None
 			)
 		return out if preact is None else (out, preact)
 
@@ -182,25 +260,22 @@ class BlasContext:
 		residual's gradient is grad itself. Passed-in wgrad (float32, or the operands' type) and bgrad (float32) follow
 		Modules/Linear.py:44-54: dst = momentum * dst + scale * d; momentum 0 overwrites. Behind an activation `preact` is what the
 		forward pass left, with dropout the same mask is passed again."""
-		what = "linearBackward"
-		desc, rows, key = self.linearDesc(what, data, W, transpW, act, dropout)
-		shape = rows + (desc.n, )
-		desc.ldy = self.linearOperand("linearBackward: grad", grad, shape, data.dtype)
-		if desc.act != lib.ACT_NONE:
+		plan = self.linearPlan("linearBackward", data, W, transpW, act, True)
+		key = self.linearMask("linearBackward", dropout)
+		n, k, shape, dtype = plan.desc.n, plan.desc.k, plan.shape, data.dtype
+		plan = self.linearOperand("linearBackward: grad", grad, shape, dtype, plan, "ldy", n)
+		if plan.desc.act != lib.ACT_NONE:
 			if preact is None:
 				raise ValueError("linearBackward: the gradient of %s needs the pre-activation" % FusedAct(act).name)
-			desc.ldp = self.linearOperand("linearBackward: preact", preact, shape, data.dtype)
+			plan = self.linearOperand("linearBackward: preact", preact, shape, dtype, plan, "ldp", n)
 		else:
 			preact = None
-		withbias = wantParams and withbias
-		if wantInput:
-			desc.ldr = desc.k
-			if out is None:
-				out = GPUArray.empty(rows + (desc.k, ), dtype=data.dtype, allocator=allocator)
-			else:
-				desc.ldr = self.linearOperand("linearBackward: out", out, rows + (desc.k, ), data.dtype)
-		else:
+		if not wantInput:
 			out = None
+		elif out is None:
+			out = GPUArray.empty(data.shape, dtype=dtype, allocator=allocator)
+		else:
+			plan = self.linearOperand("linearBackward: out", out, data.shape, dtype, plan, "ldr", k)
 		if not wantParams:
 			wgrad = bgrad = None
 		else:
@@ -215,9 +290,9 @@ class BlasContext:
 			if not withbias:
 				bgrad = None
 			elif bgrad is None:
-				bgrad = GPUArray.empty((desc.n, ), dtype=np.float32, allocator=allocator)
+				bgrad = GPUArray.empty((n, ), dtype=np.float32, allocator=allocator)
 			else:
-				requireVector(bgrad, desc.n, "linearBackward: bgrad")
+				requireVector(bgrad, n, "linearBackward: bgrad")
 		operands = (grad, data, W, preact)
 		requireDisjoint("linearBackward: out", out, *operands)
 		requireDisjoint("linearBackward: wgrad", wgrad, out, *operands)
@@ -226,22 +301,17 @@ class BlasContext:
 			return None, None, None
 
 		gptr, xptr, wptr, pptr = grad.rptr, data.rptr, W.rptr, rptrOf(preact)
-		size = c_size_t(0)
-		lib.pz_linear_bwd_workspace_bytes(
-			byref(desc), gptr, xptr, wptr, int(key is not None), int(out is not None), int(wgrad is not None), int(bgrad is not None),
-			byref(size)
-		)
-		ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+		nbytes = plan.backwardBytes(gptr, xptr, wptr, key is not None, out is not None, wgrad is not None, bgrad is not None)
+		ws, wsptr = self.workspace(nbytes, allocator)
 
 		def target(ary):
 			return None if ary is None else ary.wptr if momentum != 0.0 else ary.optr
 
-		if desc.dtype == lib.F16:
+		if plan.desc.dtype == lib.F16:
 			lazy.matrixBegin()
 		lib.pz_linear_bwd(
-			byref(desc), gptr, xptr, wptr, pptr, key, None if out is None else out.optr, target(wgrad),
-			lib.F32 if wgrad is None or wgrad.dtype == np.float32 else lib.F16, target(bgrad), scale, momentum,
-			None if ws is None else ws.optr, size.value, None
+			plan.ref, gptr, xptr, wptr, pptr, key, None if out is None else out.optr, target(wgrad),
+			lib.F32 if wgrad is None or wgrad.dtype == np.float32 else lib.F16, target(bgrad), scale, momentum, wsptr, nbytes, None
 		)
 		return out, wgrad, bgrad
 

@@ -622,8 +622,8 @@ template <typename T, bool TA, bool TB>
 void launch(const Plan &p, const Product &g, dim3 grid, hipStream_t st) {
 	if (p.bm == 256) linear_kernel<T, 256, 256, 2, 4, TA, TB><<<grid, 512, 0, st>>>(g);
 	else if (p.bm == 128 && p.bn == 128) linear_kernel<T, 128, 128, 2, 2, TA, TB><<<grid, 256, 0, st>>>(g);
-	else if (p.bm == 128) linear_kernel<T, 128, 64, 2, 1, TA, TB><<<grid, 128, 0, st>>>(g);
-	else if (p.bn == 128) linear_kernel<T, 64, 128, 1, 2, TA, TB><<<grid, 128, 0, st>>>(g);
+	else if (p.bm == 128) linear_kernel<T, 128, 64, 2, 2, TA, TB><<<grid, 256, 0, st>>>(g);
+	else if (p.bn == 128) linear_kernel<T, 64, 128, 1, 4, TA, TB><<<grid, 256, 0, st>>>(g);
 	else linear_kernel<T, 64, 64, 1, 1, TA, TB><<<grid, 64, 0, st>>>(g);
 }
 

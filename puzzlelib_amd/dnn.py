@@ -47,6 +47,7 @@ class DnnContext:
 		self.backend = backend
 		self.statsWanted = weakref.WeakKeyDictionary()      # allocation of a filter -> byte offsets of filters a BatchNorm follows
 		self.geometry = {}
+		self.groupNormPlans = {}
 		self.sideStream = None
 		self.sideLaunches = 0
 		self.earlyReady = None       # (event, gradient allocation, data allocation, their versions): see convNdBackwardData
@@ -914,21 +915,31 @@ class DnnContext:
 		return out, savemean, saveinvvar
 
 
-	@staticmethod
-	def groupNormDesc(what, data, groups, scale, bias, epsilon, act):
-		"""data (batch, ..., channels): channels last"""
-		dtype = rowDtype(data, what)
-		if data.ndim < 2 or not data.contiguous:
-			raise ValueError("%s: contiguous data (batch, ..., channels) expected, got shape %s" % (what, data.shape))
-		n, c = data.shape[0], data.shape[-1]
-		if groups <= 0 or c == 0 or c % groups != 0:
-			raise ValueError("%s: %d channels do not form %d groups" % (what, c, groups))
-		requireVector(scale, c, what + ": scale")
-		requireVector(bias, c, what + ": bias")
-		pixels = prod(data.shape[1:-1])
-		if max(n, c, pixels) > 0x7fffffff:
-			raise ValueError("%s: shape %s is too large" % (what, data.shape))
-		return lib.GroupNormDesc(dtype, FusedAct(act).value, n, pixels, c, int(groups), float(epsilon))
+	def groupNormPlan(self, what, data, groups, scale, bias, epsilon, act, backward):
+		"""data (batch, ..., channels), channels last -> (descriptor, its reference, workspace bytes), kept per shape"""
+		key = (data.shape, data.dtype, groups, epsilon, act, backward)
+		plan = self.groupNormPlans.get(key)
+		if plan is None:
+			dtype = rowDtype(data, what)
+			if data.ndim < 2:
+				raise ValueError("%s: data (batch, ..., channels) expected, got shape %s" % (what, data.shape))
+			n, c = data.shape[0], data.shape[-1]
+			if groups <= 0 or c == 0 or c % groups != 0:
+				raise ValueError("%s: %d channels do not form %d groups" % (what, c, groups))
+			pixels = prod(data.shape[1:-1])
+			if max(n, c, pixels) > 0x7fffffff:
+				raise ValueError("%s: shape %s is too large" % (what, data.shape))
+			desc = lib.GroupNormDesc(dtype, FusedAct(act).value, n, pixels, c, int(groups), float(epsilon))
+			size = c_size_t(0)
+			lib.pz_groupnorm_workspace_bytes(byref(desc), int(backward), byref(size))
+			if len(self.groupNormPlans) >= 1024:
+				self.groupNormPlans.clear()
+			plan = self.groupNormPlans[key] = (desc, byref(desc), size.value)
+		if not data.contiguous:
+			raise ValueError("%s: contiguous data (batch, ..., channels) expected" % what)
+		requireVector(scale, plan[0].c, what + ": scale")
+		requireVector(bias, plan[0].c, what + ": bias")
+		return plan
 
 
 	@staticmethod
@@ -942,7 +953,7 @@ class DnnContext:
 		"""Group normalisation of channels-last data (batch, ..., channels) with an activation behind it (float32 or float16 data;
 		scale and bias, float32 or None, per channel): out, or (out, savemean, saveinvvar) unless `test` — the shape of batchNormNd's
 		answer, with statistics per (sample, group). `out` may be `data`."""
-		desc = self.groupNormDesc("groupNormNd", data, groups, scale, bias, epsilon, act)
+		desc, ref, nbytes = self.groupNormPlan("groupNormNd", data, groups, scale, bias, epsilon, act, False)
 		if out is None:
 			out = GPUArray.empty(data.shape, dtype=data.dtype, allocator=allocator)
 		else:
@@ -967,14 +978,12 @@ class DnnContext:
 				if ary.size > 0:
 					ary.fill(0)                                     # statistics of no values: defined, never read
 		else:
-			size = c_size_t(0)
-			lib.pz_groupnorm_workspace_bytes(byref(desc), 0, byref(size))
-			ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+			ws, wsptr = self.backend.blas.workspace(nbytes, allocator)
 			xptr, sptr, bptr = data.rptr, rptrOf(scale), rptrOf(bias)
 			lib.pz_groupnorm_fwd(
-				byref(desc), xptr, sptr, bptr, out.wptr if lazy.sameBuffer(out, data) else out.optr,
+				ref, xptr, sptr, bptr, out.wptr if lazy.sameBuffer(out, data) else out.optr,
 				None if savemean is None else savemean.optr, None if saveinvvar is None else saveinvvar.optr,
-				None if ws is None else ws.optr, size.value, None
+				wsptr, nbytes, None
 			)
 		return out if test else (out, savemean, saveinvvar)
 
@@ -983,7 +992,7 @@ class DnnContext:
 							bgrad=None, affine=True, allocator=None):
 		"""(ingrad, scalegrad, bgrad) of groupNormNd from its input and saved statistics (batchNormNdBackward's answer); ingrad alone
 		without `affine`. `out` may be `grad` or `data`."""
-		desc = self.groupNormDesc("groupNormNdBackward", data, groups, scale, bias, 0.0, act)
+		desc, ref, nbytes = self.groupNormPlan("groupNormNdBackward", data, groups, scale, bias, 0.0, act, True)
 		if grad.shape != data.shape or grad.dtype != data.dtype or not grad.contiguous:
 			raise ValueError("groupNormNdBackward: grad is %s %s, expected contiguous %s %s" % (grad.shape, grad.dtype, data.shape, data.dtype))
 		self.groupNormStats("groupNormNdBackward: savemean", savemean, desc)
@@ -1009,15 +1018,12 @@ class DnnContext:
 		else:
 			scalegrad = bgrad = None
 
-		size = c_size_t(0)
-		lib.pz_groupnorm_workspace_bytes(byref(desc), 1, byref(size))
-		ws = GPUArray.empty((size.value, ), dtype=np.uint8, allocator=allocator) if size.value > 0 else None
+		ws, wsptr = self.backend.blas.workspace(nbytes, allocator)
 		gptr, xptr, sptr, bptr, mptr, vptr = grad.rptr, data.rptr, rptrOf(scale), rptrOf(bias), savemean.rptr, saveinvvar.rptr
 		inplace = lazy.sameBuffer(out, grad) or lazy.sameBuffer(out, data)
 		lib.pz_groupnorm_bwd(
-			byref(desc), gptr, xptr, sptr, bptr, mptr, vptr, out.wptr if inplace else out.optr,
-			None if scalegrad is None else scalegrad.optr, None if bgrad is None else bgrad.optr, None if ws is None else ws.optr,
-			size.value, None
+			ref, gptr, xptr, sptr, bptr, mptr, vptr, out.wptr if inplace else out.optr,
+			None if scalegrad is None else scalegrad.optr, None if bgrad is None else bgrad.optr, wsptr, nbytes, None
 		)
 		return (out, scalegrad, bgrad) if affine else out
 

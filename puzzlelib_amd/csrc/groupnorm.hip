@@ -24,13 +24,15 @@ __device__ __forceinline__ float or_else(const float *p, int i, float v) { retur
 // A workgroup holds `rows` rows of `width` consecutive values, `pitch` apart, as 16-byte vectors in registers: thread (tx, ty) the
 // vectors at tx * V of the rows ty, ty + TY, ... — its channels never change, so scale, bias and statistics are fetched once. Either
 //  - a row is a pixel's slab of channels (whole groups, at least a cache line where the shape gives one), pitch c; or
-//  - the pixels lie back to back: a row is lcm(c, V) values (`reps` pixels), whatever c is; what lies beyond `limit` does not exist.
+//  - the pixels lie back to back: a row is lcm(c, V) values (`reps` pixels), whatever c is; the last row may end early.
 struct Slab {
-	int width, tx, reps, slabs, uniform;         // uniform: every vector lies inside one group
-	long pitch;
-	long rows, limit;                            // of one chunk (the last may be shorter); limit: values of one sample
+	int width, tx, ty, reps, slabs, uniform;     // uniform: every vector lies inside one group
+	int pitch;
+	int rows, last_rows;                         // of a chunk, of the last one
+	int last_values;                             // values of the last chunk (the last row may end early)
+	float count, last_count;                     // values of a group in a chunk, in the last one
 	int chunks;
-	int paired;                                  // workgroups b and b + 8 (one XCD, hence one L2) take the two halves of a cache line
+	int sharing;                                 // slabs that share cache lines: workgroups b, b + 8, ... (one XCD, hence one L2) take them
 	int wd, period;                              // values of a group and of all channels in a row's cells (below)
 };
 
@@ -41,7 +43,7 @@ struct Vec {
 };
 
 template <typename T>
-__device__ __forceinline__ typename Vec<T>::raw load_vec(const T *p, long left) {
+__device__ __forceinline__ typename Vec<T>::raw load_vec(const T *p, int left) {
 	constexpr int V = Vec<T>::V;
 	typename Vec<T>::raw v;
 	if (left >= V) return *reinterpret_cast<const typename Vec<T>::raw *>(p);
@@ -51,7 +53,7 @@ __device__ __forceinline__ typename Vec<T>::raw load_vec(const T *p, long left) 
 }
 
 template <typename T>
-__device__ __forceinline__ void store_vec(T *p, long left, const float (&v)[Vec<T>::V]) {
+__device__ __forceinline__ void store_vec(T *p, int left, const float (&v)[Vec<T>::V]) {
 	constexpr int V = Vec<T>::V;
 	if (left >= V) {
 		typename Vec<T>::raw x;
@@ -65,34 +67,82 @@ __device__ __forceinline__ void store_vec(T *p, long left, const float (&v)[Vec<
 	}
 }
 
-// The vectors of a thread: rows ty, ty + TY, ...: `mine` of them, the last one with `last` values (V unless the data ends inside it)
-__device__ __forceinline__ void share(const Slab &s, bool active, int ty, int TY, int col, int v, long rows, long all, int most, int &mine, int &last) {
-	mine = active && ty < rows ? (int)min((long)most, (rows - ty + TY - 1) / TY) : 0;
-	last = v;
-	if (mine > 0 && s.slabs == 1) {
-		const long left = all - (ty + (long)(mine - 1) * TY) * s.pitch - col;
+// The vectors of a thread: rows ty, ty + TY, ...: `mine` of them, the last one with `last` values (V unless the data ends inside it).
+// All arithmetic on the shape is 32-bit, its divisions the host's: 64-bit ones (150 instructions each) took most of a small call's time.
+template <int V>
+__device__ __forceinline__ void share(const Slab &s, int chunk, int tx, int ty, int most, int &mine, int &last) {
+	const bool ends = chunk == s.chunks - 1;
+	const int rows = ends ? s.last_rows : s.rows;
+	mine = ty < min(s.ty, rows) ? min(most, (rows - ty + s.ty - 1) / s.ty) : 0;
+	last = V;
+	if (ends && mine > 0 && s.slabs == 1) {
+		const int left = s.last_values - (ty + (mine - 1) * s.ty) * s.pitch - tx * V;
 		if (left <= 0) mine -= 1;                    // (only the last row ends early: the one before it is whole)
-		else if (left < v) last = (int)left;
+		else if (left < V) last = left;
 	}
+}
+
+// the workgroup's slab, chunk and sample
+__device__ __forceinline__ void place(const Slab &s, int &slab, int &chunk, long &sample) {
+	const unsigned item = (blockIdx.x / (8 * s.sharing) * 8 + blockIdx.x % 8) * s.sharing + blockIdx.x / 8 % s.sharing, rest = item / s.slabs;
+	slab = item - rest * s.slabs;
+	const unsigned at = rest / s.chunks;
+	chunk = rest - at * s.chunks, sample = at;
 }
 
 // Sums of cells in LDS: red[row * across + cell], `rows` rows; output o takes the cells rep * period + o * wd ... + wd - 1, rep < reps, of
 // every row. Each output is added by up to 64 lanes in a fixed order; out[o] = sum * factor. All threads call it; the caller has synchronised.
 template <int NT>
 __device__ void sum_cells(const float *red, int across, int rows, int reps, int period, int wd, int outputs, float factor, float *out) {
-	int lanes = 64;
-	while (lanes > 1 && lanes * outputs > NT) lanes >>= 1;
-	const int items = rows * reps * wd, sub = threadIdx.x % lanes;
-	for (int o0 = 0; o0 < outputs; o0 += NT / lanes) {
-		const int o = o0 + threadIdx.x / lanes;
+	int shift = 6;
+	while (shift > 0 && (outputs << shift) > NT) --shift;
+	const int lanes = 1 << shift, sub = threadIdx.x & (lanes - 1);
+	for (int o0 = 0; o0 < outputs; o0 += NT >> shift) {
+		const int o = o0 + (threadIdx.x >> shift);
 		float s = 0.f;
-		if (o < outputs)
-			for (int t = sub; t < items; t += lanes) {
-				const int i = t % wd, rest = t / wd;
-				s += red[(rest / reps) * across + (rest % reps) * period + o * wd + i];
+		if (o < outputs) {
+			const float *p = red + o * wd;
+			if (rows > 1) {
+				for (int r = sub; r < rows; r += lanes)
+					for (int rep = 0; rep < reps; ++rep)
+						for (int i = 0; i < wd; ++i) s += p[r * across + rep * period + i];
+			} else {
+				for (int rep = 0; rep < reps; ++rep)
+					for (int i = sub; i < wd; i += lanes) s += p[rep * period + i];
 			}
+		}
 		for (int l = lanes >> 1; l > 0; l >>= 1) s += __shfl_xor(s, l, 64);
 		if (o < outputs && sub == 0) out[o] = s * factor;
+	}
+}
+
+// scale and bias (1 and 0 where there are none) of V channels from `first` on (UNI), or of the channels ch(e)
+template <int V>
+__device__ __forceinline__ void load_floats(const float *p, int first, float none, float (&v)[V]) {
+	typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+	for (int q = 0; q < V; q += 4) {
+		const vec x = p ? *reinterpret_cast<const vec *>(p + first + q) : (vec){none, none, none, none};
+#pragma unroll
+		for (int e = 0; e < 4; ++e) v[q + e] = x[e];
+	}
+}
+
+// channel and group (inside the slab) of the V values of a vector, f(e, channel, group); UNI: one group, no pixel border inside
+template <int V, bool UNI, typename F>
+__device__ __forceinline__ void each_channel(int first, int c, int width, F f) {
+	if (UNI) {
+		const int group = first / width;
+#pragma unroll
+		for (int e = 0; e < V; ++e) f(e, first + e, group);
+	} else {
+		int ch = first % c, group = ch / width, at = ch - group * width;
+#pragma unroll
+		for (int e = 0; e < V; ++e) {
+			f(e, ch, group);
+			if (++at == width) at = 0, ++group;
+			if (++ch == c) ch = 0, group = 0;
+		}
 	}
 }
 
@@ -105,27 +155,22 @@ __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *p
 	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
 	__shared__ float red[NT * CELLS];
 	__shared__ float smean[UNI ? NT : kMaxWidth], sinv[UNI ? NT : kMaxWidth];      // (vectors inside one group: no more groups than vectors in a row)
-	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = NT / s.tx;
-	const unsigned item = s.paired ? (blockIdx.x / 16 * 8 + blockIdx.x % 8) * 2 + blockIdx.x / 8 % 2 : blockIdx.x;
-	const int slab = item % s.slabs;
-	const long rest = item / s.slabs, sample = rest / s.chunks;
-	const int chunk = (int)(rest % s.chunks);
-	const int c0 = slab * s.width;                                              // (one slab: 0)
+	const int ty = threadIdx.x / s.tx, tx = threadIdx.x - ty * s.tx, TY = s.ty;
+	int slab, chunk;
+	long sample;
+	place(s, slab, chunk, sample);
+	const int c0 = slab * s.width * (s.slabs > 1);
 	const int groups = s.slabs > 1 ? s.width / g.width : g.groups, group0 = c0 / g.width;
-	const size_t start = (size_t)sample * g.pixels * g.c + c0 + (size_t)chunk * s.rows * s.pitch;
+	const size_t start = ((size_t)sample * g.pixels) * g.c + c0 + (size_t)chunk * s.rows * s.pitch;
 	const T *x = (const T *)g.x + start;
-	// one slab: values of the sample from this chunk on; several: every row is whole and there is one chunk
-	const long all = s.slabs > 1 ? (long)1 << 62 : s.limit - (long)chunk * s.rows * s.pitch;
-	const long rows = min(s.rows, s.slabs > 1 ? s.rows : (all + s.pitch - 1) / s.pitch);
-	const long count = s.slabs > 1 ? rows * g.width : min(all, s.rows * s.pitch) / g.c * g.width;        // values of a group here
-	const bool active = ty < TY;
+	const float count = chunk == s.chunks - 1 ? s.last_count : s.count;
 
 	typename Vec<T>::raw v[NV];
 	int mine, last;
-	share(s, active, ty, TY, tx * V, V, rows, all, NV, mine, last);
+	share<V>(s, chunk, tx, ty, NV, mine, last);
 #pragma unroll
 	for (int k = 0; k < NV; ++k)
-		if (k < mine) v[k] = load_vec(x + (ty + (long)k * TY) * s.pitch + tx * V, k + 1 < mine ? V : last);
+		if (k < mine) v[k] = load_vec(x + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last);
 
 	float acc[CELLS];
 	auto cells = [&](auto value) {                                              // red <- per-thread sums of value(x, cell)
@@ -142,7 +187,7 @@ __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *p
 					if (e < last) acc[UNI ? 0 : e] += value((float)v[k][e], e);
 			}
 		}
-		if (active) {
+		if (ty < TY) {
 #pragma unroll
 			for (int e = 0; e < CELLS; ++e) red[(ty * s.tx + tx) * CELLS + e] = acc[e];
 		}
@@ -150,12 +195,11 @@ __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *p
 	};
 
 	cells([](float f, int) { return f; });
-	sum_cells<NT>(red, s.tx * CELLS, TY, s.reps, s.period, s.wd, groups, 1.f / (float)count, smean);
+	sum_cells<NT>(red, s.tx * CELLS, TY, s.reps, s.period, s.wd, groups, 1.f / count, smean);
 	__syncthreads();
 
 	float mean[CELLS];
-#pragma unroll
-	for (int e = 0; e < CELLS; ++e) mean[e] = smean[(tx * V + e) % g.c / g.width];
+	each_channel<CELLS, UNI>(tx * V, g.c, g.width, [&](int e, int, int group) { mean[e] = smean[group]; });
 	cells([&](float f, int e) {
 		const float d = f - mean[UNI ? 0 : e];
 		return d * d;
@@ -169,21 +213,20 @@ __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *p
 		return;
 	}
 	for (int o = threadIdx.x; o < groups; o += NT) {
-		const float inv = 1.f / sqrtf(sinv[o] / (float)count + g.epsilon);
+		const float inv = 1.f / sqrtf(sinv[o] / count + g.epsilon);
 		sinv[o] = inv;
 		if (g.mean) g.mean[(size_t)sample * g.groups + group0 + o] = smean[o];
 		if (g.invvar) g.invvar[(size_t)sample * g.groups + group0 + o] = inv;
 	}
 	__syncthreads();
-	if (!active) return;
+	if (mine == 0) return;
 
 	float scale[V], bias[V];
-#pragma unroll
-	for (int e = 0; e < V; ++e) {
-		const int ch = (tx * V + e) % g.c;                                        // channel inside the slab
-		scale[e] = or_else(g.scale, c0 + ch, 1.f) * sinv[ch / g.width];
-		bias[e] = or_else(g.bias, c0 + ch, 0.f);
-	}
+	if (UNI) load_floats(g.scale, c0 + tx * V, 1.f, scale), load_floats(g.bias, c0 + tx * V, 0.f, bias);
+	each_channel<V, UNI>(tx * V, g.c, g.width, [&](int e, int ch, int group) {
+		if (!UNI) scale[e] = or_else(g.scale, c0 + ch, 1.f), bias[e] = or_else(g.bias, c0 + ch, 0.f);
+		scale[e] *= sinv[group];
+	});
 	T *y = (T *)g.out + start;
 #pragma unroll
 	for (int k = 0; k < NV; ++k) {
@@ -191,7 +234,7 @@ __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *p
 		float o[V];
 #pragma unroll
 		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], g.act);
-		store_vec(y + (ty + (long)k * TY) * s.pitch + tx * V, k + 1 < mine ? V : last, o);
+		store_vec(y + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last, o);
 	}
 }
 
@@ -200,49 +243,56 @@ __global__ void __launch_bounds__(256) norm_join_kernel(Norm g, Slab s, const fl
 	const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
 	if (at >= (long)g.n * g.groups) return;
 	const int lane = threadIdx.x & 63;
-	const long sample = at / g.groups, group = at % g.groups, each = s.rows * s.pitch / g.c * g.width, total = (long)g.pixels * g.width;
+	const unsigned sample = (unsigned)at / g.groups, group = (unsigned)at - sample * g.groups;
+	const double total = (double)g.pixels * g.width;
+	auto each = [&](int k) { return (double)(k == s.chunks - 1 ? s.last_count : s.count); };
 	auto sum = [](double v) {
 		for (int l = 32; l > 0; l >>= 1) v += __shfl_xor(v, l, 64);
 		return v;
 	};
 	double m = 0.0, q = 0.0;
-	for (int k = lane; k < s.chunks; k += 64) m += (double)min(each, total - k * each) * part[((size_t)sample * s.chunks + k) * g.groups + group].x;
-	m = sum(m) / (double)total;
+	for (int k = lane; k < s.chunks; k += 64) m += each(k) * part[((size_t)sample * s.chunks + k) * g.groups + group].x;
+	m = sum(m) / total;
 	for (int k = lane; k < s.chunks; k += 64) {
 		const float2 p = part[((size_t)sample * s.chunks + k) * g.groups + group];
 		const double d = p.x - m;
-		q += p.y + (double)min(each, total - k * each) * d * d;
+		q += p.y + each(k) * d * d;
 	}
-	q = sum(q) / (double)total;
+	q = sum(q) / total;
 	if (lane == 0) mean[at] = (float)m, invvar[at] = (float)(1.0 / sqrt(q + (double)g.epsilon));
 }
 
 // y from x and the statistics, a chunk of rows back to back
-template <typename T, int NV>
+template <typename T, int NV, bool UNI>
 __global__ void __launch_bounds__(256) norm_apply_kernel(Norm g, Slab s, const float *means, const float *invvars) {
-	constexpr int V = Vec<T>::V;
-	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = 256 / s.tx;
-	if (ty >= TY) return;
-	const long sample = blockIdx.x / s.chunks, row0 = (long)(blockIdx.x % s.chunks) * s.rows;
-	const size_t start = (size_t)sample * g.pixels * g.c;
+	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
+	const int ty = threadIdx.x / s.tx, tx = threadIdx.x - ty * s.tx;
+	int slab, chunk, mine, last;
+	long sample;
+	place(s, slab, chunk, sample);
+	share<V>(s, chunk, tx, ty, NV, mine, last);
+	const size_t start = (size_t)sample * g.pixels * g.c + (size_t)chunk * s.rows * s.pitch + (size_t)ty * s.pitch + tx * V;
 	const T *x = (const T *)g.x + start;
 	T *y = (T *)g.out + start;
-	float mean[V], scale[V], bias[V];
+	typename Vec<T>::raw v[NV];
 #pragma unroll
-	for (int e = 0; e < V; ++e) {
-		const int ch = (tx * V + e) % g.c;
-		const size_t at = sample * g.groups + ch / g.width;
-		mean[e] = means[at], scale[e] = or_else(g.scale, ch, 1.f) * invvars[at], bias[e] = or_else(g.bias, ch, 0.f);
-	}
+	for (int k = 0; k < NV; ++k)
+		if (k < mine) v[k] = load_vec(x + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last);
+	float mean[CELLS], scale[V], bias[V], inv = 0.f;
+	if (UNI) load_floats(g.scale, tx * V, 1.f, scale), load_floats(g.bias, tx * V, 0.f, bias);
+	each_channel<V, UNI>(tx * V, g.c, g.width, [&](int e, int ch, int group) {
+		const size_t at = sample * g.groups + group;
+		if (!UNI || e == 0) mean[UNI ? 0 : e] = means[at], inv = invvars[at];
+		if (!UNI) scale[e] = or_else(g.scale, ch, 1.f), bias[e] = or_else(g.bias, ch, 0.f);
+		scale[e] *= inv;
+	});
 #pragma unroll
 	for (int k = 0; k < NV; ++k) {
-		const long r = ty + (long)k * TY, at = (row0 + r) * s.pitch + tx * V, left = r < s.rows ? s.limit - at : 0;
-		if (left <= 0) continue;
-		const typename Vec<T>::raw v = load_vec(x + at, left);
+		if (k >= mine) continue;
 		float o[V];
 #pragma unroll
-		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[e] - mean[e]) * scale[e] + bias[e], g.act);
-		store_vec(y + at, left, o);
+		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], g.act);
+		store_vec(y + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last, o);
 	}
 }
 
@@ -255,37 +305,32 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 	__shared__ float red[2][NT * V];
 	__shared__ float chan[2][kMaxWidth];
 	__shared__ float sa[UNI ? NT : kMaxWidth], sb[UNI ? NT : kMaxWidth];
-	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = NT / s.tx;
-	const unsigned item = s.paired ? (blockIdx.x / 16 * 8 + blockIdx.x % 8) * 2 + blockIdx.x / 8 % 2 : blockIdx.x;
-	const int slab = item % s.slabs;
-	const long rest = item / s.slabs, sample = rest / s.chunks;
-	const int chunk = (int)(rest % s.chunks);
-	const int c0 = slab * s.width;
+	const int ty = threadIdx.x / s.tx, tx = threadIdx.x - ty * s.tx, TY = s.ty;
+	int slab, chunk;
+	long sample;
+	place(s, slab, chunk, sample);
+	const int c0 = slab * s.width * (s.slabs > 1);
 	const int channels = s.slabs > 1 ? s.width : g.c, groups = channels / g.width, group0 = c0 / g.width;
 	const size_t start = (size_t)sample * g.pixels * g.c + c0 + (size_t)chunk * s.rows * s.pitch;
 	const T *x = (const T *)g.x + start, *dy = (const T *)g.dy + start;
-	const long all = s.slabs > 1 ? (long)1 << 62 : s.limit - (long)chunk * s.rows * s.pitch;
-	const long rows = min(s.rows, s.slabs > 1 ? s.rows : (all + s.pitch - 1) / s.pitch);
-	const bool active = ty < TY;
 
 	typename Vec<T>::raw v[NV], d[NV];
 	int mine, last;
-	share(s, active, ty, TY, tx * V, V, rows, all, NV, mine, last);
+	share<V>(s, chunk, tx, ty, NV, mine, last);
 #pragma unroll
 	for (int k = 0; k < NV; ++k) {
-		const long at = (ty + (long)k * TY) * s.pitch + tx * V;
+		const size_t at = (ty + k * TY) * (size_t)s.pitch + tx * V;
 		const int left = k + 1 < mine ? V : last;
 		if (k < mine) v[k] = load_vec(x + at, left), d[k] = load_vec(dy + at, left);      // (beyond the end: zeros, which add nothing)
 	}
 	float mean[CELLS], inv[CELLS], scale[V], bias[V], da[V], db[V];
-#pragma unroll
-	for (int e = 0; e < V; ++e) {
-		const int ch = (tx * V + e) % g.c;
-		const size_t at = sample * g.groups + group0 + ch / g.width;
+	if (UNI) load_floats(g.scale, c0 + tx * V, 1.f, scale), load_floats(g.bias, c0 + tx * V, 0.f, bias);
+	each_channel<V, UNI>(tx * V, g.c, g.width, [&](int e, int ch, int group) {
+		const size_t at = sample * g.groups + group0 + group;
 		if (!UNI || e == 0) mean[UNI ? 0 : e] = g.mean[at], inv[UNI ? 0 : e] = g.invvar[at];
-		scale[e] = or_else(g.scale, c0 + ch, 1.f), bias[e] = or_else(g.bias, c0 + ch, 0.f);
+		if (!UNI) scale[e] = or_else(g.scale, c0 + ch, 1.f), bias[e] = or_else(g.bias, c0 + ch, 0.f);
 		da[e] = db[e] = 0.f;
-	}
+	});
 #pragma unroll
 	for (int k = 0; k < NV; ++k) {
 		if (k >= mine) continue;
@@ -296,7 +341,7 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 			da[e] += t, db[e] += t * xhat;
 		}
 	}
-	if (active) {
+	if (ty < TY) {
 #pragma unroll
 		for (int e = 0; e < V; ++e) red[0][(ty * s.tx + tx) * V + e] = da[e], red[1][(ty * s.tx + tx) * V + e] = db[e];
 	}
@@ -318,13 +363,9 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 	sum_cells<NT>(chan[0], 0, 1, 1, 0, g.width, groups, one, sa);
 	sum_cells<NT>(chan[1], 0, 1, 1, 0, g.width, groups, one, sb);
 	__syncthreads();
-	if (!active) return;
+	if (mine == 0) return;
 	float a[CELLS], b[CELLS];
-#pragma unroll
-	for (int e = 0; e < CELLS; ++e) {
-		const int group = (tx * V + e) % g.c / g.width;
-		a[e] = sa[group], b[e] = sb[group];
-	}
+	each_channel<CELLS, UNI>(tx * V, g.c, g.width, [&](int e, int, int group) { a[e] = sa[group], b[e] = sb[group]; });
 	T *dx = (T *)g.out + start;
 #pragma unroll
 	for (int k = 0; k < NV; ++k) {
@@ -337,59 +378,69 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 			const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act));
 			o[e] = inv[u] * (t - a[u] - xhat * b[u]);
 		}
-		store_vec(dx + (ty + (long)k * TY) * s.pitch + tx * V, k + 1 < mine ? V : last, o);
+		store_vec(dx + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last, o);
 	}
 }
 
-// A and B of the head, divided by m, of a (sample, group) from its chunks' channel sums: a wave each
+// A and B of the head, divided by m, of a (sample, group) from its chunks' channel sums: a workgroup each
 __global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, const float *sums, float2 *ab) {
-	const long at = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-	if (at >= (long)g.n * g.groups) return;
-	const int lane = threadIdx.x & 63;
-	const long sample = at / g.groups;
+	__shared__ double part[2][4];
+	const long at = blockIdx.x, sample = at / g.groups;
 	const int c0 = (int)(at % g.groups) * g.width;
 	double a = 0.0, b = 0.0;
-	for (long i = lane; i < (long)s.chunks * g.width; i += 64) {
-		const int ch = c0 + (int)(i % g.width);
-		const float *p = sums + ((size_t)sample * s.chunks + i / g.width) * 2 * g.c + ch;
+	for (int i = threadIdx.x; i < s.chunks * g.width; i += 256) {
+		const int chunk = i / g.width, ch = c0 + i - chunk * g.width;
+		const float *p = sums + ((size_t)sample * s.chunks + chunk) * 2 * g.c + ch;
 		const double f = or_else(g.scale, ch, 1.f);
 		a += f * p[0], b += f * p[g.c];
 	}
 	for (int l = 32; l > 0; l >>= 1) a += __shfl_xor(a, l, 64), b += __shfl_xor(b, l, 64);
+	if ((threadIdx.x & 63) == 0) part[0][threadIdx.x >> 6] = a, part[1][threadIdx.x >> 6] = b;
+	__syncthreads();
+	if (threadIdx.x > 0) return;
 	const double m = (double)g.pixels * g.width;
-	if (lane == 0) ab[at] = make_float2((float)(a / m), (float)(b / m));
+	a = part[0][0] + part[0][1] + part[0][2] + part[0][3], b = part[1][0] + part[1][1] + part[1][2] + part[1][3];
+	ab[at] = make_float2((float)(a / m), (float)(b / m));
 }
 
-template <typename T, int NV>
+template <typename T, int NV, bool UNI>
 __global__ void __launch_bounds__(256) norm_apply_bwd_kernel(Norm g, Slab s, const float2 *ab) {
-	constexpr int V = Vec<T>::V;
-	const int tx = threadIdx.x % s.tx, ty = threadIdx.x / s.tx, TY = 256 / s.tx;
-	if (ty >= TY) return;
-	const long sample = blockIdx.x / s.chunks, row0 = (long)(blockIdx.x % s.chunks) * s.rows;
-	const size_t start = (size_t)sample * g.pixels * g.c;
+	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
+	const int ty = threadIdx.x / s.tx, tx = threadIdx.x - ty * s.tx;
+	int slab, chunk, mine, last;
+	long sample;
+	place(s, slab, chunk, sample);
+	share<V>(s, chunk, tx, ty, NV, mine, last);
+	const size_t start = (size_t)sample * g.pixels * g.c + (size_t)chunk * s.rows * s.pitch + (size_t)ty * s.pitch + tx * V;
 	const T *x = (const T *)g.x + start, *dy = (const T *)g.dy + start;
 	T *dx = (T *)g.out + start;
-	float mean[V], inv[V], scale[V], bias[V];
-	float2 sum[V];
-#pragma unroll
-	for (int e = 0; e < V; ++e) {
-		const int ch = (tx * V + e) % g.c;
-		const size_t at = sample * g.groups + ch / g.width;
-		mean[e] = g.mean[at], inv[e] = g.invvar[at], scale[e] = or_else(g.scale, ch, 1.f), bias[e] = or_else(g.bias, ch, 0.f), sum[e] = ab[at];
-	}
+	typename Vec<T>::raw v[NV], d[NV];
 #pragma unroll
 	for (int k = 0; k < NV; ++k) {
-		const long r = ty + (long)k * TY, at = (row0 + r) * s.pitch + tx * V, left = r < s.rows ? s.limit - at : 0;
-		if (left <= 0) continue;
-		const typename Vec<T>::raw v = load_vec(x + at, left), d = load_vec(dy + at, left);
+		const size_t at = (size_t)k * s.ty * s.pitch;
+		const int left = k + 1 < mine ? V : last;
+		if (k < mine) v[k] = load_vec(x + at, left), d[k] = load_vec(dy + at, left);
+	}
+	float mean[CELLS], inv[CELLS], scale[V], bias[V];
+	float2 sum[CELLS];
+	if (UNI) load_floats(g.scale, tx * V, 1.f, scale), load_floats(g.bias, tx * V, 0.f, bias);
+	each_channel<V, UNI>(tx * V, g.c, g.width, [&](int e, int ch, int group) {
+		const size_t at = sample * g.groups + group;
+		if (!UNI || e == 0) mean[UNI ? 0 : e] = g.mean[at], inv[UNI ? 0 : e] = g.invvar[at], sum[UNI ? 0 : e] = ab[at];
+		if (!UNI) scale[e] = or_else(g.scale, ch, 1.f), bias[e] = or_else(g.bias, ch, 0.f);
+	});
+#pragma unroll
+	for (int k = 0; k < NV; ++k) {
+		if (k >= mine) continue;
 		float o[V];
 #pragma unroll
 		for (int e = 0; e < V; ++e) {
-			const float xhat = ((float)v[e] - mean[e]) * inv[e];
-			const float t = scale[e] * ((float)d[e] * act_slope(scale[e] * xhat + bias[e], g.act));
-			o[e] = inv[e] * (t - sum[e].x - xhat * sum[e].y);
+			const int u = UNI ? 0 : e;
+			const float xhat = ((float)v[k][e] - mean[u]) * inv[u];
+			const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act));
+			o[e] = inv[u] * (t - sum[u].x - xhat * sum[u].y);
 		}
-		store_vec(dx + at, left, o);
+		store_vec(dx + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last, o);
 	}
 }
 
@@ -474,22 +525,27 @@ __global__ void __launch_bounds__(256) norm_channel_kernel(Norm g, float *sums) 
 	sums[(sample * 2 + 1) * g.c + ch] = (float)s;
 }
 
-// dbias, dscale: the samples' (and chunks') sums, added in a fixed order in float64. A workgroup takes 64 channels, 16 rows at a time.
+// dbias, dscale: the samples' (and chunks') sums, added in a fixed order in float64. A workgroup takes 16 channels, 64 rows at a time.
 __global__ void __launch_bounds__(1024) norm_param_kernel(const float *sums, long rows, int c, float *dscale, float *dbias) {
-	__shared__ double part[2][16][64];
-	const int ch = blockIdx.x * 64 + (threadIdx.x & 63), lane = threadIdx.x & 63, row = threadIdx.x >> 6;
+	__shared__ double part[2][64][16];
+	const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, ch = blockIdx.x * 16 + lane;
 	double s = 0.0, b = 0.0;
-	if (ch < c)
-		for (long i = row; i < rows; i += 16) {
+	if (ch < c) {
+#pragma unroll 4
+		for (long i = row; i < rows; i += 64) {
 			b += sums[(size_t)i * 2 * c + ch];
 			s += sums[((size_t)i * 2 + 1) * c + ch];
 		}
+	}
 	part[0][row][lane] = b, part[1][row][lane] = s;
 	__syncthreads();
+	for (int half = 32; half > 0; half >>= 1) {
+		if (row < half) part[0][row][lane] += part[0][row + half][lane], part[1][row][lane] += part[1][row + half][lane];
+		__syncthreads();
+	}
 	if (row > 0 || ch >= c) return;
-	for (int i = 1; i < 16; ++i) b += part[0][i][lane], s += part[1][i][lane];
-	if (dbias) dbias[ch] = (float)b;
-	if (dscale) dscale[ch] = (float)s;
+	if (dbias) dbias[ch] = (float)part[0][0][lane];
+	if (dscale) dscale[ch] = (float)part[1][0][lane];
 }
 
 // ---- host --------------------------------------------------------------------------------------------------------------------------------
@@ -527,49 +583,56 @@ constexpr int kForwardVectors = 16, kBackwardVectors = 8;
 Slab back_to_back(const pz_groupnorm_desc *d, int v, int threads, int vectors) {
 	Slab s{};
 	const int width = d->c / d->groups, period = (int)(d->c / gcd(d->c, v) * v);          // lcm
-	s.width = period, s.tx = period / v, s.reps = period / d->c, s.slabs = 1, s.pitch = period;
+	s.width = s.pitch = period, s.tx = period / v, s.ty = threads / s.tx, s.reps = period / d->c, s.slabs = s.sharing = 1;
 	s.uniform = s.reps == 1 && width % v == 0;
-	s.limit = (long)d->pixels * d->c;
 	s.wd = s.uniform ? width / v : width, s.period = s.uniform ? d->c / v : d->c;
-	const long rows = (s.limit + period - 1) / period, held = (long)(threads / s.tx) * vectors;
-	s.rows = rows < held ? rows : held;
+	const long values = (long)d->pixels * d->c, rows = (values + period - 1) / period, held = (long)s.ty * vectors;
+	s.rows = (int)(rows < held ? rows : held);
 	s.chunks = (int)((rows + s.rows - 1) / s.rows);
+	const long before = (long)(s.chunks - 1) * s.rows;
+	s.last_rows = (int)(rows - before), s.last_values = (int)(values - before * period);
+	s.count = (float)((long)s.rows * period / d->c * width), s.last_count = (float)((long)s.last_values / d->c * width);
 	return s;
 }
 
 Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
 	Plan p{};
 	const int v = d->dtype == PZ_F16 ? 8 : 4, size = d->dtype == PZ_F16 ? 2 : 4, width = d->c / d->groups;
-	const long period = d->c / gcd(d->c, v) * v, limit = (long)d->pixels * d->c;
+	const long period = d->c / gcd(d->c, v) * v;
 	const int vectors = backward ? kBackwardVectors : kForwardVectors;
 	if (d->n == 0 || d->pixels == 0) return p;
 
-	// whole groups of a channel count that vectors divide: the narrowest slab that is a cache line wide (half a line where that is all that fits)
+	// whole groups of a channel count that vectors divide: the widest slab of a cache line or half of one of which a CU holds two workgroups
+	// (one loads while the other stores); where none fits, one workgroup of twice the size. Quarter lines do not pay: 115 instead of 87 us
+	// for 32 x 4096 x 512 float16
 	const long unit = width / gcd(width, v) * v;
+	const bool uniform = width % v == 0;
 	if (d->c % v == 0 && d->c % unit == 0 && unit <= kMaxWidth) {
-		for (const long bytes : {128l, 64l}) {
-			long slab = unit;
-			while (slab * size < bytes && slab < d->c) {
-				do slab += unit;
-				while (d->c % slab != 0);
-			}
-			if (slab > kMaxWidth) continue;
-			const int tx = (int)(slab / v);
-			const bool uniform = width % v == 0;
-			for (const int nt : {256, 1024})
-				for (const int nv : {4, vectors}) {
-					if (nt == 1024 && (!uniform || nv == 4) && !(backward && uniform)) continue;
-					if (tx > nt || (long)(nt / tx) * nv < d->pixels) continue;
-					p.way = WAY_ONE, p.nt = nt, p.nv = nv;
-					Slab s{};
-					s.width = (int)slab, s.tx = tx, s.reps = 1, s.slabs = (int)(d->c / slab), s.uniform = uniform, s.pitch = d->c;
-					s.rows = d->pixels, s.limit = limit, s.chunks = 1;
-					s.paired = slab * size < 128 && (long)d->n * s.slabs % 16 == 0;
-					s.wd = uniform ? width / v : width, s.period = 0;
-					if (s.slabs == 1) s.period = uniform ? d->c / v : d->c;
-					p.slab = s;
-					return p;
+		for (const int most : {512, 1024}) {
+			for (const long bytes : {128l, 64l}) {
+				long slab = unit;
+				while (slab * size < bytes && slab < d->c) {
+					do slab += unit;
+					while (d->c % slab != 0);
 				}
+				if (slab > kMaxWidth) continue;
+				const int tx = (int)(slab / v);
+				for (int nt = 256; nt <= (uniform ? most : 256); nt *= 2)
+					for (const int nv : {4, vectors}) {
+						if (tx > nt || (long)(nt / tx) * nv < d->pixels) continue;
+						p.way = WAY_ONE, p.nt = nt, p.nv = nv;
+						Slab s{};
+						s.width = (int)slab, s.tx = tx, s.ty = nt / tx, s.reps = 1, s.slabs = (int)(d->c / slab), s.uniform = uniform, s.pitch = d->c;
+						s.rows = s.last_rows = d->pixels, s.last_values = (int)(d->pixels * slab), s.chunks = 1;
+						s.count = s.last_count = (float)((long)d->pixels * width);
+						s.sharing = (int)(128 / (slab * size));
+						if (s.sharing < 1 || (long)d->n * s.slabs % (8 * s.sharing) != 0) s.sharing = 1;
+						s.wd = uniform ? width / v : width, s.period = 0;
+						if (s.slabs == 1) s.period = uniform ? d->c / v : d->c;
+						p.slab = s;
+						return p;
+					}
+			}
 		}
 	}
 	if (period > kMaxWidth || period / v > 256) return p;                                   // WAY_PLAIN
@@ -581,7 +644,7 @@ Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
 	}
 	p.way = WAY_CHUNKS, p.nt = 256, p.nv = vectors;
 	p.slab = back_to_back(d, v, 256, vectors);
-	p.apply = back_to_back(d, v, 256, 4);
+	p.apply = back_to_back(d, v, 256, 8);
 	p.part_bytes = backward ? 0 : (size_t)d->n * p.slab.chunks * d->groups * sizeof(float2);
 	p.stat_bytes = (size_t)d->n * d->groups * sizeof(float2);
 	return p;
@@ -606,6 +669,7 @@ int forward(const pz_groupnorm_desc *d, const Norm &g, char *ws, hipStream_t st)
 	if (p.way == WAY_ONE) {
 		if (p.slab.uniform) {
 			if (p.nt == 1024) slab_fwd<T, 1024, 16, true, true>(g, p, nullptr, st);
+			else if (p.nt == 512) slab_fwd<T, 512, 16, true, true>(g, p, nullptr, st);
 			else if (p.nv == 4) slab_fwd<T, 256, 4, true, true>(g, p, nullptr, st);
 			else slab_fwd<T, 256, 16, true, true>(g, p, nullptr, st);
 		} else if (p.nv == 4) slab_fwd<T, 256, 4, false, true>(g, p, nullptr, st);
@@ -622,7 +686,9 @@ int forward(const pz_groupnorm_desc *d, const Norm &g, char *ws, hipStream_t st)
 	PZ_LAUNCH_CHECK();
 	norm_join_kernel<<<pz::ceil_div((long)d->n * d->groups, 4), 256, 0, st>>>(g, p.slab, part, mean, invvar);
 	PZ_LAUNCH_CHECK();
-	norm_apply_kernel<T, 4><<<(unsigned)((long)d->n * p.apply.chunks), 256, 0, st>>>(g, p.apply, mean, invvar);
+	const unsigned blocks = (unsigned)((long)d->n * p.apply.chunks);
+	if (p.apply.uniform) norm_apply_kernel<T, 8, true><<<blocks, 256, 0, st>>>(g, p.apply, mean, invvar);
+	else norm_apply_kernel<T, 8, false><<<blocks, 256, 0, st>>>(g, p.apply, mean, invvar);
 	PZ_LAUNCH_CHECK();
 	return PZ_OK;
 }
@@ -647,7 +713,8 @@ int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, h
 	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_bwd: too many workgroups");
 	if (p.way == WAY_ONE) {
 		if (p.slab.uniform) {
-			if (p.nt == 1024) p.nv == 4 ? slab_bwd<T, 1024, 4, true, true>(g, p, sums, st) : slab_bwd<T, 1024, 8, true, true>(g, p, sums, st);
+			if (p.nt == 1024) slab_bwd<T, 1024, 8, true, true>(g, p, sums, st);
+			else if (p.nt == 512) slab_bwd<T, 512, 8, true, true>(g, p, sums, st);
 			else p.nv == 4 ? slab_bwd<T, 256, 4, true, true>(g, p, sums, st) : slab_bwd<T, 256, 8, true, true>(g, p, sums, st);
 		} else p.nv == 4 ? slab_bwd<T, 256, 4, false, true>(g, p, sums, st) : slab_bwd<T, 256, 8, false, true>(g, p, sums, st);
 		PZ_LAUNCH_CHECK();
@@ -657,9 +724,11 @@ int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, h
 	if (p.slab.uniform) slab_bwd<T, 256, 8, true, false>(g, p, sums, st);
 	else slab_bwd<T, 256, 8, false, false>(g, p, sums, st);
 	PZ_LAUNCH_CHECK();
-	norm_join_bwd_kernel<<<pz::ceil_div((long)d->n * d->groups, 4), 256, 0, st>>>(g, p.slab, sums, (float2 *)ws);
+	norm_join_bwd_kernel<<<(unsigned)((long)d->n * d->groups), 256, 0, st>>>(g, p.slab, sums, (float2 *)ws);
 	PZ_LAUNCH_CHECK();
-	norm_apply_bwd_kernel<T, 4><<<(unsigned)((long)d->n * p.apply.chunks), 256, 0, st>>>(g, p.apply, (const float2 *)ws);
+	const unsigned blocks = (unsigned)((long)d->n * p.apply.chunks);
+	if (p.apply.uniform) norm_apply_bwd_kernel<T, 8, true><<<blocks, 256, 0, st>>>(g, p.apply, (const float2 *)ws);
+	else norm_apply_bwd_kernel<T, 8, false><<<blocks, 256, 0, st>>>(g, p.apply, (const float2 *)ws);
 	PZ_LAUNCH_CHECK();
 	return PZ_OK;
 }
@@ -709,7 +778,7 @@ int pz_groupnorm_bwd(const pz_groupnorm_desc *d, const void *dy, const void *x, 
 		if (int rc = d->dtype == PZ_F16 ? backward<f16>(d, g, sums, ws, st) : backward<float>(d, g, sums, ws, st)) return rc;
 	}
 	if (dscale || dbias) {
-		norm_param_kernel<<<pz::ceil_div(d->c, 64), 1024, 0, st>>>(sums, (long)rows, d->c, dscale, dbias);
+		norm_param_kernel<<<pz::ceil_div(d->c, 16), 1024, 0, st>>>(sums, (long)rows, d->c, dscale, dbias);
 		PZ_LAUNCH_CHECK();
 	}
 	return PZ_OK;

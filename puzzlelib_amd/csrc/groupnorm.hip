@@ -154,7 +154,8 @@ template <typename T, int NT, int NV, bool UNI, bool FINISH>
 __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *part) {
 	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
 	__shared__ float red[NT * CELLS];
-	__shared__ float smean[UNI ? NT : kMaxWidth], sinv[UNI ? NT : kMaxWidth];      // (vectors inside one group: no more groups than vectors in a row)
+	constexpr int GROUPS = UNI ? NT : NT * V < kMaxWidth ? NT * V : kMaxWidth;      // (of a row of NT vectors at most; UNI: one to a vector at most)
+	__shared__ float smean[GROUPS], sinv[GROUPS];
 	const int ty = threadIdx.x / s.tx, tx = threadIdx.x - ty * s.tx, TY = s.ty;
 	int slab, chunk;
 	long sample;
@@ -303,8 +304,9 @@ template <typename T, int NT, int NV, bool UNI, bool FINISH>
 __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float *sums) {
 	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
 	__shared__ float red[2][NT * V];
-	__shared__ float chan[2][kMaxWidth];
-	__shared__ float sa[UNI ? NT : kMaxWidth], sb[UNI ? NT : kMaxWidth];
+	__shared__ float chan[2][NT * V < kMaxWidth ? NT * V : kMaxWidth];      // (a row has NT vectors at most)
+	constexpr int GROUPS = UNI ? NT : NT * V < kMaxWidth ? NT * V : kMaxWidth;
+	__shared__ float sa[GROUPS], sb[GROUPS];
 	const int ty = threadIdx.x / s.tx, tx = threadIdx.x - ty * s.tx, TY = s.ty;
 	int slab, chunk;
 	long sample;
@@ -388,6 +390,7 @@ __global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, cons
 	const long at = blockIdx.x, sample = at / g.groups;
 	const int c0 = (int)(at % g.groups) * g.width;
 	double a = 0.0, b = 0.0;
+#pragma unroll 4
 	for (int i = threadIdx.x; i < s.chunks * g.width; i += 256) {
 		const int chunk = i / g.width, ch = c0 + i - chunk * g.width;
 		const float *p = sums + ((size_t)sample * s.chunks + chunk) * 2 * g.c + ch;
@@ -617,9 +620,12 @@ Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
 				}
 				if (slab > kMaxWidth) continue;
 				const int tx = (int)(slab / v);
-				for (int nt = 256; nt <= (uniform ? most : 256); nt *= 2)
+				for (const int nt : {64, 256, 512, 1024})
 					for (const int nv : {4, vectors}) {
-						if (tx > nt || (long)(nt / tx) * nv < d->pixels) continue;
+						if (nt > (uniform ? most : 256) || (nt == 64 && nv > 4) || tx > nt || (long)(nt / tx) * nv < d->pixels) continue;
+						// few large workgroups leave most of the chip idle: chunks, although they read twice (16 workgroups of 256 KiB: 25 us,
+						// chunks 14)
+						if (nt > 256 && (long)d->n * (d->c / slab) < pz::kNumCU / 2) continue;
 						p.way = WAY_ONE, p.nt = nt, p.nv = nv;
 						Slab s{};
 						s.width = (int)slab, s.tx = tx, s.ty = nt / tx, s.reps = 1, s.slabs = (int)(d->c / slab), s.uniform = uniform, s.pitch = d->c;
@@ -636,12 +642,14 @@ Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
 		}
 	}
 	if (period > kMaxWidth || period / v > 256) return p;                                   // WAY_PLAIN
-	for (const int nv : {4, vectors}) {
-		const Slab s = back_to_back(d, v, 256, nv);
-		if (s.chunks > 1) continue;
-		p.way = WAY_ONE, p.nt = 256, p.nv = nv, p.slab = s;
-		return p;
-	}
+	for (const int nt : {64, 256})
+		for (const int nv : {4, vectors}) {
+			if (period / v > nt || (nt == 64 && nv > 4)) continue;
+			const Slab s = back_to_back(d, v, nt, nv);
+			if (s.chunks > 1) continue;
+			p.way = WAY_ONE, p.nt = nt, p.nv = nv, p.slab = s;
+			return p;
+		}
 	p.way = WAY_CHUNKS, p.nt = 256, p.nv = vectors;
 	p.slab = back_to_back(d, v, 256, vectors);
 	p.apply = back_to_back(d, v, 256, 8);
@@ -668,11 +676,13 @@ int forward(const pz_groupnorm_desc *d, const Norm &g, char *ws, hipStream_t st)
 	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_fwd: too many workgroups");
 	if (p.way == WAY_ONE) {
 		if (p.slab.uniform) {
-			if (p.nt == 1024) slab_fwd<T, 1024, 16, true, true>(g, p, nullptr, st);
+			if (p.nt == 64) slab_fwd<T, 64, 4, true, true>(g, p, nullptr, st);
+			else if (p.nt == 1024) slab_fwd<T, 1024, 16, true, true>(g, p, nullptr, st);
 			else if (p.nt == 512) slab_fwd<T, 512, 16, true, true>(g, p, nullptr, st);
 			else if (p.nv == 4) slab_fwd<T, 256, 4, true, true>(g, p, nullptr, st);
 			else slab_fwd<T, 256, 16, true, true>(g, p, nullptr, st);
-		} else if (p.nv == 4) slab_fwd<T, 256, 4, false, true>(g, p, nullptr, st);
+		} else if (p.nt == 64) slab_fwd<T, 64, 4, false, true>(g, p, nullptr, st);
+		else if (p.nv == 4) slab_fwd<T, 256, 4, false, true>(g, p, nullptr, st);
 		else slab_fwd<T, 256, 16, false, true>(g, p, nullptr, st);
 		PZ_LAUNCH_CHECK();
 		return PZ_OK;
@@ -713,10 +723,12 @@ int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, h
 	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_bwd: too many workgroups");
 	if (p.way == WAY_ONE) {
 		if (p.slab.uniform) {
-			if (p.nt == 1024) slab_bwd<T, 1024, 8, true, true>(g, p, sums, st);
+			if (p.nt == 64) slab_bwd<T, 64, 4, true, true>(g, p, sums, st);
+			else if (p.nt == 1024) slab_bwd<T, 1024, 8, true, true>(g, p, sums, st);
 			else if (p.nt == 512) slab_bwd<T, 512, 8, true, true>(g, p, sums, st);
 			else p.nv == 4 ? slab_bwd<T, 256, 4, true, true>(g, p, sums, st) : slab_bwd<T, 256, 8, true, true>(g, p, sums, st);
-		} else p.nv == 4 ? slab_bwd<T, 256, 4, false, true>(g, p, sums, st) : slab_bwd<T, 256, 8, false, true>(g, p, sums, st);
+		} else if (p.nt == 64) slab_bwd<T, 64, 4, false, true>(g, p, sums, st);
+		else p.nv == 4 ? slab_bwd<T, 256, 4, false, true>(g, p, sums, st) : slab_bwd<T, 256, 8, false, true>(g, p, sums, st);
 		PZ_LAUNCH_CHECK();
 		return PZ_OK;
 	}

@@ -33,7 +33,7 @@ int run(const void *x, const void *residual, void *y, size_t count, const pz_dro
 	constexpr int COUNT = 16 / sizeof(T);
 	const int vec = (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) & 15) == 0;
 	const size_t blocks = (count + 256 * COUNT - 1) / (256 * COUNT);
-	PZ_REQUIRE(blocks < (1ull << 31), "pz_dropout: %zu elements are too many", count);
+	PZ_REQUIRE(launchable(blocks, 256), "pz_dropout: %zu elements are too many", count);
 	dropout_kernel<T><<<(unsigned)blocks, 256, 0, st>>>((const T *)x, (const T *)residual, (T *)y, count,
 	                                                    DropKey{mask->seed, mask->call, mask->threshold, mask->keep}, vec);
 	PZ_LAUNCH_CHECK();

@@ -558,7 +558,8 @@ int check(const pz_groupnorm_desc *d, const char *who) {
 	PZ_REQUIRE(d->act >= PZ_ACT_NONE && d->act <= PZ_ACT_SILU, "%s: unknown activation %d", who, d->act);
 	PZ_REQUIRE(d->n >= 0 && d->pixels >= 0 && d->c > 0 && d->groups > 0 && d->c % d->groups == 0, "%s: bad dimensions (%d, %d, %d) in %d groups", who,
 	           d->n, d->pixels, d->c, d->groups);
-	PZ_REQUIRE((long)d->n * d->groups < (1l << 31) && (long)d->n * d->c < (1l << 38), "%s: %d samples of %d channels are too many", who, d->n, d->c);
+	PZ_REQUIRE((long)d->n * d->groups < (1l << 31) && (long)d->n * d->c < (1l << 32) - 256 && d->c < (1 << 26), "%s: %d samples of %d channels are too many", who, d->n, d->c);
+	PZ_REQUIRE(d->epsilon >= 0.f, "%s: epsilon %g", who, d->epsilon);
 	return PZ_OK;
 }
 
@@ -669,11 +670,12 @@ template <typename T>
 int forward(const pz_groupnorm_desc *d, const Norm &g, char *ws, hipStream_t st) {
 	const Plan p = plan_norm(d, false);
 	if (p.way == WAY_PLAIN) {
+		PZ_REQUIRE(launchable((long)d->n * d->groups, 256), "pz_groupnorm_fwd: too many workgroups");
 		norm_fwd_kernel<T><<<d->n * d->groups, 256, 0, st>>>(g);
 		PZ_LAUNCH_CHECK();
 		return PZ_OK;
 	}
-	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_fwd: too many workgroups");
+	PZ_REQUIRE(launchable((long)d->n * p.slab.chunks * p.slab.slabs, p.nt), "pz_groupnorm_fwd: too many workgroups");
 	if (p.way == WAY_ONE) {
 		if (p.slab.uniform) {
 			if (p.nt == 64) slab_fwd<T, 64, 4, true, true>(g, p, nullptr, st);
@@ -690,7 +692,7 @@ int forward(const pz_groupnorm_desc *d, const Norm &g, char *ws, hipStream_t st)
 	float2 *part = (float2 *)ws;
 	float *stats = (float *)(ws + p.part_bytes);
 	float *mean = g.mean ? g.mean : stats, *invvar = g.invvar ? g.invvar : stats + (size_t)d->n * d->groups;
-	PZ_REQUIRE((long)d->n * p.apply.chunks < (1l << 31), "pz_groupnorm_fwd: too many workgroups");
+	PZ_REQUIRE(launchable((long)d->n * p.apply.chunks, 256), "pz_groupnorm_fwd: too many workgroups");
 	if (p.slab.uniform) slab_fwd<T, 256, 16, true, false>(g, p, part, st);
 	else slab_fwd<T, 256, 16, false, false>(g, p, part, st);
 	PZ_LAUNCH_CHECK();
@@ -711,6 +713,7 @@ void slab_bwd(const Norm &g, const Plan &p, float *sums, hipStream_t st) {
 template <typename T>
 int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, hipStream_t st) {
 	const Plan p = plan_norm(d, true);
+	PZ_REQUIRE(p.way == WAY_ONE || launchable((long)d->n * d->groups, 256), "pz_groupnorm_bwd: too many workgroups");
 	if (p.way == WAY_PLAIN) {
 		if (sums) {
 			norm_channel_kernel<T><<<pz::ceil_div((long)d->n * d->c, 256), 256, 0, st>>>(g, sums);
@@ -720,7 +723,7 @@ int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, h
 		PZ_LAUNCH_CHECK();
 		return PZ_OK;
 	}
-	PZ_REQUIRE((long)d->n * p.slab.chunks * p.slab.slabs < (1l << 31), "pz_groupnorm_bwd: too many workgroups");
+	PZ_REQUIRE(launchable((long)d->n * p.slab.chunks * p.slab.slabs, p.nt), "pz_groupnorm_bwd: too many workgroups");
 	if (p.way == WAY_ONE) {
 		if (p.slab.uniform) {
 			if (p.nt == 64) slab_bwd<T, 64, 4, true, true>(g, p, sums, st);
@@ -732,7 +735,7 @@ int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, h
 		PZ_LAUNCH_CHECK();
 		return PZ_OK;
 	}
-	PZ_REQUIRE((long)d->n * p.apply.chunks < (1l << 31), "pz_groupnorm_bwd: too many workgroups");
+	PZ_REQUIRE(launchable((long)d->n * p.apply.chunks, 256), "pz_groupnorm_bwd: too many workgroups");
 	if (p.slab.uniform) slab_bwd<T, 256, 8, true, false>(g, p, sums, st);
 	else slab_bwd<T, 256, 8, false, false>(g, p, sums, st);
 	PZ_LAUNCH_CHECK();

@@ -634,6 +634,18 @@ void launch(const Plan &p, const Product &g, bool ta, bool tb, dim3 grid, hipStr
 	else launch<T, false, false>(p, g, grid, st);
 }
 
+// a lane's place in a tile is a 32-bit offset from the tile's start: of up to bm rows where k runs along a row, of bk steps elsewhere
+int check_reach(int dtype, const Operands &o, const char *who) {
+	const Plan p = plan_product(dtype, o);
+	auto reach = [&](bool copied, long ld, bool kmajor, int rows, int block) {
+		const long held = kmajor ? (o.k < p.bk ? o.k : p.bk) : (rows < block ? rows : block);
+		return held * (copied ? padded(kmajor ? rows : o.k) : ld) <= 0xfffff000l / (dtype == PZ_F16 ? 2 : 4);
+	};
+	PZ_REQUIRE(o.m == 0 || o.n == 0 || (reach(p.copy_a, o.lda, o.ta, o.m, p.bm) && reach(p.copy_b, o.ldb, !o.tb, o.n, p.bn)),
+	           "%s: rows of %ld and %ld elements are too far apart", who, o.lda, o.ldb);
+	return PZ_OK;
+}
+
 size_t extent_of(int rows, int wide, long ld, int size) { return rows > 0 ? ((size_t)(rows - 1) * ld + wide) * size : 0; }
 
 // C = epilogue(A B); ws: plan_product(...).bytes()
@@ -647,7 +659,7 @@ int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st
 		if (p.copy_b) b.dst = ws + p.a_bytes, b.rows = o.tb ? o.n : o.k, b.cols = o.tb ? o.k : o.n, b.pitch = padded(b.cols), o.b = b.dst, o.ldb = b.pitch;
 		auto blocks = [&](const Aligned &x) { return ((size_t)x.rows * (x.pitch * size / 16) + 255) / 256; };
 		const size_t total = blocks(a) + blocks(b);
-		PZ_REQUIRE(total < (1ull << 31), "linear: an unaligned operand of %d x %d is too large", o.m, o.k);
+		PZ_REQUIRE(launchable(total, 256), "linear: an unaligned operand of %d x %d is too large", o.m, o.k);
 		if (total > 0) {
 			if (dtype == PZ_F16) linear_align_kernel<f16><<<(unsigned)total, 256, 0, st>>>(a, b, (unsigned)blocks(a));
 			else linear_align_kernel<float><<<(unsigned)total, 256, 0, st>>>(a, b, (unsigned)blocks(a));
@@ -670,8 +682,7 @@ int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st
 	else launch<float>(p, g, o.ta, o.tb, grid, st);
 	PZ_LAUNCH_CHECK();
 	if (p.splits > 1) {
-		const size_t items = (size_t)o.m * (padded(o.n) * size / 16);
-		PZ_REQUIRE(items < (1ull << 38), "linear: %d rows are too many", o.m);
+		const size_t items = (size_t)o.m * (padded(o.n) * size / 16);         // (a split has fewer tiles than the chip has CUs)
 		const unsigned blocks = (unsigned)((items + 255) / 256);
 		if (dtype == PZ_F16) linear_join_kernel<f16><<<blocks, 256, 0, st>>>(g);
 		else linear_join_kernel<float><<<blocks, 256, 0, st>>>(g);
@@ -685,6 +696,8 @@ int check_desc(const pz_linear_desc *d, const char *who) {
 	PZ_REQUIRE(d->dtype == PZ_F32 || d->dtype == PZ_F16, "%s: unknown dtype %d", who, d->dtype);
 	PZ_REQUIRE(d->act >= PZ_ACT_NONE && d->act <= PZ_ACT_SILU, "%s: unknown activation %d", who, d->act);
 	PZ_REQUIRE(d->m >= 0 && d->n > 0 && d->k > 0, "%s: bad dimensions (%d, %d, %d)", who, d->m, d->n, d->k);
+	// (32-bit indexes run up to two tiles and a workgroup's rows beyond the end)
+	PZ_REQUIRE(d->m <= 0x7fffffff - (1 << 17) && d->n < (1 << 28) && d->k < (1 << 28), "%s: dimensions (%d, %d, %d) are too large", who, d->m, d->n, d->k);
 	PZ_REQUIRE(d->ldx >= d->k && d->ldw >= (d->trans_w ? d->k : d->n) && d->ldy >= d->n, "%s: row pitch too small", who);
 	return PZ_OK;
 }
@@ -762,6 +775,7 @@ int pz_linear_fwd(const pz_linear_desc *d, const void *x, const void *w, const f
 	PZ_REQUIRE((!residual || d->ldr >= d->n) && (!preact || d->ldp >= d->n), "pz_linear_fwd: row pitch too small");
 	const Operands o = forward_operands(d, x, w);
 	const size_t need = plan_product(d->dtype, o).bytes();
+	if (int rc = check_reach(d->dtype, o, "pz_linear_fwd")) return rc;
 	PZ_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "pz_linear_fwd: workspace needs %zu bytes", need);
 
 	const int size = d->dtype == PZ_F16 ? 2 : 4;
@@ -792,7 +806,6 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 	PZ_REQUIRE(!dx || d->ldr >= d->k, "pz_linear_bwd: row pitch too small");
 	const BackPlan p = plan_backward(d, dy, x, w, mask != nullptr, dx != nullptr, dw != nullptr, db != nullptr);
 	const size_t need = p.bytes();
-	PZ_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "pz_linear_bwd: workspace needs %zu bytes", need);
 
 	hipStream_t st = pz::as_stream(stream);
 	const int size = d->dtype == PZ_F16 ? 2 : 4;
@@ -801,6 +814,10 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 	const void *dz = p.write_dz ? (const void *)ws : dy;
 	const long lddz = p.write_dz ? padded(d->n) : d->ldy;
 	const int wide = p.write_dz ? padded(d->n) : d->n;
+	const Operands data = data_operands(d, dz, lddz, wide, w), weight = weight_operands(d, dz, lddz, wide, x);
+	if (int rc = dx ? check_reach(d->dtype, data, "pz_linear_bwd") : PZ_OK) return rc;
+	if (int rc = dw ? check_reach(d->dtype, weight, "pz_linear_bwd") : PZ_OK) return rc;
+	PZ_REQUIRE(need == 0 || (workspace && ws_bytes >= need), "pz_linear_bwd: workspace needs %zu bytes", need);
 
 	if (d->m > 0 && (p.write_dz || db)) {
 		Gate g{};
@@ -822,13 +839,13 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 	if (dx) {
 		Epilogue e{};
 		e.out = dx, e.ldo = d->ldr, e.kind = EPI_ACCUMULATE, e.alpha = 1.f, e.vec = runs_ok(dx, d->ldr, size);
-		if (int rc = product(d->dtype, data_operands(d, dz, lddz, wide, w), e, ws, st)) return rc;
+		if (int rc = product(d->dtype, data, e, ws, st)) return rc;
 	}
 	if (dw) {
 		Epilogue e{};
 		e.out = dw, e.ldo = d->trans_w ? d->k : d->n, e.kind = EPI_ACCUMULATE, e.alpha = alpha, e.beta = beta, e.out_f32 = dw_dtype == PZ_F32;
 		e.vec = runs_ok(dw, e.ldo, e.out_f32 ? 4 : 2) && (!e.out_f32 || e.ldo % (16 / size) == 0);
-		if (int rc = product(d->dtype, weight_operands(d, dz, lddz, wide, x), e, ws, st)) return rc;
+		if (int rc = product(d->dtype, weight, e, ws, st)) return rc;
 	}
 	return PZ_OK;
 }

@@ -7,6 +7,9 @@ typedef _Float16 f16;
 
 namespace {
 
+// a launch has fewer than 2^32 threads
+inline bool launchable(size_t blocks, unsigned threads) { return blocks < (1ull << 32) / threads; }
+
 // ---- activations, their derivatives: values in float32 ---------------------------------------------------------------------------
 __device__ __forceinline__ float exp_of(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
 

@@ -924,8 +924,10 @@ class DnnContext:
 			if data.ndim < 2:
 				raise ValueError("%s: data (batch, ..., channels) expected, got shape %s" % (what, data.shape))
 			n, c = data.shape[0], data.shape[-1]
-			if groups <= 0 or c == 0 or c % groups != 0:
-				raise ValueError("%s: %d channels do not form %d groups" % (what, c, groups))
+			if groups != int(groups) or groups <= 0 or c == 0 or c % groups != 0:
+				raise ValueError("%s: %d channels do not form %s groups" % (what, c, groups))
+			if not epsilon >= 0.0:
+				raise ValueError("%s: epsilon is %r" % (what, epsilon))
 			pixels = prod(data.shape[1:-1])
 			if max(n, c, pixels) > 0x7fffffff:
 				raise ValueError("%s: shape %s is too large" % (what, data.shape))

@@ -94,12 +94,17 @@ def linear_c_entry_refusals():
 		assert fwd(D(), key=lib.DropoutKey(1, 2, 3, keep)) == lib.PZ_ERR_INVALID
 	assert fwd(D(ldx=9, dtype=1)) == lib.PZ_ERR_INVALID and "workspace" in lib.lastError()          # a copy of x, no workspace for it
 	assert fwd(D(m=0)) == lib.PZ_OK
+	assert fwd(D(m=256, ldx=1 << 25)) == lib.PZ_ERR_INVALID and "too far apart" in lib.lastError()   # a tile's rows beyond 32-bit offsets
+	assert fwd(D(ldw=1 << 28)) == lib.PZ_ERR_INVALID and "too far apart" in lib.lastError()
+	for bad in (D(m=0x7fffffff), D(k=1 << 28, ldx=1 << 28), D(n=1 << 28, ldw=1 << 28, ldy=1 << 28)):
+		assert fwd(bad) == lib.PZ_ERR_INVALID and "too large" in lib.lastError()
 
 	bwd = real("pz_linear_bwd")
 	bwd.argtypes = lib._PROTOS["pz_linear_bwd"]
 	call = lambda d, dy=p, x=p, w=p, z=None, dx=p, dw=p, t=0, ws=None, n=0: bwd(ctypes.byref(d), dy, x, w, z, None, dx, dw, t, None, 1.0, 0.0, ws, n, None)
 	assert call(D(act=2)) == lib.PZ_ERR_INVALID and "pre-activation" in lib.lastError()
 	assert call(D(), t=1) == lib.PZ_ERR_INVALID and call(D(), dy=None) == lib.PZ_ERR_INVALID and call(D(ldr=7)) == lib.PZ_ERR_INVALID
+	assert call(D(m=256, ldr=8, ldx=1 << 28)) == lib.PZ_ERR_INVALID and "too far apart" in lib.lastError()
 	assert call(D(), x=None) == lib.PZ_ERR_INVALID and call(D(), w=None) == lib.PZ_ERR_INVALID
 	assert call(D(act=1), z=p) == lib.PZ_ERR_INVALID and "workspace" in lib.lastError()
 
@@ -108,11 +113,13 @@ def linear_c_entry_refusals():
 	assert drop(2, p, None, p, 4, ctypes.byref(mask), None) == lib.PZ_ERR_INVALID
 	assert drop(0, p, None, p, 4, None, None) == lib.PZ_ERR_INVALID
 	assert drop(0, None, None, p, 4, ctypes.byref(mask), None) == lib.PZ_ERR_INVALID
+	assert drop(0, p, None, p, 1 << 36, ctypes.byref(mask), None) == lib.PZ_ERR_INVALID and "too many" in lib.lastError()
 	assert drop(0, None, None, None, 0, ctypes.byref(mask), None) == lib.PZ_OK
 
 	G = lambda **kw: lib.GroupNormDesc(*[{**dict(dtype=0, act=0, n=2, pixels=3, c=8, groups=2, epsilon=1e-5), **kw}[f] for f, _ in lib.GroupNormDesc._fields_])
 	size = ctypes.c_size_t(0)
-	for bad in (G(dtype=3), G(act=9), G(n=-1), G(pixels=-1), G(c=0), G(groups=0), G(groups=3)):
+	for bad in (G(dtype=3), G(act=9), G(n=-1), G(pixels=-1), G(c=0), G(groups=0), G(groups=3), G(epsilon=-1.0),
+				G(n=1 << 30, c=64), G(c=1 << 26)):
 		refused(lambda: lib.pz_groupnorm_workspace_bytes(ctypes.byref(bad), 0, ctypes.byref(size)))
 	gf = real("pz_groupnorm_fwd")
 	gf.argtypes = lib._PROTOS["pz_groupnorm_fwd"]
@@ -127,7 +134,7 @@ def workspace_sizes():
 	"""every size the operators may be asked for has an answer: empty batches, single rows, the longest ones"""
 	size = ctypes.c_size_t(0)
 	for dtype in (lib.F32, lib.F16):
-		for m in (0, 1, 2, 63, 64, 65, 1000, 8192, 1 << 20, (1 << 31) - 1):
+		for m in (0, 1, 2, 63, 64, 65, 1000, 8192, 1 << 20, (1 << 31) - 1 - (1 << 17)):
 			for k, n in ((1, 1), (7, 5), (64, 64), (1000, 2048), (8192, 8192)):
 				desc = lib.LinearDesc(dtype, 0, 0, m, n, k, k, n, n, n, n)
 				lib.pz_linear_fwd_workspace_bytes(ctypes.byref(desc), 4096, 4096, ctypes.byref(size))
@@ -168,6 +175,9 @@ def groupnorm_refusals():
 	refused(lambda: dnn.groupNormNd(A(2, 5, 12, dtype=np.int32), s, b, 3), "float32 or float16")
 	refused(lambda: dnn.groupNormNd(x, s, b, 5), "groups")
 	refused(lambda: dnn.groupNormNd(x, s, b, 0), "groups")
+	refused(lambda: dnn.groupNormNd(x, s, b, 2.4), "groups")
+	for epsilon in (-1e-5, float("nan")):
+		refused(lambda: dnn.groupNormNd(x, s, b, 3, epsilon=epsilon), "epsilon")
 	refused(lambda: dnn.groupNormNd(x, A(11), b, 3), "scale")
 	refused(lambda: dnn.groupNormNd(x, s, A(12, dtype=np.float16), 3), "bias")
 	refused(lambda: dnn.groupNormNd(x[:, :, :6], A(6), A(6), 3), "contiguous")
@@ -210,6 +220,11 @@ def matrix_kernels_keep_apart():
 	ready = lazy.foreignBegin(stream, mark)
 	assert ready is not mark
 	assert lazy.foreignBegin(stream, mark) is mark
+	# ... on whichever stream: the older mark alone would let it run beside the product
+	other = bnd.Driver.Stream()
+	lib.trace.clear()
+	assert lazy.foreignBegin(other, mark) is mark
+	assert [n for n, _ in lib.trace].count("pz_stream_wait_event") == 2, lib.trace           # the product's event, then the mark
 	lib.trace.clear()
 	bnd.blas.linear(A(8, 16), A(16, 8))                                    # float32: no such order
 	assert "pz_stream_wait_event" not in [n for n, _ in lib.trace]

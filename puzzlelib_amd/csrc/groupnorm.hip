@@ -350,9 +350,8 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 	__syncthreads();
 	for (int i = 0; i < 2; ++i) sum_cells<NT>(red[i], s.tx * V, TY, s.reps, g.c, 1, channels, 1.f, chan[i]);
 	__syncthreads();
-	if (sums)
-		for (int i = threadIdx.x; i < 2 * channels; i += NT)
-			sums[(((size_t)sample * s.chunks + chunk) * 2 + i / channels) * g.c + c0 + i % channels] = chan[i / channels][i % channels];
+	for (int i = threadIdx.x; i < 2 * channels; i += NT)
+		sums[(((size_t)sample * s.chunks + chunk) * 2 + i / channels) * g.c + c0 + i % channels] = chan[i / channels][i % channels];
 	if (!FINISH) return;
 
 	__syncthreads();
@@ -384,26 +383,37 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 	}
 }
 
-// A and B of the head, divided by m, of a (sample, group) from its chunks' channel sums: a workgroup each
-__global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, const float *sums, float2 *ab) {
-	__shared__ double part[2][4];
+// The chunks' channel sums of a (sample, group), a workgroup each: added in a fixed order in float64 into totals[(sample * 2 + {0, 1}) * c +
+// channel] (what norm_param_kernel reads: a row per sample instead of one per chunk), and with `scale` into A and B of the head,
+// divided by m. 16 channels at a time, 16 chunks side by side.
+__global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, const float *sums, float *totals, float2 *ab) {
+	__shared__ double part[2][16][17];
 	const long at = blockIdx.x, sample = at / g.groups;
-	const int c0 = (int)(at % g.groups) * g.width;
-	double a = 0.0, b = 0.0;
+	const int c0 = (int)(at - sample * g.groups) * g.width, lane = threadIdx.x & 15, row = threadIdx.x >> 4;
+	double a = 0.0, b = 0.0;                                                    // (of lane's channels, in the threads of row 0)
+	for (int strip = 0; strip < g.width; strip += 16) {
+		const bool mine = strip + lane < g.width;
+		const int ch = c0 + strip + lane;
+		double p0 = 0.0, p1 = 0.0;
+		if (mine) {
+			const float *p = sums + ((size_t)sample * s.chunks + row) * 2 * g.c + ch;
 #pragma unroll 4
-	for (int i = threadIdx.x; i < s.chunks * g.width; i += 256) {
-		const int chunk = i / g.width, ch = c0 + i - chunk * g.width;
-		const float *p = sums + ((size_t)sample * s.chunks + chunk) * 2 * g.c + ch;
-		const double f = or_else(g.scale, ch, 1.f);
-		a += f * p[0], b += f * p[g.c];
+			for (int chunk = row; chunk < s.chunks; chunk += 16, p += (size_t)32 * g.c) p0 += p[0], p1 += p[g.c];
+		}
+		part[0][row][lane] = p0, part[1][row][lane] = p1;
+		__syncthreads();
+		if (row == 0 && mine) {
+			for (int r = 1; r < 16; ++r) p0 += part[0][r][lane], p1 += part[1][r][lane];
+			totals[(size_t)sample * 2 * g.c + ch] = (float)p0, totals[((size_t)sample * 2 + 1) * g.c + ch] = (float)p1;
+			const double f = or_else(g.scale, ch, 1.f);
+			a += f * p0, b += f * p1;
+		}
+		__syncthreads();
 	}
-	for (int l = 32; l > 0; l >>= 1) a += __shfl_xor(a, l, 64), b += __shfl_xor(b, l, 64);
-	if ((threadIdx.x & 63) == 0) part[0][threadIdx.x >> 6] = a, part[1][threadIdx.x >> 6] = b;
-	__syncthreads();
-	if (threadIdx.x > 0) return;
+	if (row > 0) return;
+	for (int l = 8; l > 0; l >>= 1) a += __shfl_xor(a, l, 16), b += __shfl_xor(b, l, 16);
 	const double m = (double)g.pixels * g.width;
-	a = part[0][0] + part[0][1] + part[0][2] + part[0][3], b = part[1][0] + part[1][1] + part[1][2] + part[1][3];
-	ab[at] = make_float2((float)(a / m), (float)(b / m));
+	if (lane == 0) ab[at] = make_float2((float)(a / m), (float)(b / m));
 }
 
 template <typename T, int NV, bool UNI>
@@ -528,14 +538,14 @@ __global__ void __launch_bounds__(256) norm_channel_kernel(Norm g, float *sums) 
 	sums[(sample * 2 + 1) * g.c + ch] = (float)s;
 }
 
-// dbias, dscale: the samples' (and chunks') sums, added in a fixed order in float64. A workgroup takes 16 channels, 64 rows at a time.
-__global__ void __launch_bounds__(1024) norm_param_kernel(const float *sums, long rows, int c, float *dscale, float *dbias) {
+// dbias, dscale: the samples' sums, added in a fixed order in float64. A workgroup takes 16 channels, 64 rows at a time.
+__global__ void __launch_bounds__(1024) norm_param_kernel(const float *sums, int rows, int c, float *dscale, float *dbias) {
 	__shared__ double part[2][64][16];
 	const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, ch = blockIdx.x * 16 + lane;
 	double s = 0.0, b = 0.0;
 	if (ch < c) {
 #pragma unroll 4
-		for (long i = row; i < rows; i += 64) {
+		for (int i = row; i < rows; i += 64) {
 			b += sums[(size_t)i * 2 * c + ch];
 			s += sums[((size_t)i * 2 + 1) * c + ch];
 		}
@@ -659,7 +669,9 @@ Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
 	return p;
 }
 
-size_t sum_rows(const pz_groupnorm_desc *d, const Plan &p) { return (size_t)d->n * (p.way == WAY_PLAIN ? 1 : p.slab.chunks); }
+// the backward pass's workspace: channel sums per sample, per chunk of a sample with WAY_CHUNKS, then A and B of the head
+size_t total_bytes(const pz_groupnorm_desc *d) { return (size_t)d->n * 2 * d->c * sizeof(float); }
+size_t chunk_bytes(const pz_groupnorm_desc *d, const Plan &p) { return p.way == WAY_CHUNKS ? total_bytes(d) * p.slab.chunks : 0; }
 
 template <typename T, int NT, int NV, bool UNI, bool FINISH>
 void slab_fwd(const Norm &g, const Plan &p, float2 *part, hipStream_t st) {
@@ -711,14 +723,13 @@ void slab_bwd(const Norm &g, const Plan &p, float *sums, hipStream_t st) {
 }
 
 template <typename T>
-int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, hipStream_t st) {
-	const Plan p = plan_norm(d, true);
+int backward(const pz_groupnorm_desc *d, const Norm &g, const Plan &p, float *sums, hipStream_t st) {
+	float *chunks = (float *)((char *)sums + total_bytes(d));
+	float2 *ab = (float2 *)((char *)chunks + chunk_bytes(d, p));
 	PZ_REQUIRE(p.way == WAY_ONE || launchable((long)d->n * d->groups, 256), "pz_groupnorm_bwd: too many workgroups");
 	if (p.way == WAY_PLAIN) {
-		if (sums) {
-			norm_channel_kernel<T><<<pz::ceil_div((long)d->n * d->c, 256), 256, 0, st>>>(g, sums);
-			PZ_LAUNCH_CHECK();
-		}
+		norm_channel_kernel<T><<<pz::ceil_div((long)d->n * d->c, 256), 256, 0, st>>>(g, sums);
+		PZ_LAUNCH_CHECK();
 		norm_bwd_kernel<T><<<d->n * d->groups, 256, 0, st>>>(g);
 		PZ_LAUNCH_CHECK();
 		return PZ_OK;
@@ -736,14 +747,14 @@ int backward(const pz_groupnorm_desc *d, const Norm &g, float *sums, char *ws, h
 		return PZ_OK;
 	}
 	PZ_REQUIRE(launchable((long)d->n * p.apply.chunks, 256), "pz_groupnorm_bwd: too many workgroups");
-	if (p.slab.uniform) slab_bwd<T, 256, 8, true, false>(g, p, sums, st);
-	else slab_bwd<T, 256, 8, false, false>(g, p, sums, st);
+	if (p.slab.uniform) slab_bwd<T, 256, 8, true, false>(g, p, chunks, st);
+	else slab_bwd<T, 256, 8, false, false>(g, p, chunks, st);
 	PZ_LAUNCH_CHECK();
-	norm_join_bwd_kernel<<<(unsigned)((long)d->n * d->groups), 256, 0, st>>>(g, p.slab, sums, (float2 *)ws);
+	norm_join_bwd_kernel<<<(unsigned)((long)d->n * d->groups), 256, 0, st>>>(g, p.slab, chunks, sums, ab);
 	PZ_LAUNCH_CHECK();
 	const unsigned blocks = (unsigned)((long)d->n * p.apply.chunks);
-	if (p.apply.uniform) norm_apply_bwd_kernel<T, 8, true><<<blocks, 256, 0, st>>>(g, p.apply, (const float2 *)ws);
-	else norm_apply_bwd_kernel<T, 8, false><<<blocks, 256, 0, st>>>(g, p.apply, (const float2 *)ws);
+	if (p.apply.uniform) norm_apply_bwd_kernel<T, 8, true><<<blocks, 256, 0, st>>>(g, p.apply, ab);
+	else norm_apply_bwd_kernel<T, 8, false><<<blocks, 256, 0, st>>>(g, p.apply, ab);
 	PZ_LAUNCH_CHECK();
 	return PZ_OK;
 }
@@ -756,7 +767,7 @@ int pz_groupnorm_workspace_bytes(const pz_groupnorm_desc *d, int backward, size_
 	if (int rc = check(d, "pz_groupnorm_workspace_bytes")) return rc;
 	PZ_REQUIRE(nbytes, "pz_groupnorm_workspace_bytes: null output");
 	const Plan p = plan_norm(d, backward != 0);
-	*nbytes = backward ? sum_rows(d, p) * 2 * d->c * sizeof(float) + p.stat_bytes : p.part_bytes + p.stat_bytes;
+	*nbytes = backward ? total_bytes(d) + chunk_bytes(d, p) + p.stat_bytes : p.part_bytes + p.stat_bytes;
 	return PZ_OK;
 }
 
@@ -787,13 +798,10 @@ int pz_groupnorm_bwd(const pz_groupnorm_desc *d, const void *dy, const void *x, 
 	g.x = x, g.dy = dy, g.out = dx, g.scale = scale, g.bias = bias, g.mean = (float *)savemean, g.invvar = (float *)saveinvvar;
 	const Plan p = plan_norm(d, true);
 	float *sums = (float *)workspace;
-	const size_t rows = empty ? 0 : sum_rows(d, p);
-	if (!empty) {
-		char *ws = (char *)workspace + rows * 2 * d->c * sizeof(float);
-		if (int rc = d->dtype == PZ_F16 ? backward<f16>(d, g, sums, ws, st) : backward<float>(d, g, sums, ws, st)) return rc;
-	}
+	if (!empty)
+		if (int rc = d->dtype == PZ_F16 ? backward<f16>(d, g, p, sums, st) : backward<float>(d, g, p, sums, st)) return rc;
 	if (dscale || dbias) {
-		norm_param_kernel<<<pz::ceil_div(d->c, 16), 1024, 0, st>>>(sums, (long)rows, d->c, dscale, dbias);
+		norm_param_kernel<<<pz::ceil_div(d->c, 16), 1024, 0, st>>>(sums, empty ? 0 : d->n, d->c, dscale, dbias);
 		PZ_LAUNCH_CHECK();
 	}
 	return PZ_OK;

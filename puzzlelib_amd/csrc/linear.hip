@@ -597,14 +597,19 @@ Plan plan_product(int dtype, const Operands &o) {
 	const int size = dtype == PZ_F16 ? 2 : 4;
 	p.bk = dtype == PZ_F16 ? kSteps<f16> : kSteps<float>;
 	p.bm = o.m > 64 ? 128 : 64, p.bn = o.n > 64 ? 128 : 64;
+	// narrower tiles where square ones give a CU one workgroup at most (2048^3: float16 33 -> 30 us, float32 147 -> 137; 4096 x 512 x 512
+	// 23 -> 13), or half of one where the reduction runs over rows (dW of 2048 x 1024 x 4096: 65 us both ways instead of 69)
+	if (p.bm == 128 && (long)pz::ceil_div(o.m, 128) * pz::ceil_div(o.n, 128) <= pz::kNumCU / (o.ta ? 2 : 1)) p.bn = 64;
 	const long tiles256 = (long)pz::ceil_div(o.m, 256) * pz::ceil_div(o.n, 256);
 	if (o.k >= (dtype == PZ_F16 ? 256 : 1024) && tiles256 >= pz::kNumCU) p.bm = p.bn = 256;
 	p.tiles_m = pz::ceil_div(o.m, p.bm), p.tiles_n = pz::ceil_div(o.n, p.bn);
 	const long tiles = (long)p.tiles_m * p.tiles_n;
-	const int ksteps = pz::ceil_div(o.k, p.bk), least = 128 / p.bk;      // a split keeps 128 steps at least
+	// k is split until every CU has a workgroup: two each cost more in slabs than they hide (1 x 4096 x 16384 32 against 29 us), and a split
+	// keeps four steps of the loop (two, in float16: 46 against 30 us for the backward pass of 256 x 2048 x 1000)
+	const int ksteps = pz::ceil_div(o.k, p.bk), least = 4;
 	int splits = 1;
 	if (tiles < pz::kNumCU) {
-		splits = (int)(2 * pz::kNumCU / tiles);
+		splits = (int)(pz::kNumCU / tiles);
 		splits = splits > ksteps / least ? ksteps / least : splits;
 		splits = splits < 1 ? 1 : splits > 64 ? 64 : splits;
 	}

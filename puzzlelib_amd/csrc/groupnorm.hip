@@ -116,7 +116,7 @@ __device__ void sum_cells(const float *red, int across, int rows, int reps, int 
 	}
 }
 
-// scale and bias (1 and 0 where there are none) of V channels from `first` on (UNI), or of the channels ch(e)
+// scale or bias (`none` where there is none) of V channels from `first` on
 template <int V>
 __device__ __forceinline__ void load_floats(const float *p, int first, float none, float (&v)[V]) {
 	typedef float vec __attribute__((ext_vector_type(4), aligned(4)));
@@ -149,6 +149,9 @@ __device__ __forceinline__ void each_channel(int first, int c, int width, F f) {
 constexpr int kMaxWidth = 2048;                  // values of a row of a slab
 
 // ---- forward: statistics, and with FINISH the normalised values, from one read ---------------------------------------------------------
+// Two passes over registers cost less than one with a running mean, and the centred sum loses nothing. 32 x 4096 x 512 float16 with SiLU:
+// 82 us (3.3 TB/s): a CU holds one workgroup of 256 KiB, whose loads and stores do not overlap; chunks that are read twice take 90.
+// 128 x 1 x 2048: one wave a slab, 7 us.
 // PART (FINISH = false): {mean, sum of centred squares} of the chunk's groups, for norm_join_kernel.
 template <typename T, int NT, int NV, bool UNI, bool FINISH>
 __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *part) {
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(256) norm_join_kernel(Norm g, Slab s, const fl
 	if (lane == 0) mean[at] = (float)m, invvar[at] = (float)(1.0 / sqrt(q + (double)g.epsilon));
 }
 
-// y from x and the statistics, a chunk of rows back to back
+// y from x and the statistics, a chunk of rows back to back, bound by memory
 template <typename T, int NV, bool UNI>
 __global__ void __launch_bounds__(256) norm_apply_kernel(Norm g, Slab s, const float *means, const float *invvars) {
 	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
@@ -299,7 +302,7 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(Norm g, Slab s, const f
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------------
 // Sums over a chunk's pixels per channel, sums[((sample * chunks + chunk) * 2 + {0: da, 1: da xhat}) * c + channel], and with FINISH dx from
-// the same registers.
+// the same registers. 64 x 1024 x 512 float16 with SiLU: 78 us (2.6 TB/s), two workgroups of 128 KiB a CU; chunks take 88.
 template <typename T, int NT, int NV, bool UNI, bool FINISH>
 __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float *sums) {
 	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
@@ -385,7 +388,8 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 
 // The chunks' channel sums of a (sample, group), a workgroup each: added in a fixed order in float64 into totals[(sample * 2 + {0, 1}) * c +
 // channel] (what norm_param_kernel reads: a row per sample instead of one per chunk), and with `scale` into A and B of the head,
-// divided by m. 16 channels at a time, 16 chunks side by side.
+// divided by m. 16 channels at a time, 16 chunks side by side (16 x 4096 x 256 float32, 128 chunks a sample: with it the backward pass takes
+// 73 us; the parameters' kernel reading a row per chunk 85).
 __global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, const float *sums, float *totals, float2 *ab) {
 	__shared__ double part[2][16][17];
 	const long at = blockIdx.x, sample = at / g.groups;
@@ -459,7 +463,7 @@ __global__ void __launch_bounds__(256) norm_apply_bwd_kernel(Norm g, Slab s, con
 
 // ---- any shape: one workgroup per (sample, group), three sweeps over its values ----------------------------------------------------------
 // Threads take consecutive channels of consecutive pixels. Only rows that no workgroup holds come here (more than kMaxWidth values in a
-// group, or a channel count whose vectors repeat later than that).
+// group, or a channel count whose vectors repeat later than that). Kept simple: it reads x three times.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_fwd_kernel(Norm g) {
 	__shared__ float red[16];
@@ -538,7 +542,8 @@ __global__ void __launch_bounds__(256) norm_channel_kernel(Norm g, float *sums) 
 	sums[(sample * 2 + 1) * g.c + ch] = (float)s;
 }
 
-// dbias, dscale: the samples' sums, added in a fixed order in float64. A workgroup takes 16 channels, 64 rows at a time.
+// dbias, dscale: the samples' sums, added in a fixed order in float64. A workgroup takes 16 channels, 64 rows at a time:
+// 64 samples of 512 channels 4 us.
 __global__ void __launch_bounds__(1024) norm_param_kernel(const float *sums, int rows, int c, float *dscale, float *dbias) {
 	__shared__ double part[2][64][16];
 	const int lane = threadIdx.x & 15, row = threadIdx.x >> 4, ch = blockIdx.x * 16 + lane;

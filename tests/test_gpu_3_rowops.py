@@ -47,17 +47,21 @@ def slope(z, name):
 	return np.ones_like(z)
 
 
-def words(seed, call, count):
-	"""Philox4x32-10 in numpy: the words of call `call`"""
+def wordsFrom(seed, call, quad, quads):
+	"""Philox4x32-10 in numpy: the words of call `call` from word 4 * quad on"""
 	mask = np.uint64(0xffffffff)
-	q = np.arange((count + 3) // 4, dtype=np.uint64)
+	q = np.arange(quad, quad + quads, dtype=np.uint64)
 	c = [q & mask, q >> np.uint64(32), np.full_like(q, call & 0xffffffff), np.full_like(q, call >> 32)]
 	k = [seed & 0xffffffff, seed >> 32]
 	for _ in range(10):
 		a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
 		c = [(b >> np.uint64(32)) ^ c[1] ^ np.uint64(k[0]), b & mask, (a >> np.uint64(32)) ^ c[3] ^ np.uint64(k[1]), a & mask]
 		k = [(k[0] + 0x9E3779B9) & 0xffffffff, (k[1] + 0xBB67AE85) & 0xffffffff]
-	return np.stack(c, axis=1).reshape(-1)[:count]
+	return np.stack(c, axis=1).reshape(-1)
+
+
+def words(seed, call, count):
+	return wordsFrom(seed, call, 0, (count + 3) // 4)[:count]
 
 
 def keep(mask, shape):
@@ -576,3 +580,104 @@ def test_feed_forward_block(bnd, dtype):
 							(db, DU.sum(axis=(0, 1)).reshape(-1), "dbias")):
 		err = np.linalg.norm(got.get().astype(np.float64) - want) / np.linalg.norm(want)
 		assert err <= tol, "%s: relative error %.3g" % (what, err)
+
+
+# ------------------------------------------------------------------------------------------------ places beyond 32 bits
+def put(buf, pitch, col, rows):
+	"""rows -> columns col ... of a flat buffer whose rows stand `pitch` apart, one by one (strided copies take 4-byte types only)"""
+	for i, row in enumerate(rows):
+		buf[i * pitch + col:i * pitch + col + row.size].set(row)
+
+
+def take(buf, pitch, col, m, n):
+	return np.stack([buf[i * pitch + col:i * pitch + col + n].get() for i in range(m)])
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_linear_rows_beyond_32_bits(bnd, dtype):
+	"""x, W, residual, out and pre-activation as columns of one buffer of more than 2^32 bytes (float16: more than 2^31 elements)"""
+	m, k, n = 290, 290, 72
+	pitch = (16 << 20) // np.dtype(dtype).itemsize
+	rng = np.random.RandomState(21)
+	x, W, r = rng.randn(m, k).astype(dtype), (rng.randn(k, n) / 16).astype(dtype), rng.randn(m, n).astype(dtype)
+	buf = bnd.GPUArray.empty((m * pitch, ), dtype=dtype)
+	grid = buf.reshape(m, pitch)
+	cols = dict(x=0, W=1024, r=2048, out=4096, z=pitch - n)
+	for name, ary in (("x", x), ("W", W), ("r", r)):
+		put(buf, pitch, cols[name], ary)
+	view = lambda name, width: grid[:, cols[name]:cols[name] + width]
+	bnd.blas.linear(view("x", k), view("W", n), act=bnd.FusedAct.relu, residual=view("r", n), preact=view("z", n), out=view("out", n))
+	x64, W64, r64 = (a.astype(np.float64) for a in (x, W, r))
+	z = x64 @ W64
+	bound = productBound(x64, W64, k)
+	within(take(buf, pitch, cols["z"], m, n), z, bound, "preact")
+	y = act(z, "relu") + r64
+	within(take(buf, pitch, cols["out"], m, n), y, bound + U32 * np.abs(y), "out")
+	for name, ary in (("x", x), ("W", W), ("r", r)):
+		assert np.array_equal(take(buf, pitch, cols[name], *ary.shape), ary), name
+
+
+def test_counter_dropout_beyond_32_bits(bnd):
+	count = (1 << 32) + 1003
+	mask = bnd.DropoutMask(77, 5, 0.25)
+	rng = np.random.RandomState(22)
+	buf = bnd.GPUArray.empty((count, ), dtype=np.float16)
+	spots = [0, (1 << 30) - 500, (1 << 31) - 500, (1 << 32) - 500, count - 500]
+	x = [rng.randn(500).astype(np.float16) for _ in spots]
+	for at, v in zip(spots, x):
+		buf[at:at + 500].set(v)
+	bnd.counterDropoutKer(np.float16)(buf, buf, mask)
+	for at, v in zip(spots, x):
+		first = at // 4 * 4
+		q = wordsFrom(mask.seed, mask.call, first // 4, 128)[at - first:at - first + 500]
+		want = np.where(q < mask.key.threshold, v.astype(np.float64) / 0.75, 0.0)
+		got = buf[at:at + 500].get()
+		within(got, want, 3 * U32 * np.abs(want), "at %d" % at)
+		assert np.array_equal(got == 0, want == 0), "the mask at %d" % at
+
+
+def test_groupnorm_beyond_32_bits(bnd):
+	"""3 x 3000001 x 256 float16 (2.3e9 elements) whose channels alternate between 2 and 1: mean 1.5, variance 1/4 in every group"""
+	shape, groups, epsilon = (3, 3000001, 256), 2, 1e-5
+	x = bnd.GPUArray.empty(shape, dtype=np.float16)
+	x.gpudata.fillD32(0x3c004000)                                   # 2.0 in the low half
+	scale, bias = gpu(bnd, np.full(256, 1.0, np.float32)), gpu(bnd, np.full(256, 0.25, np.float32))
+	y, mean, inv = bnd.dnn.groupNormNd(x, scale, bias, groups, epsilon=epsilon)
+	iv = 1.0 / np.sqrt(0.25 + epsilon)
+	# a chunk's sums pass fewer than 64 additions one after the other, the chunks are joined in 64 bits
+	within(mean.get(), np.full((3, groups), 1.5), 64 * U32 * 1.5, "mean")
+	within(inv.get(), np.full((3, groups), iv), 64 * U32 * iv, "invvar")
+	xhat = np.tile([0.5 * iv, -0.5 * iv], 128)
+	spots = [0, (1 << 30) // 256 - 2, (1 << 31) // 256 - 2, 3 * 3000001 - 4]
+	rows = lambda a: [a.reshape(-1, 256)[at:at + 4].get() for at in spots]
+	for got in rows(y):
+		within(got, np.tile(xhat + 0.25, (4, 1)), 200 * U32, "y")
+	g = y
+	g.gpudata.fillD32(0x38003c00)                                   # 1.0 in the low half, 0.5 in the high one
+	dx, dscale, dbias = bnd.dnn.groupNormNdBackward(g, x, scale, bias, mean, inv, groups)
+	d = np.tile([1.0, 0.5], 128)
+	count = 3.0 * 3000001
+	within(dbias.get(), count * d, 64 * U32 * count * d, "dbias")
+	within(dscale.get(), count * d * xhat, 200 * U32 * count * d, "dscale")
+	want = iv * (d - 0.75 - xhat * (d * xhat).mean())                # (nearly nothing: the terms cancel)
+	for got in rows(dx):
+		within(got, np.tile(want, (4, 1)), iv * 200 * U32 * 2.0, "dx")
+
+
+def test_dropout_on_a_stream_then_a_product(bnd):
+	"""a mask applied on a borrowed stream, a float16 product that reads it, the stream again: each waits for the other"""
+	rng = np.random.RandomState(23)
+	x, W = rng.randn(512, 256).astype(np.float16), (rng.randn(256, 512) / 16).astype(np.float16)
+	gx, gW = gpu(bnd, x), gpu(bnd, W)
+	ker = bnd.counterDropoutKer(np.float16)
+	stream = bnd.Driver.Stream()
+	for call in range(3):
+		one, two = bnd.DropoutMask(9, 2 * call, 0.5), bnd.DropoutMask(9, 2 * call + 1, 0.5)
+		h, out = bnd.GPUArray.empty(x.shape, dtype=np.float16), bnd.GPUArray.empty((512, 512), dtype=np.float16)
+		ker(h, gx, one, stream=stream)
+		y = bnd.blas.linear(h, gW)
+		ker(out, y, two, stream=stream)
+		dropped = x.astype(np.float64) * keep(one, x.shape)
+		within(h.get(), dropped, 3 * U32 * np.abs(dropped), "h")
+		within(y.get(), dropped @ W, productBound(dropped, W.astype(np.float64), 256), "y")
+		assert np.array_equal(out.get(), (y.get() * keep(two, (512, 512))).astype(np.float16))

@@ -232,14 +232,16 @@ __global__ void __launch_bounds__(NT) norm_slab_kernel(Norm g, Slab s, float2 *p
 		scale[e] *= sinv[group];
 	});
 	T *y = (T *)g.out + start;
+	with_act(g.act, [&](auto act) {
 #pragma unroll
-	for (int k = 0; k < NV; ++k) {
-		if (k >= mine) continue;
-		float o[V];
+		for (int k = 0; k < NV; ++k) {
+			if (k >= mine) continue;
+			float o[V];
 #pragma unroll
-		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], g.act);
-		store_vec(y + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last, o);
-	}
+			for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], act);
+			store_vec(y + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last, o);
+		}
+	});
 }
 
 // mean and 1 / sqrt(var + epsilon) of a (sample, group) from its chunks' {mean, centred squares}: a wave each, float64 sums
@@ -290,21 +292,24 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(Norm g, Slab s, const f
 		if (!UNI) scale[e] = or_else(g.scale, ch, 1.f), bias[e] = or_else(g.bias, ch, 0.f);
 		scale[e] *= inv;
 	});
+	with_act(g.act, [&](auto act) {
 #pragma unroll
-	for (int k = 0; k < NV; ++k) {
-		if (k >= mine) continue;
-		float o[V];
+		for (int k = 0; k < NV; ++k) {
+			if (k >= mine) continue;
+			float o[V];
 #pragma unroll
-		for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], g.act);
-		store_vec(y + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last, o);
-	}
+			for (int e = 0; e < V; ++e) o[e] = act_value(((float)v[k][e] - mean[UNI ? 0 : e]) * scale[e] + bias[e], act);
+			store_vec(y + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last, o);
+		}
+	});
 }
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------------
 // Sums over a chunk's pixels per channel, sums[((sample * chunks + chunk) * 2 + {0: da, 1: da xhat}) * c + channel], and with FINISH dx from
 // the same registers. 64 x 1024 x 512 float16 with SiLU: 78 us (2.6 TB/s), two workgroups of 128 KiB a CU; chunks take 88.
+// (512 threads: 128 registers, so that a CU holds two workgroups; 134 would leave one: 89 us)
 template <typename T, int NT, int NV, bool UNI, bool FINISH>
-__global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float *sums) {
+__global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) norm_slab_bwd_kernel(Norm g, Slab s, float *sums) {
 	constexpr int V = Vec<T>::V, CELLS = UNI ? 1 : V;
 	__shared__ float red[2][NT * V];
 	__shared__ float chan[2][NT * V < kMaxWidth ? NT * V : kMaxWidth];      // (a row has NT vectors at most)
@@ -336,16 +341,18 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 		if (!UNI) scale[e] = or_else(g.scale, c0 + ch, 1.f), bias[e] = or_else(g.bias, c0 + ch, 0.f);
 		da[e] = db[e] = 0.f;
 	});
+	with_act(g.act, [&](auto act) {
 #pragma unroll
-	for (int k = 0; k < NV; ++k) {
-		if (k >= mine) continue;
+		for (int k = 0; k < NV; ++k) {
+			if (k >= mine) continue;
 #pragma unroll
-		for (int e = 0; e < V; ++e) {
-			const float xhat = ((float)v[k][e] - mean[UNI ? 0 : e]) * inv[UNI ? 0 : e];
-			const float t = (float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act);
-			da[e] += t, db[e] += t * xhat;
+			for (int e = 0; e < V; ++e) {
+				const float xhat = ((float)v[k][e] - mean[UNI ? 0 : e]) * inv[UNI ? 0 : e];
+				const float t = (float)d[k][e] * act_slope(scale[e] * xhat + bias[e], act);
+				da[e] += t, db[e] += t * xhat;
+			}
 		}
-	}
+	});
 	if (ty < TY) {
 #pragma unroll
 		for (int e = 0; e < V; ++e) red[0][(ty * s.tx + tx) * V + e] = da[e], red[1][(ty * s.tx + tx) * V + e] = db[e];
@@ -371,19 +378,21 @@ __global__ void __launch_bounds__(NT) norm_slab_bwd_kernel(Norm g, Slab s, float
 	float a[CELLS], b[CELLS];
 	each_channel<CELLS, UNI>(tx * V, g.c, g.width, [&](int e, int, int group) { a[e] = sa[group], b[e] = sb[group]; });
 	T *dx = (T *)g.out + start;
+	with_act(g.act, [&](auto act) {
 #pragma unroll
-	for (int k = 0; k < NV; ++k) {
-		if (k >= mine) continue;
-		float o[V];
+		for (int k = 0; k < NV; ++k) {
+			if (k >= mine) continue;
+			float o[V];
 #pragma unroll
-		for (int e = 0; e < V; ++e) {
-			const int u = UNI ? 0 : e;
-			const float xhat = ((float)v[k][e] - mean[u]) * inv[u];
-			const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act));
-			o[e] = inv[u] * (t - a[u] - xhat * b[u]);
+			for (int e = 0; e < V; ++e) {
+				const int u = UNI ? 0 : e;
+				const float xhat = ((float)v[k][e] - mean[u]) * inv[u];
+				const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], act));
+				o[e] = inv[u] * (t - a[u] - xhat * b[u]);
+			}
+			store_vec(dx + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last, o);
 		}
-		store_vec(dx + (ty + k * TY) * (size_t)s.pitch + tx * V, k + 1 < mine ? V : last, o);
-	}
+	});
 }
 
 // The chunks' channel sums of a (sample, group), a workgroup each: added in a fixed order in float64 into totals[(sample * 2 + {0, 1}) * c +
@@ -446,19 +455,21 @@ __global__ void __launch_bounds__(256) norm_apply_bwd_kernel(Norm g, Slab s, con
 		if (!UNI || e == 0) mean[UNI ? 0 : e] = g.mean[at], inv[UNI ? 0 : e] = g.invvar[at], sum[UNI ? 0 : e] = ab[at];
 		if (!UNI) scale[e] = or_else(g.scale, ch, 1.f), bias[e] = or_else(g.bias, ch, 0.f);
 	});
+	with_act(g.act, [&](auto act) {
 #pragma unroll
-	for (int k = 0; k < NV; ++k) {
-		if (k >= mine) continue;
-		float o[V];
+		for (int k = 0; k < NV; ++k) {
+			if (k >= mine) continue;
+			float o[V];
 #pragma unroll
-		for (int e = 0; e < V; ++e) {
-			const int u = UNI ? 0 : e;
-			const float xhat = ((float)v[k][e] - mean[u]) * inv[u];
-			const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], g.act));
-			o[e] = inv[u] * (t - sum[u].x - xhat * sum[u].y);
+			for (int e = 0; e < V; ++e) {
+				const int u = UNI ? 0 : e;
+				const float xhat = ((float)v[k][e] - mean[u]) * inv[u];
+				const float t = scale[e] * ((float)d[k][e] * act_slope(scale[e] * xhat + bias[e], act));
+				o[e] = inv[u] * (t - sum[u].x - xhat * sum[u].y);
+			}
+			store_vec(dx + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last, o);
 		}
-		store_vec(dx + (size_t)k * s.ty * s.pitch, k + 1 < mine ? V : last, o);
-	}
+	});
 }
 
 // ---- any shape: one workgroup per (sample, group), three sweeps over its values ----------------------------------------------------------

@@ -8,8 +8,6 @@
 #include "philox.h"
 #include "rows.h"
 
-#include <type_traits>
-
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __fp16 tr16x4 __attribute__((ext_vector_type(4)));
@@ -51,10 +49,10 @@ __device__ __forceinline__ void finish(const Epilogue &e, float (&s)[COUNT], con
 #pragma unroll
 	for (int i = 0; i < COUNT; ++i) s[i] += bias[i];
 	if (e.preact) store_preact(s);
-	if (e.act != PZ_ACT_NONE) {
+	with_act(e.act, [&](auto act) {
 #pragma unroll
-		for (int i = 0; i < COUNT; ++i) s[i] = act_value(s[i], e.act);
-	}
+		for (int i = 0; i < COUNT; ++i) s[i] = act_value(s[i], act);
+	});
 	if (e.dropping) {
 		const unsigned bits = drop_bits<COUNT>(e.drop, index);
 #pragma unroll
@@ -539,8 +537,10 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 			if (g.act != PZ_ACT_NONE) {
 				float z[COUNT];
 				load_run((const T *)g.preact + (size_t)row * g.ldp + col, whole, left, z);
+				with_act(g.act, [&](auto act) {
 #pragma unroll
-				for (int e = 0; e < COUNT; ++e) d[e] *= act_slope(z[e], g.act);
+					for (int e = 0; e < COUNT; ++e) d[e] *= act_slope(z[e], act);
+				});
 			}
 			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)
 #pragma unroll

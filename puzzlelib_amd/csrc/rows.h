@@ -3,6 +3,8 @@
 #pragma once
 #include "common.h"
 
+#include <type_traits>
+
 typedef _Float16 f16;
 
 namespace {
@@ -51,6 +53,16 @@ __device__ __forceinline__ float act_slope(float z, int act) {
 		return s * fmaf(z, 1.f - s, 1.f);
 	}
 	return 1.f;
+}
+
+// f(activation as a constant): the choice once in front of a loop. Left inside, a branch per value keeps the values' chains from overlapping (group norm
+// backward, 64 x 1024 x 512 float16 with SiLU: 80 instead of 71 us; linear 8192 x 2048 x 8192 with GELU 320 instead of 306).
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+	if (act == PZ_ACT_NONE) f(std::integral_constant<int, PZ_ACT_NONE>{});
+	else if (act == PZ_ACT_RELU) f(std::integral_constant<int, PZ_ACT_RELU>{});
+	else if (act == PZ_ACT_GELU) f(std::integral_constant<int, PZ_ACT_GELU>{});
+	else f(std::integral_constant<int, PZ_ACT_SILU>{});
 }
 
 // ---- COUNT consecutive values of a row, float32 in registers ----------------------------------------------------------------------

@@ -150,7 +150,7 @@ constexpr int kMaxWidth = 2048;                  // values of a row of a slab
 
 // ---- forward: statistics, and with FINISH the normalised values, from one read ---------------------------------------------------------
 // Two passes over registers cost less than one with a running mean, and the centred sum loses nothing. 32 x 4096 x 512 float16 with SiLU:
-// 82 us (3.3 TB/s): a CU holds one workgroup of 256 KiB, whose loads and stores do not overlap; chunks that are read twice take 90.
+// 79 us (3.4 TB/s): a CU holds one workgroup of 256 KiB, whose loads and stores do not overlap; chunks that are read twice take 90.
 // 128 x 1 x 2048: one wave a slab, 7 us.
 // PART (FINISH = false): {mean, sum of centred squares} of the chunk's groups, for norm_join_kernel.
 template <typename T, int NT, int NV, bool UNI, bool FINISH>
@@ -306,7 +306,7 @@ __global__ void __launch_bounds__(256) norm_apply_kernel(Norm g, Slab s, const f
 
 // ---- backward ---------------------------------------------------------------------------------------------------------------------------
 // Sums over a chunk's pixels per channel, sums[((sample * chunks + chunk) * 2 + {0: da, 1: da xhat}) * c + channel], and with FINISH dx from
-// the same registers. 64 x 1024 x 512 float16 with SiLU: 78 us (2.6 TB/s), two workgroups of 128 KiB a CU; chunks take 88.
+// the same registers. 64 x 1024 x 512 float16 with SiLU: 68 us (3.0 TB/s), two workgroups of 128 KiB a CU; chunks take 84.
 // (512 threads: 128 registers, so that a CU holds two workgroups; 134 would leave one: 89 us)
 template <typename T, int NT, int NV, bool UNI, bool FINISH>
 __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) norm_slab_bwd_kernel(Norm g, Slab s, float *sums) {
@@ -397,8 +397,8 @@ __global__ void __launch_bounds__(NT, NT == 512 ? 4 : 1) norm_slab_bwd_kernel(No
 
 // The chunks' channel sums of a (sample, group), a workgroup each: added in a fixed order in float64 into totals[(sample * 2 + {0, 1}) * c +
 // channel] (what norm_param_kernel reads: a row per sample instead of one per chunk), and with `scale` into A and B of the head,
-// divided by m. 16 channels at a time, 16 chunks side by side (16 x 4096 x 256 float32, 128 chunks a sample: with it the backward pass takes
-// 73 us; the parameters' kernel reading a row per chunk 85).
+// divided by m. 16 channels at a time, 16 chunks side by side (16 x 4096 x 256 float32, 128 chunks a sample: with it the backward pass took
+// 73 us; with the parameters' kernel reading a row per chunk 85).
 __global__ void __launch_bounds__(256) norm_join_bwd_kernel(Norm g, Slab s, const float *sums, float *totals, float2 *ab) {
 	__shared__ double part[2][16][17];
 	const long at = blockIdx.x, sample = at / g.groups;
@@ -651,7 +651,7 @@ Plan plan_norm(const pz_groupnorm_desc *d, bool backward) {
 					for (const int nv : {4, vectors}) {
 						if (nt > (uniform ? most : 256) || (nt == 64 && nv > 4) || tx > nt || (long)(nt / tx) * nv < d->pixels) continue;
 						// few large workgroups leave most of the chip idle: chunks, although they read twice (16 workgroups of 256 KiB: 25 us,
-						// chunks 14)
+						// chunks 20)
 						if (nt > 256 && (long)d->n * (d->c / slab) < pz::kNumCU / 2) continue;
 						p.way = WAY_ONE, p.nt = nt, p.nv = nv;
 						Slab s{};

@@ -330,7 +330,7 @@ __device__ __forceinline__ void multiply_add(f32x4 (&acc)[N], const f32x4 &a, co
 }
 
 // Bound by the matrix pipe: float16 8192 x 8192 x 2048 with dropout and residual 235 us (1170 TFLOP/s), 8192 x 2048 x 8192 with GELU and the
-// kept pre-activation 286 us (960; the epilogue writes 268 MB and evaluates 65536 GELUs a CU), float32 4096^3 with ReLU and residual 960 us
+// kept pre-activation 275 us (1000; the epilogue writes 268 MB and evaluates 65536 GELUs a CU), float32 4096^3 with ReLU and residual 958 us
 // (143 TFLOP/s). Single rows are bound by the weights: 1 x 4096 x 16384 float16 23-25 us (5.4 TB/s), then the join.
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB>
 __global__ void __launch_bounds__(64 * WM * WN) linear_kernel(Product g) {

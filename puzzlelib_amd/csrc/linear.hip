@@ -529,11 +529,6 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 		for (int row = row0 + wave; row < row1; row += 4) {
 			float d[COUNT];
 			load_run((const T *)g.dy + (size_t)row * g.lddy + col, whole, left, d);
-			if (g.dropping) {
-				const unsigned bits = drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col);
-#pragma unroll
-				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] * g.inv_keep : 0.f;
-			}
 			if (g.act != PZ_ACT_NONE) {
 				float z[COUNT];
 				load_run((const T *)g.preact + (size_t)row * g.ldp + col, whole, left, z);
@@ -541,6 +536,11 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 #pragma unroll
 					for (int e = 0; e < COUNT; ++e) d[e] *= act_slope(z[e], act);
 				});
+			}
+			if (g.dropping) {                                            // (last: nothing comes through a dropped element, whatever dy and z hold)
+				const unsigned bits = drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col);
+#pragma unroll
+				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] * g.inv_keep : 0.f;
 			}
 			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)
 #pragma unroll

@@ -501,13 +501,22 @@ __global__ void __launch_bounds__(256) linear_align_kernel(Aligned a, Aligned b,
 }
 
 // ---- dz = dy * keep / (1 - p) * act'(z), and partial column sums -----------------------------------------------------------------------
+// dz is held in the operands' type, the only one that the matrix instructions of the two products take at their full rate; db sums it before
+// that rounding. In float16 it is held as dz * held_part * (1 - p), which dy's own range always has room for: 1 / (1 - p) and an activation's
+// slope above 1 would take dz = 65504 / (1 - p) * 1.13 to infinity although dx and dW are in range. The products' sums are multiplied by
+// what is missing, in float32. So without an activation nothing is rounded (a dropped dy is dy or zero), and behind one dz carries one
+// rounding: half a step of 2^-11 relative (8192 x 2048 x 8192 with GELU: dx 2.9e-4 off the 64-bit result, root mean square, where 2.1e-4 is
+// the rounding of dx itself), or 2^-25 absolute where it is below 2^-14, as far as dy can be off. A second product with what the rounding
+// left would double the pass: 505 us.
+float held_part(int dtype, int act) { return dtype == PZ_F16 && (act == PZ_ACT_GELU || act == PZ_ACT_SILU) ? 0.875f : 1.f; }      // (slopes up to 1.13)
+
 struct Gate {
 	const void *dy, *preact;
 	void *dz;                        // optional: without it only the sums are made
 	float *sums;                     // [row blocks][n], optional
 	long lddy, ldp, lddz;
 	int m, n, act, dropping, vec, rows_per_block;
-	float inv_keep;
+	float inv_keep, held;            // dz is stored as held * (1 - p) of its value
 	DropKey drop;
 };
 
@@ -540,11 +549,11 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 			if (g.dropping) {                                            // (last: nothing comes through a dropped element, whatever dy and z hold)
 				const unsigned bits = drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col);
 #pragma unroll
-				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] * g.inv_keep : 0.f;
+				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] : 0.f;
 			}
-			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)
 #pragma unroll
-			for (int e = 0; e < COUNT; ++e) sum[e] += d[e];
+			for (int e = 0; e < COUNT; ++e) sum[e] += d[e], d[e] *= g.held;
+			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)
 		}
 	}
 	if (!g.sums) return;
@@ -553,7 +562,7 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 	__syncthreads();
 	for (int i = threadIdx.x; i < 64 * COUNT; i += 256) {
 		const int l = i / COUNT, e = i % COUNT, c = (blockIdx.x * 64 + l) * COUNT + e;
-		if (c < g.n) g.sums[(size_t)blockIdx.y * g.n + c] = part[0][l][e] + part[1][l][e] + part[2][l][e] + part[3][l][e];
+		if (c < g.n) g.sums[(size_t)blockIdx.y * g.n + c] = (part[0][l][e] + part[1][l][e] + part[2][l][e] + part[3][l][e]) * g.inv_keep;
 	}
 }
 
@@ -828,6 +837,7 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 	const void *dz = p.write_dz ? (const void *)ws : dy;
 	const long lddz = p.write_dz ? padded(d->n) : d->ldy;
 	const int wide = p.write_dz ? padded(d->n) : d->n;
+	const float held = held_part(d->dtype, d->act), inv_keep = mask ? 1.f / mask->keep : 1.f;
 	const Operands data = data_operands(d, dz, lddz, wide, w), weight = weight_operands(d, dz, lddz, wide, x);
 	if (int rc = dx ? check_reach(d->dtype, data, "pz_linear_bwd") : PZ_OK) return rc;
 	if (int rc = dw ? check_reach(d->dtype, weight, "pz_linear_bwd") : PZ_OK) return rc;
@@ -839,7 +849,7 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 		g.lddy = d->ldy, g.ldp = d->ldp, g.lddz = lddz;
 		g.m = d->m, g.n = d->n, g.act = d->act, g.dropping = mask != nullptr, g.rows_per_block = p.rows_per_block;
 		g.vec = runs_ok(dy, d->ldy, size) && (d->act == PZ_ACT_NONE || runs_ok(preact, d->ldp, size));
-		g.drop = key_of(mask), g.inv_keep = 1.f / g.drop.keep;
+		g.drop = key_of(mask), g.inv_keep = inv_keep, g.held = held;
 		const dim3 grid((unsigned)pz::ceil_div(d->n, 1024 / size), (unsigned)p.row_blocks);
 		if (d->dtype == PZ_F16) linear_gate_kernel<f16><<<grid, 256, 0, st>>>(g);
 		else linear_gate_kernel<float><<<grid, 256, 0, st>>>(g);
@@ -852,12 +862,12 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
 	ws += p.dz_bytes + p.sum_bytes;
 	if (dx) {
 		Epilogue e{};
-		e.out = dx, e.ldo = d->ldr, e.kind = EPI_ACCUMULATE, e.alpha = 1.f, e.vec = runs_ok(dx, d->ldr, size);
+		e.out = dx, e.ldo = d->ldr, e.kind = EPI_ACCUMULATE, e.alpha = inv_keep / held, e.vec = runs_ok(dx, d->ldr, size);
 		if (int rc = product(d->dtype, data, e, ws, st)) return rc;
 	}
 	if (dw) {
 		Epilogue e{};
-		e.out = dw, e.ldo = d->trans_w ? d->k : d->n, e.kind = EPI_ACCUMULATE, e.alpha = alpha, e.beta = beta, e.out_f32 = dw_dtype == PZ_F32;
+		e.out = dw, e.ldo = d->trans_w ? d->k : d->n, e.kind = EPI_ACCUMULATE, e.alpha = alpha * (inv_keep / held), e.beta = beta, e.out_f32 = dw_dtype == PZ_F32;
 		e.vec = runs_ok(dw, e.ldo, e.out_f32 ? 4 : 2) && (!e.out_f32 || e.ldo % (16 / size) == 0);
 		if (int rc = product(d->dtype, weight, e, ws, st)) return rc;
 	}

@@ -33,3 +33,29 @@ def test_nothing_comes_through_a_dropped_element(bnd, dtype, name):
 
 	for got, want in zip(grads(dy, bad), grads(np.where(dropped, dtype(0), c.dy), z)):
 		assert np.isfinite(want).all() and np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("name,p,top", [("none", 0.875, 65504.0), ("relu", 0.75, 60000.0), ("gelu", 0.0, 65504.0), ("gelu", 0.875, 65504.0), ("silu", 0.5, 65504.0)])
+def test_gradients_at_the_end_of_float16(bnd, name, p, top):
+	"""dz = dy * act' / (1 - p) lies beyond float16, dx and dW do not"""
+	m, k, n = 33, 72, 40
+	c = Case(bnd, np.float16, m, k, n, seed=33)
+	c.dy = (np.sign(c.dy.astype(np.float64)) * top).astype(np.float16)
+	c.W, c.x = (c.W.astype(np.float32) / 512).astype(np.float16), (c.x.astype(np.float32) / 512).astype(np.float16)
+	z = np.full((m, n), 1.5, np.float16)                                         # (slopes 1.128 and 1.04)
+	mask = bnd.DropoutMask(6, 7, p) if p else None
+	kept = keep(mask, (m, n)) * np.ones((m, n))
+	dz = c.dy.astype(np.float64) * kept * slope(z.astype(np.float64), name)
+	assert np.abs(dz).max() > 65504.0
+	dx, dW, db = bnd.blas.linearBackward(
+		gpu(bnd, c.dy), gpu(bnd, c.x), gpu(bnd, c.W), act=bnd.FusedAct[name], preact=gpu(bnd, z), dropout=mask
+	)
+	# without a curved activation dz is dy or zero times one factor: no rounding of its own. Behind one: half a step, and the slope's
+	# own few roundings (exp and two products of values up to 1.13)
+	curved = name in ("gelu", "silu")
+	off = np.abs(dz) * ((2.0 ** -11 if curved else 0.0) + 32 * U32)
+	x64, W64 = c.x.astype(np.float64), c.W.astype(np.float64)
+	assert np.abs(dz @ W64.T).max() < 60000 and np.abs(x64.T @ dz).max() < 60000
+	within(dx.get(), dz @ W64.T, productBound(dz, W64.T, n) + off @ np.abs(W64.T), "dx")
+	within(dW.get(), x64.T @ dz, productBound(x64.T, dz, m) + np.abs(x64.T) @ off, "dW")
+	within(db.get(), dz.sum(axis=0), off.sum(axis=0) + (m + 4) * U32 * np.abs(dz).sum(axis=0), "db")

@@ -248,6 +248,11 @@ struct Stage {
 	}
 	__device__ __forceinline__ static int spot(int r) { return r >> 1 & 7; }
 
+	// a byte offset as the buffer instructions take it. Every row of the operand lies within 32 bits of its tile's start (check_reach); a row
+	// that does not is one behind the last, of which a tile of few rows has many: past every buffer's end, it reads as zeros
+	static constexpr unsigned NOWHERE = 0xfffffff0u;
+	__device__ __forceinline__ static unsigned reached(size_t offset) { return offset < 0xfffff000u ? (unsigned)offset : NOWHERE; }
+
 	long bytes, step;                // what is left of the operand from the next tile on (negative: nothing); advance per tile
 	const char *p;                   // the next tile
 	long shift;                      // from half 0 to half 1
@@ -265,11 +270,11 @@ struct Stage {
 			const int o = ((wave * PIECES + i) * 64 + lane) * 16;                // place in the LDS tile
 			if (KMAJOR) {
 				const int k = o / (ROWS * SIZE), at = o % (ROWS * SIZE) / 16, q = ((at / SIZE) ^ turn(k)) * 16 + at % SIZE * C;
-				off[i] = (unsigned)((size_t)k * ld * SIZE) + (q / RUN * (2 * RUN) + q % RUN) * SIZE;
+				off[i] = reached(((size_t)k * ld + (q / RUN * (2 * RUN) + q % RUN)) * SIZE);
 			} else {
 				const int q = o / 128, piece = (o / 16 % 8) ^ spot(q);
 				kpiece[i] = piece * C;
-				off[i] = (unsigned)((size_t)(q / RUN * (2 * RUN) + q % RUN) * ld * SIZE) + piece * 16;
+				off[i] = reached((size_t)(q / RUN * (2 * RUN) + q % RUN) * ld * SIZE + piece * 16);
 			}
 		}
 	}
@@ -280,7 +285,7 @@ struct Stage {
 		const int high = (int)(left >> 32);                                  // (32-bit tests: they stay in the scalar unit)
 		const unsigned span = high > 0 ? 0xfffff000u : high < 0 ? 0u : min((unsigned)left, 0xfffff000u);
 		const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(p + half * shift), 0, span, 0x00020000);
-		dma16(rs, lds + (wave * PIECES + i) * 1024, KMAJOR || k + kpiece[i] < kend ? off[i] : 0xfffffff0u);
+		dma16(rs, lds + (wave * PIECES + i) * 1024, KMAJOR || k + kpiece[i] < kend ? off[i] : NOWHERE);
 	}
 
 	__device__ __forceinline__ void advance() { p += step, bytes -= step; }

@@ -59,3 +59,34 @@ def test_gradients_at_the_end_of_float16(bnd, name, p, top):
 	within(dx.get(), dz @ W64.T, productBound(dz, W64.T, n) + off @ np.abs(W64.T), "dx")
 	within(dW.get(), x64.T @ dz, productBound(x64.T, dz, m) + np.abs(x64.T) @ off, "dW")
 	within(db.get(), dz.sum(axis=0), off.sum(axis=0) + (m + 4) * U32 * np.abs(dz).sum(axis=0), "db")
+
+
+# ------------------------------------------------------------------------------------------------ linear: few rows, far apart
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("rows,pitch", [(3, 1 << 28), (8, (1 << 27) - 8192), (2, 1 << 28)])
+def test_a_tile_of_few_rows_far_apart(bnd, dtype, rows, pitch):
+	"""A tile takes 32 (float16: 64) rows of an operand whose rows run along the reduction; the product of their number and such a pitch
+	passes 32 bits, and there are rows of neither operand at the places that would wrap onto row 0. dW from x and dy, then x W with W in the buffer, all as
+	columns of one buffer that holds NaN in between."""
+	rng = np.random.RandomState(41)
+	k, n = 16, 24
+	x, dy, W = rng.randn(rows, k).astype(dtype), rng.randn(rows, n).astype(dtype), rng.randn(rows, n).astype(dtype)
+	buf = bnd.GPUArray.empty((rows * pitch, ), dtype=dtype)
+	buf.gpudata.fillD32(0x7fc07e00)                                 # NaN in either type
+	cols = {"x": 0, "dy": 1024, "W": 4096}
+	for name, ary in (("x", x), ("dy", dy), ("W", W)):
+		put(buf, pitch, cols[name], ary)
+	grid = buf.reshape(rows, pitch)
+	view = lambda name, width: grid[:, cols[name]:cols[name] + width]
+
+	x64, dy64, W64 = (a.astype(np.float64) for a in (x, dy, W))
+	_, dW, db = bnd.blas.linearBackward(view("dy", n), view("x", k), gpu(bnd, np.zeros((k, n), dtype)), wantInput=False)
+	within(dW.get(), x64.T @ dy64, productBound(x64.T, dy64, rows), "dW")
+	within(db.get(), dy64.sum(axis=0), (rows + 2) * U32 * np.abs(dy64).sum(axis=0), "db")
+	a = rng.randn(5, rows).astype(dtype)
+	y = bnd.blas.linear(gpu(bnd, a), view("W", n))
+	within(y.get(), a.astype(np.float64) @ W64, productBound(a.astype(np.float64), W64, rows), "y")
+	# what stands in row 0 comes in once: an infinity does not meet the zeros behind the last column of a
+	put(buf, pitch, cols["W"], np.full((1, n), np.inf, dtype))
+	y = bnd.blas.linear(gpu(bnd, np.abs(a)), view("W", n)).get()
+	assert np.isposinf(y).all()

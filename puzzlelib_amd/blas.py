@@ -247,11 +247,10 @@ class BlasContext:
 			xptr, wptr, bptr, rptr = data.rptr, W.rptr, rptrOf(bias), rptrOf(residual)
 			nbytes = plan.forwardBytes(xptr, wptr)
 			ws, wsptr = self.workspace(nbytes, allocator)
+			yptr, pptr = out.optr, None if preact is None else preact.optr
 			if desc.dtype == lib.F16:
 				lazy.matrixBegin()
-			lib.pz_linear_fwd(
-				plan.ref, xptr, wptr, bptr, rptr, key, out.optr, None if preact is None else preact.optr, wsptr, nbytes, None
-			)
+			lib.pz_linear_fwd(plan.ref, xptr, wptr, bptr, rptr, key, yptr, pptr, wsptr, nbytes, None)
 		return out if preact is None else (out, preact)
 
 
@@ -308,11 +307,12 @@ class BlasContext:
 		def target(ary):
 			return None if ary is None else ary.wptr if momentum != 0.0 else ary.optr
 
+		dxptr, dwptr, dbptr = None if out is None else out.optr, target(wgrad), target(bgrad)
 		if plan.desc.dtype == lib.F16:
 			lazy.matrixBegin()
 		lib.pz_linear_bwd(
-			plan.ref, gptr, xptr, wptr, pptr, key, None if out is None else out.optr, target(wgrad),
-			lib.F32 if wgrad is None or wgrad.dtype == np.float32 else lib.F16, target(bgrad), scale, momentum, wsptr, nbytes, None
+			plan.ref, gptr, xptr, wptr, pptr, key, dxptr, dwptr, lib.F32 if wgrad is None or wgrad.dtype == np.float32 else lib.F16,
+			dbptr, scale, momentum, wsptr, nbytes, None
 		)
 		return out, wgrad, bgrad
 

@@ -536,6 +536,23 @@ class HipReduceOps:
 		from puzzlelib_amd.surface import bound
 		return bound().backend.dnn.convMath == "f32"
 
+	def before(self, token):
+		"""the communication stream follows the token's marks, and float16 products (blas.linear) issued since: they are matrix kernels
+		of the same kind as the split ones, which collective and product keep apart from by waiting (lazy.matrixBegin)"""
+		from puzzlelib_amd import lazy
+		main, side = token
+		lazy.afterMatrix(self.node.commStream)
+		self.node.commStream.waitEvent(main)
+		if side is not None:
+			self.node.commStream.waitEvent(side)
+
+	def issued(self, token, begin, start, nbytes):
+		from puzzlelib_amd import driver, lazy
+		done = driver.Event()
+		done.record(self.node.commStream)
+		lazy.foreignLaunched(done)
+		self.events.append((token, done, start, nbytes, begin))
+
 	def markReady(self):
 		"""'final up to here' = an event on the compute stream plus one behind the filter-gradient stream, where the
 		gradients of this bucket were accumulated (DnnContext.filterGradStream)"""
@@ -550,18 +567,12 @@ class HipReduceOps:
 		from puzzlelib_amd import lib, driver
 		node = self.node
 
-		main, side = token
-		node.commStream.waitEvent(main)
-		if side is not None:
-			node.commStream.waitEvent(side)
+		self.before(token)
 		ptr = self.tensor.gpudata.ptr + start      # ordering is carried by the two events, not by the arena's barrier
 		begin = driver.Event()
 		begin.record(node.commStream)
 		lib.pz_comm_allreduce_sum_f32(node.comm, ptr, ptr, (stop - start) // 4, node.commStream.handle)
-
-		done = driver.Event()
-		done.record(node.commStream)
-		self.events.append((token, done, start, stop - start, begin))
+		self.issued(token, begin, start, stop - start)
 
 	def allreduceRanges(self, ranges, token):
 		"""a bucket of several byte ranges of the arena: ONE RCCL group on the communication stream (pz_comm_allreduce_sum_f32_ranges)"""
@@ -569,19 +580,14 @@ class HipReduceOps:
 		from puzzlelib_amd import lib, driver
 		node = self.node
 
-		main, side = token
-		node.commStream.waitEvent(main)
-		if side is not None:
-			node.commStream.waitEvent(side)
+		self.before(token)
 		n = len(ranges)
 		offsets = (ctypes.c_size_t * n)(*[lo // 4 for lo, _ in ranges])
 		counts = (ctypes.c_size_t * n)(*[(hi - lo) // 4 for lo, hi in ranges])
 		begin = driver.Event()
 		begin.record(node.commStream)
 		lib.pz_comm_allreduce_sum_f32_ranges(node.comm, self.tensor.gpudata.ptr, offsets, counts, n, node.commStream.handle)
-		done = driver.Event()
-		done.record(node.commStream)
-		self.events.append((token, done, ranges[0][0], sum(hi - lo for lo, hi in ranges), begin))
+		self.issued(token, begin, ranges[0][0], sum(hi - lo for lo, hi in ranges))
 
 	def unlaunch(self, ranges, scale):
 		"""GradReducer.unlaunch: the compute stream waits for the collectives over `ranges`, scales them to the mean, and the

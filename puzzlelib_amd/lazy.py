@@ -344,28 +344,46 @@ def prune(block=False):
 # stream waits for every foreign launch in front of it, and every later foreign launch waits for it, whatever older mark it brings.
 matrixIssued = False     # since matrixEvent was last recorded
 matrixEvent = None
+beside = deque()         # completion events of launches that `held` does not list: collectives of the gradient exchange, whose reductions
+                         # may hold the same arithmetic (foreignLaunched)
 
 
 def matrixBegin():
+	"""The main stream keeps the float16 product that is launched next apart from what other streams were given so far. To be called when
+	every address of the product has been taken: a barrier may launch on another stream (grid.ArenaWatcher)."""
 	global matrixIssued
 	joinAll()
+	while beside:
+		lib.pz_stream_wait_event(None, beside.popleft().handle)
 	matrixIssued = True
+
+
+def afterMatrix(stream):
+	"""`stream` waits for the float16 products issued so far."""
+	global matrixIssued, matrixEvent
+	if matrixIssued:
+		matrixIssued = False
+		matrixEvent = matrixEvent or newEvent()
+		matrixEvent.record(None)
+	if matrixEvent is not None:
+		stream.waitEvent(matrixEvent)
+
+
+def foreignLaunched(done):
+	"""`done`, an event its owner keeps, lies behind a launch on another stream that left no marks on buffers (foreignEnd)."""
+	while beside and beside[0].query():
+		beside.popleft()
+	beside.append(done)
 
 
 def foreignBegin(stream, ready=None):
 	"""Everything issued on the main stream so far — or up to `ready`, an event the caller recorded on it earlier and knows
 	to lie behind every write of what the launch reads — happens before what `stream` is given next."""
-	global matrixIssued, matrixEvent
 	prune()
 	if ready is None or matrixIssued:
-		if matrixIssued:
-			matrixIssued = False
-			matrixEvent = matrixEvent or newEvent()
-			matrixEvent.record(None)
 		ready = newEvent()
 		ready.record(None)
-	elif matrixEvent is not None:
-		stream.waitEvent(matrixEvent)
+	afterMatrix(stream)
 	stream.waitEvent(ready)
 	return ready
 

@@ -277,7 +277,8 @@ class Mi355Backend:
 						not (outdata.contiguous and indata.contiguous):
 					raise ValueError("%s(outdata %s, indata %s): contiguous %s -> %s arrays of one size, no slice" % (
 						name, outdata.dtype, indata.dtype, np.dtype(src).name, np.dtype(dst).name))
-				entry(outdata.optr, indata.rptr, indata.size, None if stream is None else stream.handle)
+				with lazy.On(stream, (indata, ), (outdata, )) as ((inptr, ), (outptr, )):
+					entry(outptr, inptr, indata.size, streamHandle(stream))
 			cast.__name__ = name
 			return cast
 		self.castFP16toFP32 = castKernel("castFP16toFP32", lib.pz_cast_f16_f32, np.float16, np.float32)

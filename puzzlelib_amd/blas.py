@@ -222,8 +222,8 @@ class BlasContext:
 		Linear, Activation, Dropout and Add do one after the other (Modules/Linear.py:36-41, Activation.py:52-55, Dropout.py:33-58,
 		Add.py:15-22). data is (..., k) in rows of one pitch, W (k, n), or (n, k) with transpW. `preact`: an array for
 		data W + bias (linearBackward needs it behind an activation), or True to have one made; the call then returns (out, preact).
-		`out` may be `residual` (in place). A float16 product keeps apart from the package's launches on other streams; kernels of the
-		user's own on a stream of their own (SourceModule) are the user's to order."""
+		`out` may be `residual` (in place). A float16 product keeps apart from the package's launches on other streams, user kernels
+		(SourceModule) among them; what a program launches by other means is its own to order."""
 		plan = self.linearPlan("linear", data, W, transpW, act, False)
 		key = self.linearMask("linear", dropout)
 		n, shape, dtype = plan.desc.n, plan.shape, data.dtype

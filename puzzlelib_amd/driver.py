@@ -10,7 +10,7 @@ keep their parent alive.
 import ctypes, threading, weakref
 from ctypes import byref, c_int, c_size_t, c_void_p, c_float
 
-from puzzlelib_amd import lib
+from puzzlelib_amd import lib, lazy
 from puzzlelib_amd.lib import HipError
 
 
@@ -209,7 +209,6 @@ class Buffer:
 		"""The span's address after the lazy-buffer barriers (lazy.py) for a main-stream read or write."""
 		root = self.root
 		if root.lz is not None:
-			from puzzlelib_amd import lazy
 			if write:
 				lazy.writeBarrier(root, self, whole and self.size == root.size)
 			else:
@@ -217,8 +216,42 @@ class Buffer:
 		return self.ptr
 
 
+	# as an operand of a launch on some stream (lazy.On), like an array
+	@property
+	def gpudata(self):
+		return self
+
+
+	@property
+	def rptr(self):
+		return self.access()
+
+
+	@property
+	def wptr(self):
+		return self.access(True)
+
+
+	@property
+	def optr(self):
+		return self.access(True, True)
+
+
+	def ptrOn(self, stream, write):
+		"""Address for a launch on a foreign stream: pending contents are settled (on the main stream, which the foreign
+		stream is made to follow), events of *other* streams are waited for by `stream`."""
+		root = self.root
+		if root.lz is not None:
+			if write:
+				lazy.writeBarrier(root, self, False, stream)
+			else:
+				lazy.readBarrier(root, self, stream)
+		return self.ptr
+
+
 	def fillD32(self, value, stream=None):
-		lib.pz_memset_d32(self.access(True, True), int(value) & 0xffffffff, self.size // 4, streamHandle(stream))
+		with lazy.On(stream, (), (self, )) as (_, (ptr, )):
+			lib.pz_memset_d32(ptr, int(value) & 0xffffffff, self.size // 4, streamHandle(stream))
 		return self
 
 
@@ -228,16 +261,19 @@ class Buffer:
 		elif dst.size < self.size:
 			raise ValueError("destination buffer is too small")
 
-		lib.pz_memcpy_d2d(dst.access(True), self.access(), self.size, streamHandle(stream))
+		with lazy.On(stream, (self, ), (dst, ), partial=True) as ((src, ), (ptr, )):
+			lib.pz_memcpy_d2d(ptr, src, self.size, streamHandle(stream))
 		return dst
 
 
 	def set(self, hostptr, nbytes, stream=None):
-		lib.pz_memcpy_h2d(self.access(True), hostptr, nbytes, streamHandle(stream))
+		with lazy.On(stream, (), (self, ), partial=True) as (_, (ptr, )):
+			lib.pz_memcpy_h2d(ptr, hostptr, nbytes, streamHandle(stream))
 
 
 	def get(self, hostptr, nbytes, stream=None):
-		lib.pz_memcpy_d2h(hostptr, self.access(), nbytes, streamHandle(stream))
+		with lazy.On(stream, (self, )) as ((ptr, ), _):
+			lib.pz_memcpy_d2h(hostptr, ptr, nbytes, streamHandle(stream))
 		lib.pz_stream_sync(streamHandle(stream))
 
 
@@ -362,7 +398,8 @@ class MemoryPool:
 
 def memcpy2D(width, height, src, srcPitch, dst, dstPitch, srcX=0, dstX=0, stream=None):
 	"""Pitched device-to-device copy; argument order of Driver.memcpy2D as used by Cuda/GPUBackend.py:296,320."""
-	lib.pz_memcpy_2d(dst.access(True) + dstX, dstPitch, src.access() + srcX, srcPitch, width, height, streamHandle(stream))
+	with lazy.On(stream, (src, ), (dst, ), partial=True) as ((srcptr, ), (dstptr, )):
+		lib.pz_memcpy_2d(dstptr + dstX, dstPitch, srcptr + srcX, srcPitch, width, height, streamHandle(stream))
 
 
 def allocateFromIPCHandle(handle, size):

@@ -165,14 +165,7 @@ class GPUArray:
 	def ptrOn(self, stream, write):
 		"""Address for a launch on a foreign stream: pending contents are settled (on the main stream, which the foreign
 		stream is made to follow), events of *other* streams are waited for by `stream`."""
-		buf = self.gpudata
-		root = buf.root
-		if root.lz is not None:
-			if write:
-				lazy.writeBarrier(root, buf, False, stream)
-			else:
-				lazy.readBarrier(root, buf, stream)
-		return buf.ptr
+		return self.gpudata.ptrOn(stream, write)
 
 
 	@property
@@ -238,7 +231,8 @@ class GPUArray:
 	def stridedCopyFrom(self, src, stream=None):
 		self.enforceWordSized()
 		shape = (ctypes.c_int64 * max(self.ndim, 1))(*self.shape)
-		lib.pz_strided_copy(self.wptr, self.elemStrides(), src.rptr, src.elemStrides(), shape, self.ndim, streamHandle(stream))
+		with lazy.On(stream, (src, ), (self, ), partial=True) as ((srcptr, ), (ptr, )):
+			lib.pz_strided_copy(ptr, self.elemStrides(), srcptr, src.elemStrides(), shape, self.ndim, streamHandle(stream))
 
 
 	def get(self, stream=None):
@@ -246,7 +240,8 @@ class GPUArray:
 		out = np.empty(self.shape, dtype=self.dtype)
 
 		if self.nbytes > 0:
-			lib.pz_memcpy_d2h(out.ctypes.data, src.rptr, self.nbytes, streamHandle(stream))
+			with lazy.On(stream, (src, )) as ((ptr, ), _):
+				lib.pz_memcpy_d2h(out.ctypes.data, ptr, self.nbytes, streamHandle(stream))
 			lib.pz_stream_sync(streamHandle(stream))
 
 		return out
@@ -260,7 +255,8 @@ class GPUArray:
 				))
 
 			if self.contiguous and ary.contiguous:
-				lib.pz_memcpy_d2d(self.optr, ary.rptr, self.nbytes, streamHandle(stream))
+				with lazy.On(stream, (ary, ), (self, )) as ((src, ), (ptr, )):
+					lib.pz_memcpy_d2d(ptr, src, self.nbytes, streamHandle(stream))
 			else:
 				self.stridedCopyFrom(ary, stream)
 			return
@@ -276,7 +272,8 @@ class GPUArray:
 			return
 
 		if self.contiguous:
-			lib.pz_memcpy_h2d(self.optr, ary.ctypes.data, self.nbytes, streamHandle(stream))
+			with lazy.On(stream, (), (self, )) as (_, (ptr, )):
+				lib.pz_memcpy_h2d(ptr, ary.ctypes.data, self.nbytes, streamHandle(stream))
 			lib.pz_stream_sync(streamHandle(stream))      # the host array may die right after this call
 		else:
 			self.stridedCopyFrom(GPUArray.toGpu(ary), stream)

@@ -423,6 +423,32 @@ def foreignEnd(stream, ready, reads=(), writes=(), keep=()):
 	return done
 
 
+class On:
+	"""`with On(stream, reads, writes) as (rptrs, wptrs)`: the addresses for launches on `stream` that read and write these arrays or
+	buffers (None among them stays None). On a stream other than the main one (None) they follow everything issued so far, and the
+	main stream follows them where it touches what they touched. `partial`: not all of each written array is overwritten."""
+	__slots__ = ("stream", "reads", "writes", "partial", "ready")
+
+	def __init__(self, stream, reads=(), writes=(), partial=False):
+		self.stream, self.reads, self.writes, self.partial = stream, reads, writes, partial
+
+	def __enter__(self):
+		stream = self.stream
+		if stream is None:
+			return [None if a is None else a.rptr for a in self.reads], [
+				None if a is None else a.wptr if self.partial else a.optr for a in self.writes
+			]
+		ptrs = [None if a is None else a.ptrOn(stream, False) for a in self.reads], [
+			None if a is None else a.ptrOn(stream, True) for a in self.writes
+		]
+		self.ready = foreignBegin(stream)
+		return ptrs
+
+	def __exit__(self, kind, value, trace):
+		if self.stream is not None and kind is None:
+			foreignEnd(self.stream, self.ready, *[[a for a in arrays if a is not None] for arrays in (self.reads, self.writes)])
+
+
 def joinAll():
 	"""The main stream waits for everything foreign streams were given (device-wide ordering point)."""
 	prune()

@@ -382,11 +382,11 @@ class PointwiseCost:
 		requireF32(a, error, grad)
 		assert grad.size == a.size
 		terms = GPUArray.empty((a.size, ), dtype=np.float32, allocator=allocator)
-		lib.pz_cost_pointwise(
-			kind, a.rptr, rptrOf(other), rptrOf(labels), error.wptr, grad.optr,
-			None if grad2 is None else grad2.optr, terms.optr, a.size, int(numsamples), int(numcases), float(norm), float(fullnorm),
-			streamHandle(stream)
-		)
+		# (the error is read too: what it holds is added to)
+		with lazy.On(stream, (a, other, labels, error), (error, grad, grad2, terms)) as (rptrs, wptrs):
+			lib.pz_cost_pointwise(
+				kind, *rptrs[:3], *wptrs, a.size, int(numsamples), int(numcases), float(norm), float(fullnorm), streamHandle(stream)
+			)
 
 
 class PReluModule:

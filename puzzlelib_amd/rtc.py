@@ -17,7 +17,7 @@ import ctypes, json, struct
 
 import numpy as np
 
-from puzzlelib_amd import lib
+from puzzlelib_amd import lib, lazy
 from puzzlelib_amd.driver import streamHandle
 from puzzlelib_amd.gpuarray import GPUArray
 
@@ -78,13 +78,15 @@ class Function:
 		self.module, self.name, self.handle = module, name, handle
 
 	def __call__(self, *args, block, grid, shared=0, stream=None, formats=None, writes=()):
-		values, fmts = [], []
+		values, fmts, reads, written = [], [], [], []
 		for idx, arg in enumerate(args):
 			if isinstance(arg, GPUArray):
 				if not arg.contiguous:
 					raise ValueError("gpuarray is not contiguous")
 				# (without a parameter list nobody knows which arrays a kernel writes: every array is treated as written)
-				values.append(arg.ptr if (formats is None or idx in writes) else arg.rptr)
+				write = formats is None or idx in writes
+				(written if write else reads).append(arg)
+				values.append(arg.ptrOn(stream, write) if stream is not None else arg.ptr if write else arg.rptr)
 				fmts.append("P")
 			elif formats is not None:
 				values.append(arg)
@@ -97,7 +99,11 @@ class Function:
 		buf = pack(fmts, values)
 		g = (ctypes.c_uint32 * 3)(*(tuple(int(v) for v in grid) + (1, 1))[:3])
 		b = (ctypes.c_uint32 * 3)(*(tuple(int(v) for v in block) + (1, 1))[:3])
+		# (on a stream of the caller's: behind everything issued so far, and the main stream waits for it when it touches these arrays)
+		ready = None if stream is None else lazy.foreignBegin(stream)
 		lib.pz_function_launch(self.handle, g, b, int(shared), buf, len(buf), streamHandle(stream))
+		if stream is not None:
+			lazy.foreignEnd(stream, ready, reads=reads, writes=written)
 
 
 class SourceModule:

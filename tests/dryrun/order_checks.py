@@ -151,6 +151,72 @@ def float32_needs_no_order():
 	node.close()
 
 
+def entries():
+	"""every entry that takes a stream: name, launch(stream), the array it reads, the array it writes, the library call"""
+	f, h = np.float32, np.float16
+	x, y, z, e = A(64), A(64), A(64), A(1)
+	labels, few = A(64, dtype=np.int32), A(8, dtype=np.int32)
+	half, other = A(64, dtype=h), A(64)
+	host = np.zeros(64, f)
+	grid2 = A(8, 16)
+	mask = bnd.DropoutMask(1, 2, 0.5)
+	scale = bnd.ElementwiseKernel([("float *", "out"), ("const float *", "data")], "out[i] = 2 * data[i]", "scaleKer")
+	total = bnd.ReductionKernel(f, "0", "a + b", "data[i]", [("const float *", "data")], "totalKer")
+	return [
+		("eltwise", lambda s: bnd.toVectorAddVectorKer(f)(y, x, 1.0, stream=s), x, y, "pz_eltwise"),
+		("addKer", lambda s: bnd.addKer(f)(y, x, 1.0, z, 1.0, stream=s), x, y, "pz_eltwise"),
+		("counterDropoutKer", lambda s: bnd.counterDropoutKer(f)(y, x, mask, stream=s), x, y, "pz_dropout"),
+		("castFP32toFP16", lambda s: bnd.castFP32toFP16(half, x, stream=s), x, half, "pz_cast_f32_f16"),
+		("castFP16toFP32", lambda s: bnd.castFP16toFP32(x, half, stream=s), half, x, "pz_cast_f16_f32"),
+		("bceKer", lambda s: bnd.bceKer(x, labels, e, y, 64, 1, stream=s), x, y, "pz_cost_pointwise"),
+		("bceKer's error", lambda s: bnd.bceKer(x, labels, e, y, 64, 1, stream=s), labels, e, "pz_cost_pointwise"),
+		("hingeKer", lambda s: bnd.hingeKer(x, labels, e, y, 8, 8, stream=s), x, y, "pz_cost_pointwise"),
+		("smoothL1Ker", lambda s: bnd.smoothL1Ker(x, z, e, y, 1.0, 1.0, stream=s), z, y, "pz_cost_pointwise"),
+		("l1HingeKer", lambda s: bnd.l1HingeKer(x, z, few, e, y, other, 8, 8, stream=s), few, other, "pz_cost_pointwise"),
+		("set from an array", lambda s: y.set(x, stream=s), x, y, "pz_memcpy_d2d"),
+		("strided set", lambda s: grid2[:, :8].set(x.reshape(8, 8), stream=s), x, grid2, "pz_strided_copy"),
+		("set from the host", lambda s: y.set(host, stream=s), None, y, "pz_memcpy_h2d"),
+		("get", lambda s: x.get(stream=s), x, None, "pz_memcpy_d2h"),
+		("Buffer.fillD32", lambda s: y.gpudata.fillD32(1, stream=s), None, y, "pz_memset_d32"),
+		("Buffer.copy", lambda s: x.gpudata.copy(y.gpudata, stream=s), x, y, "pz_memcpy_d2d"),
+		("Buffer.set", lambda s: y.gpudata.set(host.ctypes.data, 256, stream=s), None, y, "pz_memcpy_h2d"),
+		("Buffer.get", lambda s: x.gpudata.get(host.ctypes.data, 256, stream=s), x, None, "pz_memcpy_d2h"),
+		("memcpy2D", lambda s: bnd.Driver.memcpy2D(16, 4, x.gpudata, 32, y.gpudata, 32, stream=s), x, y, "pz_memcpy_2d"),
+		("ElementwiseKernel", lambda s: scale(y, x, stream=s), x, y, "pz_function_launch"),
+		("ReductionKernel", lambda s: total(x, stream=s), x, None, "pz_function_launch"),
+	]
+
+
+def streams():
+	"""each entry on a stream of the caller's: behind what the main stream was given, in front of what touches the same arrays there
+	afterwards, and apart from float16 products on either side"""
+	product = products("pz_linear_fwd")
+	for name, launch, source, target, entry in entries():
+		stream = bnd.Driver.Stream()
+		order = watched()
+		if source is not None:
+			source.gpudata.fillD32(7)                            # its input is written on the main stream ...
+		product()                                                # ... and a product runs there
+		earlier = len(order.launches)
+		launch(stream)
+		foreign = [i for i, (n, s) in enumerate(order.launches) if n == entry and s == stream.handle]
+		assert foreign and foreign[0] >= earlier, (name, order.launches)
+		for i in foreign:
+			for j in range(earlier):
+				order.follows(i, j)
+		product()
+		order.follows(len(order.launches) - 1, foreign[-1])
+		# afterwards on the main stream: reading what was written, overwriting what was read
+		order = watched()
+		launch(stream)
+		foreign = [i for i, (n, s) in enumerate(order.launches) if n == entry and s == stream.handle]
+		for array in (source, target):
+			if array is not None:
+				since = len(order.launches)
+				(array.gpudata.copy if array is target else lambda: array.gpudata.fillD32(9))()
+				order.follows(since, foreign[-1 if array is target else 0])         # (a reduction reads in its first launch)
+
+
 if __name__ == "__main__":
 	globals()[sys.argv[1]]()
 	print("OK")

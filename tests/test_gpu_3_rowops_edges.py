@@ -90,3 +90,31 @@ def test_a_tile_of_few_rows_far_apart(bnd, dtype, rows, pitch):
 	put(buf, pitch, cols["W"], np.full((1, n), np.inf, dtype))
 	y = bnd.blas.linear(gpu(bnd, np.abs(a)), view("W", n)).get()
 	assert np.isposinf(y).all()
+
+
+# ------------------------------------------------------------------------------------------------ streams
+def test_casts_costs_and_user_kernels_on_a_stream_around_a_product(bnd):
+	"""what a mixed-precision step would put beside its float16 product on a borrowed stream: each launch waits for the one whose result it takes"""
+	rng = np.random.RandomState(51)
+	m, k, n = 512, 384, 640
+	W = (rng.randn(k, n) / 16).astype(np.float16)
+	gW = gpu(bnd, W)
+	stream = bnd.Driver.Stream()
+	twice = bnd.ElementwiseKernel([("float *", "out"), ("const float *", "data")], "out[i] = 2.0f * data[i]", "twiceKer")
+	E = lambda shape, dtype: bnd.GPUArray.empty(shape, dtype=dtype)
+	for call in range(3):
+		x = rng.randn(m, k).astype(np.float32)
+		master, h, y32, t, g, err = E((m, k), np.float32), E((m, k), np.float16), E((m, n), np.float32), E((m, n), np.float32), E((m, n), np.float32), gpu(bnd, np.zeros((1, ), np.float32))
+		master.set(gpu(bnd, x), stream=stream)
+		bnd.castFP32toFP16(h, master, stream=stream)
+		y = bnd.blas.linear(h, gW)
+		bnd.castFP16toFP32(y32, y, stream=stream)
+		twice(t, y32, stream=stream)
+		bnd.smoothL1Ker(t, y32, err, g, 1.0, 1.0, stream=stream)
+		z = bnd.blas.linear(y, gpu(bnd, np.eye(n, dtype=np.float16)))                   # another product while the stream still works
+		want = y.get().astype(np.float32)
+		x16 = x.astype(np.float16).astype(np.float64)
+		assert np.array_equal(h.get().astype(np.float64), x16)
+		within(y.get(), x16 @ W, productBound(x16, W.astype(np.float64), k), "y")
+		assert np.array_equal(y32.get(), want) and np.array_equal(t.get(stream=stream), 2.0 * want) and np.array_equal(z.get(), y.get())
+		assert np.isfinite(err.get()).all() and np.isfinite(g.get()).all()

@@ -549,7 +549,8 @@ enum { PZ_ACT_NONE = 0, PZ_ACT_RELU = 1, PZ_ACT_GELU = 2, PZ_ACT_SILU = 3 };
 
 /* A dropout mask by its key: element i (in row-major order of the tensor) is kept where word i of call `call` of the generator `seed`
  * — exactly the word pz_rng_fill_u32 would have written — is below `threshold`; kept elements are divided by `keep`, dropped ones are
- * zero whatever they hold. The same key gives the same mask forward and backward; nothing is stored.                                  */
+ * zero whatever they hold. The same key gives the same mask forward and backward; nothing is stored. Threshold 2^32 - 1 with keep 1
+ * (p = 0) keeps every element, also the one in 2^32 whose word is the threshold itself.                                               */
 typedef struct pz_dropout_mask {
 	uint64_t seed, call;
 	uint32_t threshold;

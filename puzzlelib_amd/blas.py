@@ -200,7 +200,7 @@ class BlasContext:
 			return None
 		if not isinstance(dropout, DropoutMask):
 			raise ValueError("%s: dropout is a DropoutMask, got %r" % (what, dropout))
-		return byref(dropout.key)
+		return byref(dropout.key) if dropout.drops else None
 
 
 	@staticmethod

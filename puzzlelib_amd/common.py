@@ -90,9 +90,9 @@ class FusedAct(Enum):                  # the activation inside blas.linear / dnn
 class DropoutMask:
 	"""A dropout mask by its key. Element i of a tensor (row-major) is kept where word i of call `call` of the generator `seed` is
 	below (1 - p) * (2^32 - 1), and kept elements are divided by 1 - p: the mask fillInteger + dropoutKer
-	(Modules/Dropout.py:33-72) would apply, computed where it is needed instead of stored. The same object gives the same mask
-	forward and backward. RandomNumberGenerator.dropoutMask(p) hands out a mask nobody else gets."""
-	__slots__ = ("seed", "call", "p", "key")
+	(Modules/Dropout.py:33-72) would apply, computed where it is needed instead of stored; at p = 0 every element is kept, also one
+	whose word is 2^32 - 1. The same object gives the same mask forward and backward. RandomNumberGenerator.dropoutMask(p) hands out a mask nobody else gets."""
+	__slots__ = ("seed", "call", "p", "key", "drops")
 
 	def __init__(self, seed, call, p):
 		if not 0.0 <= p < 1.0:
@@ -102,6 +102,7 @@ class DropoutMask:
 			raise ValueError("a dropout mask's seed and call are unsigned 64-bit numbers")
 		keep = 1.0 - self.p
 		self.key = lib.DropoutKey(self.seed, self.call, int(keep * np.iinfo(np.uint32).max), keep)
+		self.drops = self.key.threshold != np.iinfo(np.uint32).max
 
 
 class ConvPerf:                        # Hip/Wrappers/MIOpen.py:82-100

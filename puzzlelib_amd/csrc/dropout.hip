@@ -9,13 +9,13 @@ namespace {
 // 16 bytes of T a lane: COUNT consecutive elements, so a lane evaluates whole quads of the generator. Bound by memory: 8192 x 8192 float16
 // with a residual 68 us (402 MB, 5.9 TB/s); 256 x 1024 float32 2.5 us, the launch.
 template <typename T>
-__global__ void __launch_bounds__(256) dropout_kernel(const T *x, const T *residual, T *y, size_t count, DropKey key, int vec) {
+__global__ void __launch_bounds__(256) dropout_kernel(const T *x, const T *residual, T *y, size_t count, DropKey key, int dropping, int vec) {
 	constexpr int COUNT = 16 / sizeof(T);
 	const size_t first = ((size_t)blockIdx.x * 256 + threadIdx.x) * COUNT;
 	if (first >= count) return;
 	const int left = count - first < COUNT ? (int)(count - first) : COUNT;
 	const bool whole = vec && left == COUNT;
-	const unsigned bits = drop_bits<COUNT>(key, first);
+	const unsigned bits = dropping ? drop_bits<COUNT>(key, first) : ~0u;
 	float v[COUNT];
 	load_run(x + first, whole, left, v);
 #pragma unroll
@@ -36,7 +36,7 @@ int run(const void *x, const void *residual, void *y, size_t count, const pz_dro
 	const size_t blocks = (count + 256 * COUNT - 1) / (256 * COUNT);
 	PZ_REQUIRE(launchable(blocks, 256), "pz_dropout: %zu elements are too many", count);
 	dropout_kernel<T><<<(unsigned)blocks, 256, 0, st>>>((const T *)x, (const T *)residual, (T *)y, count,
-	                                                    DropKey{mask->seed, mask->call, mask->threshold, mask->keep}, vec);
+	                                                    DropKey{mask->seed, mask->call, mask->threshold, mask->keep}, drops(mask), vec);
 	PZ_LAUNCH_CHECK();
 	return PZ_OK;
 }

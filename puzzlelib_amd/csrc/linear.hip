@@ -798,6 +798,7 @@ int pz_linear_fwd(const pz_linear_desc *d, const void *x, const void *w, const f
                   void *y, void *preact, void *workspace, size_t ws_bytes, pz_stream_t stream) {
 	if (int rc = check_desc(d, "pz_linear_fwd")) return rc;
 	if (int rc = check_mask(mask, "pz_linear_fwd")) return rc;
+	if (!drops(mask)) mask = nullptr;
 	if (d->m == 0) return PZ_OK;
 	PZ_REQUIRE(x && w && y, "pz_linear_fwd: null tensor");
 	PZ_REQUIRE((!residual || d->ldr >= d->n) && (!preact || d->ldp >= d->n), "pz_linear_fwd: row pitch too small");
@@ -828,6 +829,7 @@ int pz_linear_bwd(const pz_linear_desc *d, const void *dy, const void *x, const 
                   void *dx, void *dw, int dw_dtype, float *db, float alpha, float beta, void *workspace, size_t ws_bytes, pz_stream_t stream) {
 	if (int rc = check_desc(d, "pz_linear_bwd")) return rc;
 	if (int rc = check_mask(mask, "pz_linear_bwd")) return rc;
+	if (!drops(mask)) mask = nullptr;
 	PZ_REQUIRE(dw_dtype == PZ_F32 || dw_dtype == d->dtype, "pz_linear_bwd: weight gradients are float32 or the operands' type");
 	PZ_REQUIRE(d->m == 0 || (dy && (!dx || w) && (!dw || x)), "pz_linear_bwd: null tensor");
 	PZ_REQUIRE(d->m == 0 || d->act == PZ_ACT_NONE || (preact && d->ldp >= d->n), "pz_linear_bwd: the activation's gradient needs the pre-activation");

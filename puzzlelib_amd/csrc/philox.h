@@ -24,6 +24,9 @@ struct DropKey {
 	float keep;
 };
 
+// A mask of p = 0 keeps everything and is no mask at all: below its threshold of 2^32 - 1 every word lies but one
+inline bool drops(const pz_dropout_mask *mask) { return mask && !(mask->threshold == 0xffffffffu && mask->keep == 1.f); }
+
 // words of elements 4 * quad ... 4 * quad + 3
 __device__ __forceinline__ uint4 drop_words(const DropKey &d, uint64_t quad) {
 	return philox4x32_10(make_uint4((uint32_t)quad, (uint32_t)(quad >> 32), (uint32_t)d.call, (uint32_t)(d.call >> 32)),

@@ -5,8 +5,9 @@ values at the ends of the types' ranges, row pitches whose multiples pass 32 bit
 import numpy as np
 import pytest
 
+from puzzlelib_amd import lib
 from test_gpu_3_rowops import (
-	ACTS, LIPSCHITZ, TINY, U, U32, Case, act, gpu, keep, normBounds, normOracle, productBound, put, slope, take, within
+	ACTS, LIPSCHITZ, TINY, U, U32, Case, act, gpu, keep, normBounds, normOracle, productBound, put, slope, take, within, words
 )
 
 pytestmark = pytest.mark.gpu
@@ -59,6 +60,33 @@ def test_gradients_at_the_end_of_float16(bnd, name, p, top):
 	within(dx.get(), dz @ W64.T, productBound(dz, W64.T, n) + off @ np.abs(W64.T), "dx")
 	within(dW.get(), x64.T @ dz, productBound(x64.T, dz, m) + np.abs(x64.T) @ off, "dW")
 	within(db.get(), dz.sum(axis=0), off.sum(axis=0) + (m + 4) * U32 * np.abs(dz).sum(axis=0), "db")
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+def test_a_mask_of_p_0_keeps_everything(bnd, dtype):
+	"""word 1979 of call 117436 of seed 2026 is 2^32 - 1, the one word that does not lie below the threshold of p = 0"""
+	seed, call, at, m, n = 2026, 117436, 1979, 32, 128
+	assert words(seed, call, at + 1)[at] == 0xffffffff
+	mask = bnd.DropoutMask(seed, call, 0.0)
+	c = Case(bnd, dtype, m, 40, n, seed=34)
+	args = gpu(bnd, c.x), gpu(bnd, c.W)
+	plain = bnd.blas.linear(*args)
+	assert plain.get().reshape(-1)[at] != 0 and np.array_equal(bnd.blas.linear(*args, dropout=mask).get(), plain.get())
+	with_mask, without = (bnd.blas.linearBackward(gpu(bnd, c.dy), *args, dropout=d) for d in (mask, None))
+	assert all(np.array_equal(a.get(), b.get()) for a, b in zip(with_mask, without))
+	y = bnd.GPUArray.empty((m, n), dtype=dtype)
+	bnd.counterDropoutKer(dtype)(y, plain, mask)
+	assert np.array_equal(y.get(), plain.get())
+	# through the C entries as well, whatever hands them the key
+	lib.pz_dropout(lib.F32 if dtype == np.float32 else lib.F16, plain.rptr, None, y.optr, y.size, lib.byref(mask.key), None)
+	assert np.array_equal(y.get(), plain.get())
+	desc = lib.LinearDesc(lib.F32 if dtype == np.float32 else lib.F16, 0, 0, m, n, 40, 40, n, n, n, n)
+	lib.pz_linear_fwd(lib.byref(desc), args[0].rptr, args[1].rptr, None, None, lib.byref(mask.key), y.optr, None, None, 0, None)
+	assert np.array_equal(y.get(), plain.get())
+	# one in 2^32 is what the stored form drops there; the smallest p that drops anything does too
+	least = bnd.DropoutMask(seed, call, 2.0 ** -32)
+	bnd.counterDropoutKer(dtype)(y, plain, least)
+	assert y.get().reshape(-1)[at] == 0
 
 
 # ------------------------------------------------------------------------------------------------ linear: few rows, far apart

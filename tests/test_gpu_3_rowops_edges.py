@@ -120,6 +120,37 @@ def test_a_tile_of_few_rows_far_apart(bnd, dtype, rows, pitch):
 	assert np.isposinf(y).all()
 
 
+# ------------------------------------------------------------------------------------------------ group norm
+def test_groupnorm_of_many_values_to_a_group(bnd):
+	"""4096 x 4100 values to one group, close together and far from zero: every value's rounding would fall the same way in a long float32 sum"""
+	shape, u = (1, 4096, 4100), U32
+	rng = np.random.RandomState(61)
+	x = (1.1 + 1e-3 * rng.randn(*shape)).astype(np.float32)
+	dy = (1.1 + 1e-3 * rng.randn(*shape)).astype(np.float32)
+	gx = gpu(bnd, x)
+	y, gm, gv = bnd.dnn.groupNormNd(gx, None, None, 1)
+	x64, dy64 = x.astype(np.float64), dy.astype(np.float64)
+	mean, var = x64.mean(), x64.var()
+	invvar = 1.0 / np.sqrt(var + 1e-5)
+	# the mean and 1 / sqrt are rounded once; a centred value is off by a rounding and the mean's, so that the variance moves by twice that
+	dmean = u * mean
+	dinv = invvar * 4 * (dmean * invvar + u)
+	within(gm.get(), np.full((1, 1), mean), 0.0, "mean")
+	within(gv.get(), np.full((1, 1), invvar), dinv, "invvar")
+	xhat = (x64 - mean) * invvar
+	within(y.get(), xhat, np.abs(xhat) * (dinv / invvar + 3 * u) + 2 * dmean * invvar, "y")
+
+	m32, i32 = np.full((1, 1), mean, np.float32), np.full((1, 1), invvar, np.float32)
+	xh = (x64 - np.float64(m32[0, 0])) * np.float64(i32[0, 0])
+	a, b = dy64.mean(), (dy64 * xh).mean()
+	dx = np.float64(i32[0, 0]) * (dy64 - a - xh * b)
+	# xhat: a rounding of the difference (up to |x| in size, exact here: both lie within a factor of two) and one of the product; products and
+	# differences of values up to dy
+	off = 4 * u * (np.abs(dy64) + np.abs(xh * b) + np.abs(xh))
+	got, _, _ = bnd.dnn.groupNormNdBackward(gpu(bnd, dy), gx, None, None, gpu(bnd, m32), gpu(bnd, i32), 1)
+	within(got.get(), dx, np.float64(i32[0, 0]) * off, "dx")
+
+
 # ------------------------------------------------------------------------------------------------ streams
 def test_casts_costs_and_user_kernels_on_a_stream_around_a_product(bnd):
 	"""what a mixed-precision step would put beside its float16 product on a borrowed stream: each launch waits for the one whose result it takes"""

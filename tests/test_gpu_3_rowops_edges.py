@@ -6,9 +6,8 @@ import numpy as np
 import pytest
 
 from puzzlelib_amd import lib
-from test_gpu_3_rowops import (
-	ACTS, LIPSCHITZ, TINY, U, U32, Case, act, gpu, keep, normBounds, normOracle, productBound, put, slope, take, within, words
-)
+import test_gpu_3_rowops as rowops
+from test_gpu_3_rowops import ACTS, NORMS, U32, Case, act, gpu, keep, productBound, put, slope, within, words
 
 pytestmark = pytest.mark.gpu
 
@@ -89,6 +88,106 @@ def test_a_mask_of_p_0_keeps_everything(bnd, dtype):
 	assert y.get().reshape(-1)[at] == 0
 
 
+def curve(z, name):
+	"""value, slope in 64 bits, and what their evaluation in float32 may be off, as a bound of its own: u = 2^-24 a rounding, 2 u an exp2, a
+	reciprocal or a rounded constant"""
+	from scipy.special import erfc
+	u, a = U32, np.abs(z)
+	if name == "gelu":
+		# tail = R e with e = exp(-z^2 / 2): the exponent z^2 / 2 log2(e) carries three roundings, which move e by 3 u z^2 / 2; R is a fit of
+		# 1.2e-7 at a reciprocal, evaluated in eight steps whose terms add up to twice their sum at most
+		tail, phi = 0.5 * erfc(a / np.sqrt(2.0)), np.exp(-0.5 * z * z) / np.sqrt(2.0 * np.pi)
+		cdf = np.where(z < 0, tail, 1.0 - tail)
+		rel = 1.2e-7 + (1.5 * z * z + 24) * u
+		off = tail * rel + np.where(z < 0, 0.0, u)
+		return z * cdf, a * off + 2 * u * np.abs(z * cdf), cdf + z * phi, off + a * phi * (rel + 4 * u) + 2 * u * (cdf + a * phi)
+	# exp(-z): the exponent carries two roundings, 2 u |z|; s = 1 / (1 + exp(-z)) moves by that times 1 - s
+	s, c = 1.0 / (1.0 + np.exp(-z)), 1.0 / (1.0 + np.exp(z))                      # (c = 1 - s)
+	off = s * (c * (2 * a + 2) * u + 4 * u)
+	return z * s, a * off + 2 * u * a * s, s * (1.0 + z * c), off * (1.0 + a * c) + s * (a * (off + u) + 2 * u * (1.0 + a * c))
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("name,far", [("gelu", 12.0), ("silu", 80.0)])
+def test_activation_tails(bnd, dtype, name, far):
+	"""the fused activations and their slopes over their whole range, through products with the identity: relative to the value itself, so that
+	a tail of zeros does not pass"""
+	k = 64
+	z = np.concatenate((np.linspace(-far, far, 40 * k), np.linspace(-6.0, -2.0, 20 * k), np.linspace(-1.0, 1.0, 4 * k))).astype(dtype)
+	z = np.concatenate((z, [0.0, -0.0, 1e-7, -1e-7], np.zeros(k - 4))).astype(dtype).reshape(-1, k)
+	z64 = z.astype(np.float64)
+	value, voff, der, doff = curve(z64, name)
+	one = gpu(bnd, np.eye(k, dtype=dtype))
+	y, pre = bnd.blas.linear(gpu(bnd, z), one, act=bnd.FusedAct[name], preact=True)
+	assert np.array_equal(pre.get(), z)
+	within(y.get(), value, voff, name)
+	dx, _, db = bnd.blas.linearBackward(gpu(bnd, np.ones_like(z)), gpu(bnd, z), one, act=bnd.FusedAct[name], preact=pre)
+	held = 0.0 if dtype == np.float32 else 2.0 ** -11 * np.abs(der) + 2.0 ** -24
+	within(dx.get(), der, doff + held + 2 * U32 * np.abs(der), name + "'")
+	within(db.get(), der.sum(axis=0), doff.sum(axis=0) + (z.shape[0] + 2) * U32 * np.abs(der).sum(axis=0), "sum of " + name + "'")
+
+
+# ------------------------------------------------------------------------------------------------ linear: the tiles of large products
+@pytest.fixture(scope="module")
+def operands():
+	"""one set of operands a type: (m, 4104), (4104, 4104) and gradients, of which each test takes a corner"""
+	made = {}
+
+	def get(dtype):
+		if dtype not in made:
+			rng = np.random.Generator(np.random.Philox(71))
+			made[dtype] = [rng.standard_normal((4104, 4104), dtype=np.float32).astype(dtype) for _ in range(3)]
+		return made[dtype]
+	yield get
+	made.clear()
+
+
+# 256 x 256 tiles where there are 256 of them (k of 1024 on in float32, 256 in float16), 128 x 128 ones where more than 256 of those are; the
+# last tile of every axis is ragged, and 2101 lies off 16 bytes
+FORWARD = [(np.float32, 4000, 1100, 3908), (np.float16, 4000, 328, 3912), (np.float32, 2100, 516, 2108), (np.float16, 2100, 200, 2104), (np.float16, 2101, 201, 2101)]
+
+
+@pytest.mark.parametrize("dtype,m,k,n", FORWARD)
+@pytest.mark.parametrize("transpW", [False, True])
+def test_large_tiles_forward(bnd, operands, dtype, m, k, n, transpW):
+	a, b, c = operands(dtype)
+	x, W, r = a[:m, :k], (b[:n, :k] if transpW else b[:k, :n]), c[:m, :n]
+	bias = a[-1, :n].astype(np.float32)
+	mask = bnd.DropoutMask(72, 1 << 33, 0.25)
+	out, pre = bnd.blas.linear(gpu(bnd, x), gpu(bnd, W), gpu(bnd, bias), act=bnd.FusedAct.relu, dropout=mask, residual=gpu(bnd, r), preact=True, transpW=transpW)
+	rows = np.unique(np.concatenate((np.arange(0, m, 53), [m - 1])))
+	x64, W64 = x[rows].astype(np.float64), (W.T if transpW else W).astype(np.float64)
+	z = x64 @ W64 + bias
+	zb = productBound(x64, W64, k) + U32 * np.abs(z)
+	within(pre.get()[rows], z, zb, "preact")
+	kept = keep(mask, (m, n))[rows]
+	y = act(z, "relu") * kept
+	within(out.get()[rows], y + r[rows], zb * kept + 3 * U32 * (np.abs(y) + np.abs(r[rows].astype(np.float64))), "y")
+
+
+BACKWARD = [(np.float32, 4000, 3908, 4100), (np.float16, 4000, 3912, 4104), (np.float32, 2100, 2108, 2116), (np.float16, 2100, 2104, 2120), (np.float16, 2101, 2099, 2101)]
+
+
+@pytest.mark.parametrize("dtype,m,k,n", BACKWARD)
+@pytest.mark.parametrize("transpW", [False, True])
+def test_large_tiles_backward(bnd, operands, dtype, m, k, n, transpW):
+	"""dx of m x k with n terms to a sum, dW of k x n with m: both in the tiles above, reduced along and across the rows"""
+	a, b, c = operands(dtype)
+	x, W, dy = a[:m, :k], (b[:n, :k] if transpW else b[:k, :n]), c[:m, :n]
+	mask = bnd.DropoutMask(73, 2, 0.5)
+	dx, dW, db = bnd.blas.linearBackward(gpu(bnd, dy), gpu(bnd, x), gpu(bnd, W), dropout=mask, transpW=transpW)
+	dz = dy.astype(np.float64) * keep(mask, (m, n))                              # (dy doubled or nothing: no rounding)
+	W64 = (W.T if transpW else W).astype(np.float64)
+	rows = np.unique(np.concatenate((np.arange(0, m, 131), [m - 1])))
+	got = dx.get()[rows]
+	within(got, dz[rows] @ W64.T, productBound(dz[rows], W64.T, n), "dx")
+	cols = np.unique(np.concatenate((np.arange(0, k, 127), [k - 1])))
+	got = (dW.get().T if transpW else dW.get())[cols]
+	xt = x[:, cols].T.astype(np.float64)
+	within(got, xt @ dz, productBound(xt, dz, m), "dW")
+	within(db.get(), dz.sum(axis=0), (m + 2) * U32 * np.abs(dz).sum(axis=0), "db")
+
+
 # ------------------------------------------------------------------------------------------------ linear: few rows, far apart
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 @pytest.mark.parametrize("rows,pitch", [(3, 1 << 28), (8, (1 << 27) - 8192), (2, 1 << 28)])
@@ -149,6 +248,44 @@ def test_groupnorm_of_many_values_to_a_group(bnd):
 	off = 4 * u * (np.abs(dy64) + np.abs(xh * b) + np.abs(xh))
 	got, _, _ = bnd.dnn.groupNormNdBackward(gpu(bnd, dy), gx, None, None, gpu(bnd, m32), gpu(bnd, i32), 1)
 	within(got.get(), dx, np.float64(i32[0, 0]) * off, "dx")
+
+
+# A slab is 128 bytes of channels wide, or 64 (two workgroups then share a line), where a workgroup of 512 or 1024 threads holds all pixels of it:
+# up to 1024 (128 bytes, 512 threads), 2048 (64 bytes), 4096 (64 bytes, 1024 threads) forward, half as many backward; whole groups of 128
+# bytes take 1024 threads at once. At least 128 such slabs, or the pixels are cut into chunks. Last: more samples than slabs of a power of two.
+LARGE = [((16, 999, 512), 32), ((8, 1999, 512), 32), ((8, 3999, 512), 32), ((16, 1777, 512), 8), ((16, 333, 512), 32), ((8, 777, 512), 32), ((16, 901, 512), 8),
+		 ((43, 700, 192), 12)]
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("shape,groups", LARGE)
+def test_groupnorm_large_slabs(bnd, dtype, shape, groups):
+	if dtype == np.float32:
+		shape = shape[:2] + (shape[2] // 2, )                                       # (the same bytes a row)
+	rowops.test_groupnorm(bnd, dtype, shape, groups // 2 if dtype == np.float32 else groups, "silu")
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("shape,groups", LARGE)
+@pytest.mark.parametrize("name", ["relu", "silu"])
+def test_groupnorm_backward_large_slabs(bnd, dtype, shape, groups, name):
+	if dtype == np.float32:
+		shape = shape[:2] + (shape[2] // 2, )
+	rowops.test_groupnorm_backward(bnd, dtype, shape, groups // 2 if dtype == np.float32 else groups, name)
+
+
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("shape,groups", NORMS)
+def test_groupnorm_backward_gelu(bnd, dtype, shape, groups):
+	rowops.test_groupnorm_backward(bnd, dtype, shape, groups, "gelu")
+
+
+# rows of all channels that no workgroup holds, next to the ones that one just does: float32 above 1024 channels, float16 above 2048
+@pytest.mark.parametrize("dtype", [np.float32, np.float16])
+@pytest.mark.parametrize("shape,groups", [((2, 70, 1024), 1), ((1, 90, 1028), 1), ((2, 400, 1280), 32), ((1, 50, 2056), 1), ((2, 300, 2560), 32), ((3, 40, 4096), 1)])
+def test_groupnorm_many_channels(bnd, dtype, shape, groups):
+	rowops.test_groupnorm(bnd, dtype, shape, groups, "silu")
+	rowops.test_groupnorm_backward(bnd, dtype, shape, groups, "silu")
 
 
 # ------------------------------------------------------------------------------------------------ streams

@@ -121,6 +121,7 @@ struct Product {
 	float *slabs;                    // partial sums [split][m][slab_n] when splits > 1
 	int slab_n;                      // n up to whole runs
 	long lda, ldb;
+	int reach_a, reach_b;            // stored rows within 32 bits of a tile's start (reach_of)
 	int m, n, k;
 	int tiles_m, tiles_n, splits, ksteps_per_split;
 	size_t a_bytes, b_bytes;         // extents of the operands
@@ -248,10 +249,9 @@ struct Stage {
 	}
 	__device__ __forceinline__ static int spot(int r) { return r >> 1 & 7; }
 
-	// a byte offset as the buffer instructions take it. Every row of the operand lies within 32 bits of its tile's start (check_reach); a row
-	// that does not is one behind the last, of which a tile of few rows has many: past every buffer's end, it reads as zeros
+	// past every buffer's end: zeros. Of a tile's stored rows the first `reach` lie within 32 bits of its start, the operand's own among
+	// them (check_reach); the others, of which a tile of few rows has many, must not wrap onto those.
 	static constexpr unsigned NOWHERE = 0xfffffff0u;
-	__device__ __forceinline__ static unsigned reached(size_t offset) { return offset < 0xfffff000u ? (unsigned)offset : NOWHERE; }
 
 	long bytes, step;                // what is left of the operand from the next tile on (negative: nothing); advance per tile
 	const char *p;                   // the next tile
@@ -259,22 +259,24 @@ struct Stage {
 	unsigned off[PIECES];            // a lane's byte offsets from there
 	int kpiece[PIECES];              // KMAJOR = false: first k of the lane's pieces
 
-	__device__ __forceinline__ void init(const void *src, size_t extent, long ld, int row0, int kbeg, int wave, int lane) {
+	__device__ __forceinline__ void init(const void *src, size_t extent, long ld, int reach, int row0, int kbeg, int wave, int lane) {
 		const size_t start = KMAJOR ? ((size_t)kbeg * ld + row0) * SIZE : ((size_t)row0 * ld + kbeg) * SIZE;
 		p = (const char *)src + start;
 		bytes = (long)(extent - start);
 		step = KMAJOR ? HK * ld * SIZE : HK * SIZE;
 		shift = KMAJOR ? RUN * SIZE : RUN * ld * SIZE;
+		const unsigned pitch = (unsigned)ld * SIZE;
 #pragma unroll
 		for (int i = 0; i < PIECES; ++i) {
 			const int o = ((wave * PIECES + i) * 64 + lane) * 16;                // place in the LDS tile
 			if (KMAJOR) {
 				const int k = o / (ROWS * SIZE), at = o % (ROWS * SIZE) / 16, q = ((at / SIZE) ^ turn(k)) * 16 + at % SIZE * C;
-				off[i] = reached(((size_t)k * ld + (q / RUN * (2 * RUN) + q % RUN)) * SIZE);
+				off[i] = k < reach ? k * pitch + (q / RUN * (2 * RUN) + q % RUN) * SIZE : NOWHERE;
 			} else {
 				const int q = o / 128, piece = (o / 16 % 8) ^ spot(q);
 				kpiece[i] = piece * C;
-				off[i] = reached((size_t)(q / RUN * (2 * RUN) + q % RUN) * ld * SIZE + piece * 16);
+				const int row = q / RUN * (2 * RUN) + q % RUN;
+				off[i] = row < reach ? row * pitch + piece * 16 : NOWHERE;
 			}
 		}
 	}
@@ -365,8 +367,8 @@ __global__ void __launch_bounds__(64 * WM * WN) linear_kernel(Product g) {
 
 	SA sa;
 	SB sb;
-	sa.init(g.a, g.a_bytes, g.lda, m0, kbeg, wave, lane);
-	sb.init(g.b, g.b_bytes, g.ldb, n0, kbeg, wave, lane);
+	sa.init(g.a, g.a_bytes, g.lda, g.reach_a, m0, kbeg, wave, lane);
+	sb.init(g.b, g.b_bytes, g.ldb, g.reach_b, n0, kbeg, wave, lane);
 	const unsigned at = lds_address(lds);
 	auto ask_a = [&](int tile, int half, int i) {
 		sa.issue(i, at + ((tile & 1) * TILE + half * SA::VALUES) * (int)sizeof(T), kbeg + tile * HK, kend, wave, half);
@@ -543,6 +545,8 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 		for (int row = row0 + wave; row < row1; row += 4) {
 			float d[COUNT];
 			load_run((const T *)g.dy + (size_t)row * g.lddy + col, whole, left, d);
+			// (the words while the loads are on their way: 256 x 1000 float32 2 us)
+			const unsigned bits = g.dropping ? drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col) : ~0u;
 			if (g.act != PZ_ACT_NONE) {
 				float z[COUNT];
 				load_run((const T *)g.preact + (size_t)row * g.ldp + col, whole, left, z);
@@ -551,11 +555,8 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 					for (int e = 0; e < COUNT; ++e) d[e] *= act_slope(z[e], act);
 				});
 			}
-			if (g.dropping) {                                            // (last: nothing comes through a dropped element, whatever dy and z hold)
-				const unsigned bits = drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col);
 #pragma unroll
-				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] : 0.f;
-			}
+			for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] : 0.f;      // (last: nothing comes through a dropped element, whatever dy and z hold)
 #pragma unroll
 			for (int e = 0; e < COUNT; ++e) sum[e] += d[e], d[e] *= g.held;
 			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)
@@ -662,12 +663,18 @@ void launch(const Plan &p, const Product &g, bool ta, bool tb, dim3 grid, hipStr
 	else launch<T, false, false>(p, g, grid, st);
 }
 
+// how many rows of a pitch of ld elements a 32-bit byte offset reaches whole
+int reach_of(long ld, int size) {
+	const long rows = 0xfffff000l / size / ld;
+	return rows < 0x7fffffff ? (int)rows : 0x7fffffff;
+}
+
 // a lane's place in a tile is a 32-bit offset from the tile's start: of up to bm rows where k runs along a row, of bk steps elsewhere
 int check_reach(int dtype, const Operands &o, const char *who) {
 	const Plan p = plan_product(dtype, o);
 	auto reach = [&](bool copied, long ld, bool kmajor, int rows, int block) {
 		const long held = kmajor ? (o.k < p.bk ? o.k : p.bk) : (rows < block ? rows : block);
-		return held * (copied ? padded(kmajor ? rows : o.k) : ld) <= 0xfffff000l / (dtype == PZ_F16 ? 2 : 4);
+		return held <= reach_of(copied ? padded(kmajor ? rows : o.k) : ld, dtype == PZ_F16 ? 2 : 4);
 	};
 	PZ_REQUIRE(o.m == 0 || o.n == 0 || (reach(p.copy_a, o.lda, o.ta, o.m, p.bm) && reach(p.copy_b, o.ldb, !o.tb, o.n, p.bn)),
 	           "%s: rows of %ld and %ld elements are too far apart", who, o.lda, o.ldb);
@@ -696,7 +703,7 @@ int product(int dtype, Operands o, const Epilogue &epi, char *ws, hipStream_t st
 	}
 
 	Product g;
-	g.a = o.a, g.b = o.b, g.lda = o.lda, g.ldb = o.ldb;
+	g.a = o.a, g.b = o.b, g.lda = o.lda, g.ldb = o.ldb, g.reach_a = reach_of(o.lda, size), g.reach_b = reach_of(o.ldb, size);
 	g.slabs = (float *)(ws + p.a_bytes + p.b_bytes);
 	g.m = o.m, g.n = o.n, g.k = o.k, g.slab_n = padded(o.n);
 	g.tiles_m = p.tiles_m, g.tiles_n = p.tiles_n, g.splits = p.splits, g.ksteps_per_split = p.ksteps_per_split;

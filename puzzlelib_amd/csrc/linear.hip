@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 				load_run((const T *)g.preact + (size_t)row * g.ldp + col, whole, left, z);
 				with_act(g.act, [&](auto act) {
 #pragma unroll
-					for (int e = 0; e < COUNT; ++e) d[e] *= act_slope(z[e], act);
+					for (int e = 0; e < COUNT; ++e) d[e] *= act_slope<true>(z[e], act);      // (a z beyond its type was stored as an infinity)
 				});
 			}
 #pragma unroll

@@ -42,15 +42,19 @@ __device__ __forceinline__ float act_value(float z, int act) {
 	return z;
 }
 
+// INF: z may be infinite, where the slopes are 0 and 1 and z times nothing is not; from 100 on they are that in float32. (The median forgets a
+// NaN, the exponential beside it does not.)
+template <bool INF = false>
 __device__ __forceinline__ float act_slope(float z, int act) {
+	const float f = INF ? __builtin_amdgcn_fmed3f(z, -100.f, 100.f) : z;
 	if (act == PZ_ACT_RELU) return z > 0.f ? 1.f : 0.f;
 	if (act == PZ_ACT_GELU) {
 		const float e = exp_of(-0.5f * z * z), q = normal_tail(fabsf(z), e);
-		return fmaf(z * 0.39894228040143268f, e, z < 0.f ? q : 1.f - q);
+		return fmaf(f * 0.39894228040143268f, e, z < 0.f ? q : 1.f - q);
 	}
 	if (act == PZ_ACT_SILU) {
 		const float s = __builtin_amdgcn_rcpf(1.f + exp_of(-z));
-		return s * fmaf(z, 1.f - s, 1.f);
+		return s * fmaf(f, 1.f - s, 1.f);
 	}
 	return 1.f;
 }

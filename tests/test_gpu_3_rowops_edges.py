@@ -61,6 +61,27 @@ def test_gradients_at_the_end_of_float16(bnd, name, p, top):
 	within(db.get(), dz.sum(axis=0), off.sum(axis=0) + (m + 4) * U32 * np.abs(dz).sum(axis=0), "db")
 
 
+@pytest.mark.parametrize("name", ["relu", "gelu", "silu"])
+def test_pre_activations_beyond_float16(bnd, name):
+	"""x W + b beyond 65504 either way: what the forward pass leaves is infinite, the output below is 0 and so is the slope; above it is 1"""
+	m, k, n = 8, 16, 24
+	x, W = np.full((m, k), 250.0, np.float16), np.full((k, n), 30.0, np.float16)
+	W[:, ::2] = -30.0                                                              # z = +-120000
+	y, z = bnd.blas.linear(gpu(bnd, x), gpu(bnd, W), act=bnd.FusedAct[name], preact=True)
+	assert np.isneginf(z.get()[:, ::2]).all() and np.isposinf(z.get()[:, 1::2]).all() and np.all(y.get()[:, ::2] == 0)
+	dy = np.random.RandomState(35).randn(m, n).astype(np.float16)
+	dx, dW, db = bnd.blas.linearBackward(gpu(bnd, dy), gpu(bnd, x), gpu(bnd, W), act=bnd.FusedAct[name], preact=z)
+	dz = np.where(np.arange(n) % 2 == 1, dy.astype(np.float64), 0.0)
+	stored = 2.0 ** -11 * np.abs(dz) + 2.0 ** -24
+	W64, x64 = W.astype(np.float64), x.astype(np.float64)
+	within(dx.get(), dz @ W64.T, productBound(dz, W64.T, n) + stored @ np.abs(W64.T), "dx")
+	within(dW.get(), x64.T @ dz, productBound(x64.T, dz, m) + np.abs(x64.T) @ stored, "dW")
+	within(db.get(), dz.sum(axis=0), (m + 4) * U32 * np.abs(dz).sum(axis=0), "db")
+	# NaN is not taken for either
+	nan = gpu(bnd, np.full((m, n), np.nan, np.float16))
+	assert name == "relu" or np.isnan(bnd.blas.linearBackward(gpu(bnd, dy), gpu(bnd, x), gpu(bnd, W), act=bnd.FusedAct[name], preact=nan)[2].get()).all()
+
+
 @pytest.mark.parametrize("dtype", [np.float32, np.float16])
 def test_a_mask_of_p_0_keeps_everything(bnd, dtype):
 	"""word 1979 of call 117436 of seed 2026 is 2^32 - 1, the one word that does not lie below the threshold of p = 0"""

@@ -221,7 +221,7 @@ class BlasContext:
 		"""out = residual + dropout(act(data W + bias)) in one product (float32 or float16 tensors, float32 sums and bias): what
 		Linear, Activation, Dropout and Add do one after the other (Modules/Linear.py:36-41, Activation.py:52-55, Dropout.py:33-58,
 		Add.py:15-22). data is (..., k) in rows of one pitch, W (k, n), or (n, k) with transpW. `preact`: an array for
-		data W + bias (linearBackward needs it behind an activation), or True to have one made; the call then returns (out, preact).
+		data W + bias (linearBackward needs it behind an activation), or True to have one made (None or False: not kept); the call then returns (out, preact).
 		`out` may be `residual` (in place). A float16 product keeps apart from the package's launches on other streams, user kernels
 		(SourceModule) among them; what a program launches by other means is its own to order."""
 		plan = self.linearPlan("linear", data, W, transpW, act, False)
@@ -236,7 +236,9 @@ class BlasContext:
 			plan = self.linearOperand("linear: out", out, shape, dtype, plan, "ldy", n)
 			inplace = residual is not None and lazy.sameBuffer(out, residual) and out.strides == residual.strides
 			requireDisjoint("linear: out", out, data, W, bias, None if inplace else residual)
-		if preact is True:
+		if preact is False:
+			preact = None
+		elif preact is True:
 			preact = GPUArray.empty(shape, dtype=dtype, allocator=allocator)
 		elif preact is not None:
 			plan = self.linearOperand("linear: preact", preact, shape, dtype, plan, "ldp", n)

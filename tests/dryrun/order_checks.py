@@ -217,6 +217,16 @@ def streams():
 				order.follows(since, foreign[-1 if array is target else 0])         # (a reduction reads in its first launch)
 
 
+def preact_is_a_choice():
+	"""preact=False is what it says, as None is"""
+	x, W = A(4, 16), A(16, 8)
+	for preact in (None, False):
+		lib.trace.clear()
+		assert bnd.blas.linear(x, W, preact=preact).shape == (4, 8)
+	out, z = bnd.blas.linear(x, W, preact=True)
+	assert out.shape == z.shape == (4, 8)
+
+
 if __name__ == "__main__":
 	globals()[sys.argv[1]]()
 	print("OK")

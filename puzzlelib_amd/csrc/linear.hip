@@ -555,8 +555,10 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 					for (int e = 0; e < COUNT; ++e) d[e] *= act_slope<true>(z[e], act);      // (a z beyond its type was stored as an infinity)
 				});
 			}
+			if (g.dropping) {                                            // (last: nothing comes through a dropped element, whatever dy and z hold)
 #pragma unroll
-			for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] : 0.f;      // (last: nothing comes through a dropped element, whatever dy and z hold)
+				for (int e = 0; e < COUNT; ++e) d[e] = bits >> e & 1u ? d[e] : 0.f;
+			}
 #pragma unroll
 			for (int e = 0; e < COUNT; ++e) sum[e] += d[e], d[e] *= g.held;
 			if (g.dz) store_run((T *)g.dz + (size_t)row * g.lddz + col, true, COUNT, d);     // (pitch of 8s: what lies beyond n are the zeros loaded)

@@ -51,6 +51,7 @@ class DnnContext:
 		self.sideStream = None
 		self.sideLaunches = 0
 		self.earlyReady = None       # (event, gradient allocation, data allocation, their versions): see convNdBackwardData
+		self.earlyReleases = 0       # ... and how many blocks had been given back by then
 		self.poolBnCache = {}
 		self.packCache = weakref.WeakKeyDictionary()        # allocation of a filter -> {(offset, pass, algo, geometry): PackEntry}
 		self.packEpoch = lib.modeEpoch
@@ -541,7 +542,7 @@ class DnnContext:
 			return
 		event = lazy.newEvent()
 		event.record(None)
-		self.earlyReady = (event, groot, droot, glz.version, dlz.version)
+		self.earlyReady, self.earlyReleases = (event, groot, droot, glz.version, dlz.version), driver.MemoryPool.releases
 
 
 	# ---- filter gradients on a side stream. Backward-data and backward-filter of a layer read the same incoming gradient
@@ -651,7 +652,9 @@ class DnnContext:
 		mark = None
 		if side is not None and early is not None and not folded and xbn is None and not fresh and grad.gpudata.root is early[1] and \
 				data.gpudata.root is early[2] and lazy.cleanSince(early[1], early[3]) and lazy.cleanSince(early[2], early[4]) and \
-				all(lazy.quiet(a) for a in writes):          # (a settle — a pending zero fill of the arena — would be behind the mark)
+				all(lazy.quiet(a) for a in writes) and driver.MemoryPool.releases == self.earlyReleases:
+			# (a settle — a pending zero fill of the arena — would be behind the mark, and so may be the launches that used memory
+			# given back since, which the workspace below could be)
 			mark = early[0]
 			lazy.count("wgrad_early_start")
 

@@ -298,6 +298,9 @@ class MemoryPool:
 	frontPerClass = 64
 	pools = weakref.WeakSet()
 
+	releases = 0               # blocks given back so far, by all pools: whoever takes memory for a launch that runs in front of what the
+	                           # main stream was given last (DnnContext.convNdBackwardParams) must not take any of it
+
 	def __init__(self):
 		handle = c_void_p()
 		lib.pz_pool_create(byref(handle))
@@ -354,6 +357,7 @@ class MemoryPool:
 	def release(self, ptr, nbytes=None):
 		if self.handle is None:
 			return
+		MemoryPool.releases += 1
 		if nbytes is not None and self.holding and self.frontBytes < self.frontLimit:
 			cls = self.classSize(nbytes)
 			with self.lock:

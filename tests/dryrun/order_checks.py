@@ -227,6 +227,36 @@ def preact_is_a_choice():
 	assert out.shape == z.shape == (4, 8)
 
 
+def filter_gradient_behind_a_row_operator():
+	"""A filter gradient may start at the mark in front of its layer's backward-data kernel, earlier than where it is called. Its workspace may
+	be memory that an operator called in between has just given back, so it follows that operator."""
+	f = np.float32
+	dnn, conv = bnd.dnn, lambda: (A(8, 16, 12, 12), A(32, 16, 3, 3), A(8, 32, 10, 10))
+	x, W, g = conv()
+	wgrad, bgrad = A(32, 16, 3, 3), A(32)
+	rows, V, norm, stat = A(6, 8), A(8, 10), A(2, 5, 12), A(2, 3)
+	between = {
+		"pz_linear_fwd": lambda: bnd.blas.linear(rows, V), "pz_linear_bwd": lambda: bnd.blas.linearBackward(A(6, 10), rows, V),
+		"pz_groupnorm_fwd": lambda: dnn.groupNormNd(norm, None, None, 3),
+		"pz_groupnorm_bwd": lambda: dnn.groupNormNdBackward(norm, norm, None, None, stat, stat, 3),
+		"pz_dropout": lambda: bnd.counterDropoutKer(f)(A(6, 8), rows, bnd.DropoutMask(1, 2, 0.5)),
+	}
+	for entry in (None, ) + tuple(between):
+		order = watched()
+		taken = lazy.counters.get("wgrad_early_start", 0)
+		ingrad = dnn.convNdBackwardData(g, W, data=x)
+		if entry is not None:
+			between[entry]()
+		dnn.convNdBackwardParams(x, g, W, withbias=True, wgrad=wgrad, bgrad=bgrad, momentum=1.0)
+		del ingrad
+		filters = [i for i, (n, s) in enumerate(order.launches) if n.startswith("pz_conv2d_bwd_filter")][-1]
+		assert order.launches[filters][1] is not None, "no second stream: nothing is tested"
+		if entry is None:
+			assert lazy.counters["wgrad_early_start"] == taken + 1, "no early start: nothing is tested"
+		else:
+			order.follows(filters, order.only(entry))
+
+
 if __name__ == "__main__":
 	globals()[sys.argv[1]]()
 	print("OK")

@@ -11,7 +11,7 @@ from conftest import ROOT
 SCRIPT = os.path.join(ROOT, "tests", "dryrun", "order_checks.py")
 
 
-@pytest.mark.parametrize("check", ["collectives", "collective_out_of_a_barrier", "float32_needs_no_order", "streams", "preact_is_a_choice"])
+@pytest.mark.parametrize("check", ["collectives", "collective_out_of_a_barrier", "float32_needs_no_order", "streams", "preact_is_a_choice", "filter_gradient_behind_a_row_operator"])
 def test_order(check):
 	env = dict(os.environ, PUZZLE_MI355_DRYRUN="1", PUZZLE_MI355_LAZY="1")
 	env.pop("PUZZLE_MI355_DEBUG_ALLOC", None)

@@ -7,7 +7,7 @@
 namespace {
 
 // 16 bytes of T a lane: COUNT consecutive elements, so a lane evaluates whole quads of the generator. Bound by memory: 8192 x 8192 float16
-// with a residual 68 us (402 MB, 5.9 TB/s); 256 x 1024 float32 2.5 us, the launch.
+// with a residual 70 us (402 MB, 5.7 TB/s); 256 x 1024 float32 2.5 us, the launch.
 template <typename T>
 __global__ void __launch_bounds__(256) dropout_kernel(const T *x, const T *residual, T *y, size_t count, DropKey key, int dropping, int vec) {
 	constexpr int COUNT = 16 / sizeof(T);

@@ -337,7 +337,7 @@ __device__ __forceinline__ void multiply_add(f32x4 (&acc)[N], const f32x4 &a, co
 }
 
 // Bound by the matrix pipe: float16 8192 x 8192 x 2048 with dropout and residual 235 us (1170 TFLOP/s), 8192 x 2048 x 8192 with GELU and the
-// kept pre-activation 275 us (1000; the epilogue writes 268 MB and evaluates 65536 GELUs a CU), float32 4096^3 with ReLU and residual 958 us
+// kept pre-activation 279 us (985; the epilogue writes 268 MB and evaluates 65536 GELUs a CU), float32 4096^3 with ReLU and residual 958 us
 // (143 TFLOP/s). Single rows are bound by the weights: 1 x 4096 x 16384 float16 23-25 us (5.4 TB/s), then the join.
 template <typename T, int BM, int BN, int WM, int WN, bool TA, bool TB>
 __global__ void __launch_bounds__(64 * WM * WN) linear_kernel(Product g) {
@@ -514,7 +514,7 @@ __global__ void __launch_bounds__(256) linear_align_kernel(Aligned a, Aligned b,
 // what is missing, in float32. So without an activation nothing is rounded (a dropped dy is dy or zero), and behind one dz carries one
 // rounding: half a step of 2^-11 relative (8192 x 2048 x 8192 with GELU: dx 2.9e-4 off the 64-bit result, root mean square, where 2.1e-4 is
 // the rounding of dx itself), or 2^-25 absolute where it is below 2^-14, as far as dy can be off. A second product with what the rounding
-// left would double the pass: 505 us.
+// left would double the pass: 507 us.
 float held_part(int dtype, int act) { return dtype == PZ_F16 && (act == PZ_ACT_GELU || act == PZ_ACT_SILU) ? 0.875f : 1.f; }      // (slopes up to 1.13)
 
 struct Gate {
@@ -528,7 +528,7 @@ struct Gate {
 };
 
 // block = 4 waves x (64 lanes x 16 bytes of columns), rows dealt out over the waves. Once for both products, which read dz several times
-// over; bound by its bytes: 8192 x 8192 float16 with GELU 87 us (402 MB, 4.6 TB/s).
+// over; bound by its bytes: 8192 x 8192 float16 with GELU 90 us (402 MB, 4.5 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 	constexpr int COUNT = 16 / sizeof(T);
@@ -624,7 +624,7 @@ Plan plan_product(int dtype, const Operands &o) {
 	p.bk = dtype == PZ_F16 ? kSteps<f16> : kSteps<float>;
 	p.bm = o.m > 64 ? 128 : 64, p.bn = o.n > 64 ? 128 : 64;
 	// narrower tiles where square ones give a CU one workgroup at most (2048^3: float16 33 -> 30 us, float32 147 -> 137; 4096 x 512 x 512
-	// 23 -> 13), or half of one where the reduction runs over rows (dW of 2048 x 1024 x 4096: 65 us both ways instead of 69)
+	// 27 -> 13), or half of one where the reduction runs over rows (dW of 2048 x 1024 x 4096: 65 us both ways instead of 69)
 	if (p.bm == 128 && (long)pz::ceil_div(o.m, 128) * pz::ceil_div(o.n, 128) <= pz::kNumCU / (o.ta ? 2 : 1)) p.bn = 64;
 	const long tiles256 = (long)pz::ceil_div(o.m, 256) * pz::ceil_div(o.n, 256);
 	if (o.k >= (dtype == PZ_F16 ? 256 : 1024) && tiles256 >= pz::kNumCU) p.bm = p.bn = 256;

@@ -566,7 +566,7 @@ int pz_dropout(int dtype, const void *x, const void *residual, void *y, size_t c
  * preact receives x W + b, which the backward pass of an activation needs. y may be residual, nothing else may overlap.
  * The backward pass: dz = act'(preact) * dropout(dy); dx = dz W^T; dW <- beta dW + alpha x^T dz (Modules/Linear.py:44-54's contract,
  * float32 or the operands' type); db <- beta db + alpha * column sums of dz. NULL outputs are not computed; the residual's gradient is
- * dy itself. In float16 dz is rounded to float16 behind an activation, in front of the two products (the matrix pipe's operand type);
+ * dy itself. In float16 dz is rounded to float16 behind GELU and SiLU, in front of the two products (the matrix pipe's operand type);
  * its 1 / (1 - p) comes behind them, so that dz has room for any dy.                                                                  */
 typedef struct pz_linear_desc {
 	int dtype, act, trans_w;

@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(256) linear_align_kernel(Aligned a, Aligned b,
 // dz is held in the operands' type, the only one that the matrix instructions of the two products take at their full rate; db sums it before
 // that rounding. In float16 it is held as dz * held_part * (1 - p), which dy's own range always has room for: 1 / (1 - p) and an activation's
 // slope above 1 would take dz = 65504 / (1 - p) * 1.13 to infinity although dx and dW are in range. The products' sums are multiplied by
-// what is missing, in float32. So without an activation nothing is rounded (a dropped dy is dy or zero), and behind one dz carries one
+// what is missing, in float32. So without a curved activation nothing is rounded (dy or zero), and behind GELU or SiLU dz carries one
 // rounding: half a step of 2^-11 relative (8192 x 2048 x 8192 with GELU: dx 2.9e-4 off the 64-bit result, root mean square, where 2.1e-4 is
 // the rounding of dx itself), or 2^-25 absolute where it is below 2^-14, as far as dy can be off. A second product with what the rounding
 // left would double the pass: 507 us.
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(256) linear_gate_kernel(Gate g) {
 		for (int row = row0 + wave; row < row1; row += 4) {
 			float d[COUNT];
 			load_run((const T *)g.dy + (size_t)row * g.lddy + col, whole, left, d);
-			// (the words while the loads are on their way: 256 x 1000 float32 2 us)
+			// (the words are drawn while the loads are on their way)
 			const unsigned bits = g.dropping ? drop_bits<COUNT>(g.drop, (uint64_t)row * g.n + col) : ~0u;
 			if (g.act != PZ_ACT_NONE) {
 				float z[COUNT];
